@@ -58,9 +58,7 @@ __device__ __forceinline__ float emit_weight_bound(const GatherGemmParams& p, in
 typedef float emit_f2 __attribute__((ext_vector_type(2)));
 typedef _Float16 emit_h2 __attribute__((ext_vector_type(2)));
 
-// Activation, scale and fp16 pair split of 4 values, two at a time on the packed fp32 / packed-convert instructions
-// (v_pk_mul_f32, v_cvt_pk_f16_f32, v_pk_add_f32: ~7 VALU operations per value where the scalar form took 16 -- the
-// emitting epilogues of the 64-channel layers had become a third slower than the plain ones).  `up` = the consumer's
+// Activation, scale and fp16 pair split of 4 values, two at a time (packed converts, v_cvt_pk_f16_f32).  `up` = the consumer's
 // scale, or 0 for a row that must not count; vmaxs accumulates max |activation * up| BEFORE the clamp, so
 // emit_finish can tell both the magnitude (vmaxs / up, exact: a power of two) and whether anything left the fp16 window.
 // Value for value what pair_image_kernel<true> (image.hip) computes: RN(a), RN(a - RN(a)), clamp to +-65504.

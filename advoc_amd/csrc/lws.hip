@@ -230,8 +230,7 @@ static_assert(kSweepFrames >= 8, "tile_work is sized for tiles of at least 8 fra
 //   sum_p alpha_q(p) (-i)^(q (f + p)) x[f + p] = (-i)^(q f) * sum_c (-i)^(q c) * [ sum_{p = c mod 4} alpha_q(p) x[f + p] ]
 // -- compile-time quarter turns on the four class sums, one per-thread unit factor rot[q] = (-i)^(q f) per row.
 typedef float f2v __attribute__((ext_vector_type(2)));
-// c += al * x (complex) as TWO packed instructions: v_pk_fma_f32 takes the scalar weight, the half swap and the sign flip
-// as operand modifiers
+// c += al * x (complex) as two 2-wide multiply-adds
 __device__ __forceinline__ void cmac(f2v& c, float2 al, f2v x) {
   c = __builtin_elementwise_fma((f2v){al.x, al.x}, x, c);
   c = __builtin_elementwise_fma((f2v){-al.y, al.y}, __builtin_shufflevector(x, x, 1, 0), c);

@@ -6,10 +6,9 @@
 //
 // Mapping to the hardware
 //   * one wavefront = TWO consecutive frames of one clip at a time, carried in the two halves of
-//     2-wide fp32 vectors so that every butterfly / twiddle multiply is one packed instruction
-//     (v_pk_add_f32 / v_pk_mul_f32 / v_pk_fma_f32) for both frames: the kernel is bound by VALU
-//     issue (a 1024-point FFT per 3 KB of traffic), not by HBM, so halving the instruction count
-//     per frame is what moves it up the bandwidth roofline.
+//     2-wide fp32 vectors: two independent chains per butterfly / twiddle multiply.  The kernel is
+//     bound by VALU issue (a 1024-point FFT per 3 KB of traffic), not by HBM.  (The vectors were laid
+//     out for packed fp32 instructions; the library is built without those, see the Makefile.)
 //   * The 1024-point real FFT is a 512-point complex FFT (z[n] = x[2n] + i x[2n+1]) held 8 complex
 //     values per lane, computed as three radix-8 passes (512 = 8*8*8); the two inter-pass
 //     transposes go through a private, bank-conflict-free LDS plane per wave (no workgroup
@@ -505,8 +504,6 @@ __global__ __launch_bounds__(kWaves * 64) void stft1024_hop256_kernel(
 //     magnitudes at the end are one packed multiply-add per two bins);
 //   * the pass twiddles are applied on the way IN to the next pass, inside its first butterflies: with y = t x4,
 //     s = x0 + y and d = 2 x0 - s are six multiply-adds where twiddle + add + subtract are eight.
-// The swizzled packed operations (x (-i), complex products) are inline assembly: the compiler builds them from v_mov / v_xor.
-#define ADVOC_PK_ADD(D, A, B, MODS) asm("v_pk_add_f32 %0, %1, %2 " MODS : "=v"(D) : "v"(A), "v"(B))
 // forward 8-point DFT of complex values held as (re, im) pairs; v[a] <- sum_a v[a] exp(-2 pi i a p / 8)
 __device__ __forceinline__ void dft8_cp(f2 (&v)[8]) {
   const float h = 0.70710678118654752440f;
@@ -517,28 +514,22 @@ __device__ __forceinline__ void dft8_cp(f2 (&v)[8]) {
     d[n] = v[n] - v[n + 4];
   }
   {  // d[n] *= W8^n (d[2] x (-i) is folded into its consumers)
-    f2 u;
-    ADVOC_PK_ADD(u, d[1], d[1], "op_sel:[0,1] op_sel_hi:[1,0] neg_hi:[0,1]");            // (dr + di, di - dr)
-    d[1] = u * h;
-    ADVOC_PK_ADD(u, d[3], d[3], "op_sel:[1,0] op_sel_hi:[0,1] neg_lo:[0,1] neg_hi:[1,1]");   // (di - dr, -dr - di)
-    d[3] = u * h;
+    d[1] = (f2){d[1].x + d[1].y, d[1].y - d[1].x} * h;
+    d[3] = (f2){d[3].y - d[3].x, -d[3].x - d[3].y} * h;
   }
   {  // even outputs: 4-point DFT of s
     const f2 b0 = s[0] + s[2], b2 = s[0] - s[2], b1 = s[1] + s[3];
-    f2 b3;
-    ADVOC_PK_ADD(b3, s[1], s[3], "op_sel:[1,1] op_sel_hi:[0,0] neg_lo:[0,1] neg_hi:[1,0]");  // (s1 - s3) x (-i)
+    const f2 b3 = {s[1].y - s[3].y, s[3].x - s[1].x};   // (s1 - s3) x (-i)
     v[0] = b0 + b1; v[4] = b0 - b1; v[2] = b2 + b3; v[6] = b2 - b3;
   }
   {  // odd outputs: 4-point DFT of (d0, d1, d2 x (-i), d3)
-    f2 b0, b2, b3;
-    ADVOC_PK_ADD(b0, d[0], d[2], "op_sel:[0,1] op_sel_hi:[1,0] neg_hi:[0,1]");              // d0 + d2 x (-i)
-    ADVOC_PK_ADD(b2, d[0], d[2], "op_sel:[0,1] op_sel_hi:[1,0] neg_lo:[0,1]");              // d0 - d2 x (-i)
+    const f2 b0 = {d[0].x + d[2].y, d[0].y - d[2].x};   // d0 + d2 x (-i)
+    const f2 b2 = {d[0].x - d[2].y, d[0].y + d[2].x};   // d0 - d2 x (-i)
     const f2 b1 = d[1] + d[3];
-    ADVOC_PK_ADD(b3, d[1], d[3], "op_sel:[1,1] op_sel_hi:[0,0] neg_lo:[0,1] neg_hi:[1,0]");
+    const f2 b3 = {d[1].y - d[3].y, d[3].x - d[1].x};
     v[1] = b0 + b1; v[5] = b0 - b1; v[3] = b2 + b3; v[7] = b2 - b3;
   }
 }
-#undef ADVOC_PK_ADD
 
 // forward 8-point DFT of x[a] = t[a] v[a] (t[0] = 1), frame-packed; TW(a) gives t[a] as float2 {re, im}
 template <typename TW>
