@@ -60,6 +60,26 @@ class ConvLayer(ctypes.Structure):
       ('dx1_amax', _p),
   ]
 
+class Rows(ctypes.Structure):
+  """struct advoc_rows (include/advoc_hip.h)."""
+  _fields_ = [('p', _p), ('pitch', _i64)]
+
+
+class ResidualNorm(ctypes.Structure):
+  """struct advoc_residual_norm (include/advoc_hip.h)."""
+  _fields_ = [
+      ('rows', _i64), ('cols', _i32), ('dtype', _i32), ('res_dtype', _i32),
+      ('norm_post', _i32), ('norm_pre', _i32), ('gate_act', _i32), ('gate_group', _i64),
+      ('w_post', _p), ('b_post', _p), ('scale', _p), ('w_pre', _p), ('b_pre', _p),
+      ('alpha', _f32), ('eps', _f32), ('keep_prob', _f32), ('accumulate', _i32),
+      ('seed', ctypes.c_uint64), ('offset', ctypes.c_uint64), ('seed_dev', _p),
+      ('h', Rows), ('x', Rows), ('gate', Rows), ('r', Rows), ('z', Rows), ('stats', _p),
+      ('dz', Rows), ('dr', Rows), ('dh', Rows), ('dx', Rows), ('dgate', Rows),
+      ('dw_post', _p), ('db_post', _p), ('dscale', _p), ('dw_pre', _p), ('db_pre', _p),
+      ('workspace', _p), ('workspace_bytes', _i64),
+  ]
+
+
 WGRAD_TABLE_BYTES = 262144      # ADVOC_WGRAD_TABLE_BYTES
 
 
@@ -118,6 +138,13 @@ PROTOTYPES = {
     'advoc_sigmoid_f32': (ctypes.c_int, [_p, _p, _i64, _p]),
     'advoc_zero_f32': (ctypes.c_int, [_p, _i64, _p]),
     'advoc_dropout_mask_u8': (ctypes.c_int, [_p, _i64, ctypes.c_uint64, ctypes.c_uint64, _f32, _p]),
+    'advoc_dropout': (ctypes.c_int, [_p, _i64, _p, _i64, _i64, _i64, _i32, _f32, ctypes.c_uint64, ctypes.c_uint64, _p, _p]),
+    'advoc_residual_norm_forward': (ctypes.c_int, [_p, _p]),
+    'advoc_residual_norm_workspace_bytes': (_i64, [_p]),
+    'advoc_residual_norm_backward': (ctypes.c_int, [_p, _p]),
+    'advoc_f8_quantize': (ctypes.c_int, [_p, _i64, _i64, _i64, _i32, _i32, _p, _p, _p, _p, _p]),
+    'advoc_matmul_nt_f8_workspace_bytes': (_i64, [_i64, _i64, _i64]),
+    'advoc_matmul_nt_f8': (ctypes.c_int, [_p, _p, _i32, _p, _p, _i32, _p, _i32, _i32, _i64, _i64, _i64, _p, _i64, _p]),
 }
 
 _lock = threading.Lock()

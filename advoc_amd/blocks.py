@@ -1,0 +1,356 @@
+"""Operators of residual blocks over the frames of a clip: dropout without a stored mask, the norms around a block with its
+gate and residual scale, and products of 8-bit block-scaled matrices, each with its gradients.
+
+Like ``conv.Layer`` this module only checks arguments and calls into libadvoc_hip.so (``include/advoc_hip.h`` holds the
+formulas); no arithmetic happens in Python/torch, and there is no CPU path.  Tensors live in HBM; fp32, bf16 and fp16 are
+taken, rows may be padded (unit stride inside a row, one distance between rows).  Every call is asynchronous on the current
+stream of the tensors' device and can be captured into a graph.
+
+  z, x8   = one block:   z = N_pre(x);  y = W z;  r = x + alpha * scale * gate * dropout(N_post(y));  next z = N_pre(r)
+
+  norm = blocks.ResidualNorm(cols, post='rms', pre='rms', w_post=..., scale=..., w_pre=..., keep_prob=0.9)
+  y = blocks.matmul_nt_f8(blocks.quantize_f8(z), w8, out_dtype=z.dtype)          # w8 = blocks.quantize_f8(w), once
+  r, z, stats = norm.forward(y, x, gate=gate, seed=step, save=True)
+  g = norm.backward(dz, dr, y, r, stats, gate=gate, seed=step)                   # g.dh is dL/dy, g.dx dL/dx
+  dy, dyt = blocks.quantize_f8_both(g.dh, 'e5m2')
+  dz = blocks.matmul_nt_f8(dy, w8t)                                              # w8t = blocks.quantize_f8_transposed(w)
+  dw = blocks.matmul_nt_f8(dyt, z8t)                                             # z8t = blocks.quantize_f8_transposed(z)
+"""
+import collections
+import ctypes
+
+import torch
+
+from advoc_amd import _lib
+
+NORMS = {'none': 0, 'rms': 1, 'layer': 2}
+GATE_ACTS = {'none': 0, 'sigmoid': 1}
+FORMATS = {'e4m3': 0, 'e5m2': 1}
+MAX_COLS = 16384
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_MASK64 = 2 ** 64 - 1
+
+
+def _choice(table, key, what):
+  try:
+    return table[key]
+  except (KeyError, TypeError):
+    raise _lib.AdvocHipError('{} {!r} is none of {}'.format(what, key, sorted(table)))
+
+
+def _dtype(t, name):
+  code = _DTYPES.get(t.dtype)
+  if code is None:
+    raise _lib.AdvocHipError('{} must be float32, bfloat16 or float16, got {}'.format(name, t.dtype))
+  return code
+
+
+def _rows(t, name, device=None):
+  """(address, rows, cols, elements from row to row) of a tensor as rows of its last dimension."""
+  if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    raise _lib.AdvocHipError('{} must be a torch tensor on a HIP device (no CPU path exists)'.format(name))
+  if device is not None and t.device != device:
+    raise _lib.AdvocHipError('{} is on {}, the other tensors on {}'.format(name, t.device, device))
+  if t.dim() == 0:
+    raise _lib.AdvocHipError('{} must have at least one dimension'.format(name))
+  cols = t.shape[-1]
+  if t.is_contiguous():
+    return t.data_ptr(), t.numel() // cols if cols else 0, cols, cols
+  rows, pitch, expect = 1, cols, None
+  for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    if size == 1:
+      continue
+    if expect is None:
+      pitch = stride
+    elif stride != expect:
+      raise _lib.AdvocHipError('{} (shape {}, strides {}) is not rows at one distance'.format(name, tuple(t.shape), t.stride()))
+    rows *= size
+    expect = stride * size
+  if cols > 1 and t.stride(-1) != 1 or rows > 1 and pitch < cols:
+    raise _lib.AdvocHipError('{} (shape {}, strides {}): a row must have unit stride and rows must not overlap'.format(
+        name, tuple(t.shape), t.stride()))
+  return t.data_ptr(), rows, cols, pitch
+
+
+def _seed_word(seed_dev, device):
+  if seed_dev is None:
+    return None
+  if not isinstance(seed_dev, torch.Tensor) or seed_dev.device != device or seed_dev.numel() != 1 or seed_dev.dtype not in (
+      torch.int64, torch.uint64):
+    raise _lib.AdvocHipError('seed_dev must be one int64 or uint64 on {}'.format(device))
+  return seed_dev.data_ptr()
+
+
+def _call(fn, what, device, *args):
+  """One library call on the current stream of `device`, with that device current."""
+  if device.index == torch.cuda.current_device():
+    rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+  else:
+    with torch.cuda.device(device):
+      rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+  if rc:
+    _lib.check(rc, what)
+
+
+def dropout(x, keep_prob, seed, offset=0, seed_dev=None, out=None):
+  """x / keep_prob where a counter-based generator keeps an element, 0 elsewhere (``advoc_dropout``): the same elements as the
+  mask ``advoc_dropout_mask_u8`` writes for (seed, offset), without the mask.  The gradient is the same call on dy with the
+  same numbers.
+
+  Element i (in logical order, whatever the strides) draws at offset + i: shards of a batch that pass their own offset (a
+  multiple of 4) drop what the whole batch would.  seed_dev: one int64 on the device, added to the seed by the kernel, for
+  graphs whose replays must not repeat a mask.  out: a tensor of x's shape and dtype, or x itself."""
+  px, rows, cols, pitch = _rows(x, 'x')
+  code = _dtype(x, 'x')
+  if out is None:
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    py, out_pitch = out.data_ptr(), cols
+  else:
+    py, _, _, out_pitch = _rows(out, 'out', x.device)
+    if out.shape != x.shape or out.dtype != x.dtype:
+      raise _lib.AdvocHipError('out must have the shape and dtype of x')
+  _call(_lib.load().advoc_dropout, 'advoc_dropout', x.device, px, pitch, py, out_pitch, rows, cols, code, keep_prob,
+        seed & _MASK64, offset & _MASK64, _seed_word(seed_dev, x.device))
+  return out
+
+
+ResidualNormGrads = collections.namedtuple('ResidualNormGrads',
+                                           ['dh', 'dx', 'dgate', 'dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre'])
+
+
+class ResidualNorm(object):
+  """The glue between two residual blocks (``advoc_residual_norm_forward / _backward``), per row of `cols` channels:
+
+    u = N_post(h) * w_post + b_post                   the norm behind the block that computed h
+    r = x + alpha * scale * act(gate) * dropout(u)    its gate, residual scale and dropout, and the residual sum
+    z = N_pre(r) * w_pre + b_pre                      the norm before the next block
+
+  post, pre: 'none' | 'rms' | 'layer'; gate_act: 'none' | 'sigmoid'.  The parameters are float32 [cols] tensors, each may be
+  None; they are read at every call, so in-place updates are seen.  h, gate and z have one dtype; x and r have that dtype or
+  float32."""
+
+  def __init__(self, cols, post='rms', pre='rms', gate_act='none', alpha=1.0, eps=1e-5, keep_prob=1.0, w_post=None,
+               b_post=None, scale=None, w_pre=None, b_pre=None):
+    if not 1 <= cols <= MAX_COLS:
+      raise _lib.AdvocHipError('cols must be 1 ... {}, got {}'.format(MAX_COLS, cols))
+    if not eps > 0 or not 0 < keep_prob <= 1:
+      raise _lib.AdvocHipError('eps must be positive and keep_prob in (0, 1]')
+    self.cols = cols
+    self.post, self.pre = _choice(NORMS, post, 'norm'), _choice(NORMS, pre, 'norm')
+    self.gate_act = _choice(GATE_ACTS, gate_act, 'gate activation')
+    self.alpha, self.eps, self.keep_prob = alpha, eps, keep_prob
+    self.w_post, self.b_post, self.scale, self.w_pre, self.b_pre = w_post, b_post, scale, w_pre, b_pre
+    if not self.post and (w_post is not None or b_post is not None) or not self.pre and (w_pre is not None or b_pre is not None):
+      raise _lib.AdvocHipError('a norm of kind none takes no weight or bias')
+
+  def _vector(self, t, name, device):
+    if t is None:
+      return None
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.float32 or t.shape != (self.cols,) or not (
+        t.is_contiguous()):
+      raise _lib.AdvocHipError('{} must be a contiguous float32 tensor of {} on {}'.format(name, self.cols, device))
+    return t.data_ptr()
+
+  def _bind(self, d, name, t, rows, device, dtype=None):
+    p, n, cols, pitch = _rows(t, name, device)
+    if n != rows or cols != self.cols:
+      raise _lib.AdvocHipError('{} has shape {}: {} rows of {} wanted'.format(name, tuple(t.shape), rows, self.cols))
+    if dtype is not None and t.dtype != dtype:
+      raise _lib.AdvocHipError('{} is {}, {} wanted'.format(name, t.dtype, dtype))
+    field = getattr(d, name)
+    field.p, field.pitch = p, pitch
+
+  def _descriptor(self, x, name, dtype, gate, seed, offset, seed_dev, has_h):
+    """What both directions share; x (r in the backward pass) sets rows, device and residual dtype."""
+    px, rows, cols, pitch = _rows(x, name)
+    if cols != self.cols:
+      raise _lib.AdvocHipError('{} has {} columns, {} wanted'.format(name, cols, self.cols))
+    device = x.device
+    d = _lib.ResidualNorm()
+    d.rows, d.cols, d.dtype, d.res_dtype = rows, cols, _DTYPES.get(dtype, -1), _dtype(x, name)
+    if d.dtype < 0 or d.res_dtype not in (d.dtype, 0):
+      raise _lib.AdvocHipError('{} is {}: it must be float32 or the dtype of the block ({})'.format(name, x.dtype, dtype))
+    d.norm_pre, d.alpha, d.eps, d.keep_prob = self.pre, self.alpha, self.eps, self.keep_prob
+    d.w_pre, d.b_pre = self._vector(self.w_pre, 'w_pre', device), self._vector(self.b_pre, 'b_pre', device)
+    if has_h:
+      d.norm_post, d.gate_act = self.post, self.gate_act
+      d.w_post, d.b_post = self._vector(self.w_post, 'w_post', device), self._vector(self.b_post, 'b_post', device)
+      d.scale = self._vector(self.scale, 'scale', device)
+      d.seed, d.offset, d.seed_dev = seed & _MASK64, offset & _MASK64, _seed_word(seed_dev, device)
+      if gate is not None:
+        p, n, cols, gate_pitch = _rows(gate, 'gate', device)
+        if cols != self.cols or gate.dtype != dtype or (rows % n if n else rows):
+          raise _lib.AdvocHipError('gate {} {} does not divide {} rows of {} {}'.format(
+              gate.dtype, tuple(gate.shape), rows, self.cols, dtype))
+        self._check_gate_shape(gate, x)
+        d.gate.p, d.gate.pitch, d.gate_group = p, gate_pitch, rows // n if n else 1
+    elif gate is not None:
+      raise _lib.AdvocHipError('a gate needs a block output h')
+    field = getattr(d, name)
+    field.p, field.pitch = px, pitch
+    return d, rows, device
+
+  def _check_gate_shape(self, gate, x):
+    """A gate has x's shape, with ones for trailing row dimensions that share it: [clips, 1, cols] for [clips, frames, cols]."""
+    lead, want = list(gate.shape[:-1]), list(x.shape[:-1])
+    if len(lead) == len(want):
+      i = 0
+      while i < len(lead) and lead[i] == want[i]:
+        i += 1
+      if all(n == 1 for n in lead[i:]):
+        return
+    raise _lib.AdvocHipError('gate of shape {} for rows of shape {}'.format(tuple(gate.shape), tuple(x.shape)))
+
+  def forward(self, h, x, gate=None, seed=0, offset=0, seed_dev=None, save=False, r=None, z=None):
+    """(r, z, stats).  h None: only z = N_pre(x), the norm before the first block (r is x).  z is None without a pre norm,
+    stats [rows, 4] is None unless `save` (a later backward needs it).  r, z: buffers to write into; r may be x."""
+    dtype = h.dtype if isinstance(h, torch.Tensor) else z.dtype if z is not None else x.dtype
+    d, rows, device = self._descriptor(x, 'x', dtype, gate, seed, offset, seed_dev, h is not None)
+    if h is None:
+      if not self.pre:
+        raise _lib.AdvocHipError('neither h nor a pre norm: nothing to compute')
+      r = x
+    else:
+      self._bind(d, 'h', h, rows, device)
+      if r is None:
+        r = torch.empty(x.shape, dtype=x.dtype, device=device)
+      self._bind(d, 'r', r, rows, device, x.dtype)
+    if self.pre:
+      if z is None:
+        z = torch.empty(x.shape, dtype=dtype, device=device)
+      self._bind(d, 'z', z, rows, device, dtype)
+    else:
+      z = None
+    stats = None
+    if save:
+      stats = torch.empty(rows, 4, dtype=torch.float32, device=device)
+      d.stats = stats.data_ptr()
+    _call(_lib.load().advoc_residual_norm_forward, 'advoc_residual_norm_forward', device, ctypes.byref(d))
+    return r, z, stats
+
+  def backward(self, dz, dr, h, r, stats, gate=None, seed=0, offset=0, seed_dev=None, into=None, accumulate=False):
+    """Gradients of forward(h, x, gate, seed, offset) with its r and stats (h None: r is x).  dz: gradient of z (None without a
+    pre norm), dr: gradient of r from elsewhere (may be None with a pre norm).  Gradients of what was not given are None.
+    into: {'dw_post': float32 [cols] buffer, ...} to write parameter gradients into, or with `accumulate` to add to."""
+    like = h if h is not None else dz
+    if not isinstance(like, torch.Tensor):
+      raise _lib.AdvocHipError('h or dz is needed')
+    d, rows, device = self._descriptor(r, 'r', like.dtype, gate, seed, offset, seed_dev, h is not None)
+    if (dz is None) != (not self.pre) or (dz is None and dr is None):
+      raise _lib.AdvocHipError('dz goes with a pre norm, and dz or dr must be given')
+    if dz is not None:
+      self._bind(d, 'dz', dz, rows, device, like.dtype)
+    if dr is not None:
+      self._bind(d, 'dr', dr, rows, device, r.dtype)
+    if h is not None:
+      self._bind(d, 'h', h, rows, device)
+    if self.pre or h is not None and self.post:
+      if not isinstance(stats, torch.Tensor) or stats.device != device or stats.dtype != torch.float32 or (
+          stats.shape != (rows, 4)) or not stats.is_contiguous():
+        raise _lib.AdvocHipError('stats must be the contiguous float32 [rows, 4] tensor of forward(..., save=True)')
+      d.stats = stats.data_ptr()
+    g = dict.fromkeys(ResidualNormGrads._fields)
+    g['dx'] = torch.empty(r.shape, dtype=r.dtype, device=device)
+    if h is not None:
+      g['dh'] = torch.empty(r.shape, dtype=h.dtype, device=device)
+    if gate is not None:
+      g['dgate'] = torch.empty(gate.shape, dtype=gate.dtype, device=device)
+    for name in ('dh', 'dx', 'dgate'):
+      if g[name] is not None:
+        field = getattr(d, name)
+        field.p, field.pitch = g[name].data_ptr(), self.cols
+    into = into or {}
+    for name in ('w_post', 'b_post', 'scale', 'w_pre', 'b_pre'):
+      if getattr(self, name) is None or h is None and name in ('w_post', 'b_post', 'scale'):
+        if 'd' + name in into:
+          raise _lib.AdvocHipError('d{} has nothing to be the gradient of'.format(name))
+        continue
+      t = into.get('d' + name)
+      if t is None:
+        if accumulate:
+          raise _lib.AdvocHipError('accumulate needs a buffer for d{}'.format(name))
+        t = torch.empty(self.cols, dtype=torch.float32, device=device)
+      g['d' + name] = t
+      setattr(d, 'd' + name, self._vector(t, 'd' + name, device))
+    unknown = set(into) - {k for k in g if k[1:] in ('w_post', 'b_post', 'scale', 'w_pre', 'b_pre')}
+    if unknown:
+      raise _lib.AdvocHipError('no such parameter gradients: {}'.format(sorted(unknown)))
+    d.accumulate = int(bool(accumulate))
+    lib = _lib.load()
+    nbytes = lib.advoc_residual_norm_workspace_bytes(ctypes.byref(d))
+    if nbytes:
+      work = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+      d.workspace, d.workspace_bytes = work.data_ptr(), nbytes
+    if rows == 0 and not accumulate:
+      for name in ('dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre'):
+        if g[name] is not None:
+          g[name].zero_()
+    _call(lib.advoc_residual_norm_backward, 'advoc_residual_norm_backward', device, ctypes.byref(d))
+    return ResidualNormGrads(**g)
+
+
+class F8Matrix(object):
+  """A matrix held in 8 bits with a power of two for each block of 128 along its rows: `data` [rows, kp] and `scale`
+  [rows, sp] (uint8; layout in include/advoc_hip.h), made by the quantize_f8 functions."""
+  __slots__ = ('data', 'scale', 'rows', 'k', 'format')
+
+  def __init__(self, rows, k, format, device):
+    kp = -(-k // 128) * 128
+    self.rows, self.k, self.format = rows, k, format
+    self.data = torch.empty(rows, kp, dtype=torch.uint8, device=device)
+    self.scale = torch.empty(rows, -(-kp // 512) * 4, dtype=torch.uint8, device=device)
+
+  @property
+  def shape(self):
+    return (self.rows, self.k)
+
+
+def _quantize(x, fmt, want_rows, want_cols):
+  code = _choice(FORMATS, fmt, 'format')
+  p, rows, cols, pitch = _rows(x, 'x')
+  if not rows or not cols:
+    raise _lib.AdvocHipError('x of shape {} holds nothing to quantise'.format(tuple(x.shape)))
+  a = F8Matrix(rows, cols, code, x.device) if want_rows else None
+  t = F8Matrix(cols, rows, code, x.device) if want_cols else None
+  _call(_lib.load().advoc_f8_quantize, 'advoc_f8_quantize', x.device, p, pitch, rows, cols, _dtype(x, 'x'), code,
+        a.data.data_ptr() if a else None, a.scale.data_ptr() if a else None,
+        t.data.data_ptr() if t else None, t.scale.data_ptr() if t else None)
+  return a, t
+
+
+def quantize_f8(x, fmt='e4m3'):
+  """The rows of x [..., k] in 8 bits ('e4m3' | 'e5m2'), a scale per block of 128 along k: an operand of matmul_nt_f8."""
+  return _quantize(x, fmt, True, False)[0]
+
+
+def quantize_f8_transposed(x, fmt='e4m3'):
+  """x^T in 8 bits, blocks of 128 along x's rows: the operand of a product that contracts over the rows of x."""
+  return _quantize(x, fmt, False, True)[1]
+
+
+def quantize_f8_both(x, fmt='e4m3'):
+  """(quantize_f8(x), quantize_f8_transposed(x)) with one read of x."""
+  return _quantize(x, fmt, True, True)
+
+
+def matmul_nt_f8(a, b, out_dtype=torch.float32, out=None, accumulate=False):
+  """a b^T of two F8Matrix operands with the same k -> [a.rows, b.rows], accumulated in fp32 (``advoc_matmul_nt_f8``).
+  accumulate: add to `out` (float32), e.g. a gradient arena's slice."""
+  if not isinstance(a, F8Matrix) or not isinstance(b, F8Matrix) or a.k != b.k or a.data.device != b.data.device:
+    raise _lib.AdvocHipError('two F8Matrix operands with the same k on one device are needed')
+  device, m, n = a.data.device, a.rows, b.rows
+  if out is None:
+    if accumulate:
+      raise _lib.AdvocHipError('accumulate needs out')
+    out = torch.empty(m, n, dtype=out_dtype, device=device)
+  elif not isinstance(out, torch.Tensor) or out.device != device or out.shape != (m, n) or not out.is_contiguous():
+    raise _lib.AdvocHipError('out must be a contiguous [{}, {}] tensor on {}'.format(m, n, device))
+  code = _dtype(out, 'out')
+  lib = _lib.load()
+  nbytes = lib.advoc_matmul_nt_f8_workspace_bytes(m, n, a.k)
+  work = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+  _call(lib.advoc_matmul_nt_f8, 'advoc_matmul_nt_f8', device, a.data.data_ptr(), a.scale.data_ptr(), a.format,
+        b.data.data_ptr(), b.scale.data_ptr(), b.format, out.data_ptr(), code, int(bool(accumulate)), m, n, a.k,
+        work.data_ptr() if nbytes else None, nbytes)
+  return out

@@ -1,0 +1,98 @@
+// Dropout whose mask is never stored (gfx950): y_i = x_i / keep where word i of the Philox stream (philox.h) is kept, exactly 0
+// elsewhere whatever x_i holds; the gradient is the same call on dy.  Reads and writes each element once: no byte of mask in
+// HBM, and the backward pass draws the same words again.
+#include "philox.h"
+#include "rows.h"
+
+namespace {
+
+using advoc::DropKey;
+using advoc::f32x8;
+
+constexpr int kThreads = 256, kPer = 8;              // a thread's chunk: 8 consecutive elements = two Philox blocks
+
+struct Args {
+  const void* x;
+  void* y;
+  int64_t n, x_pitch, y_pitch;
+  uint32_t cols;
+  DropKey key;
+};
+
+// PITCHED: rows of `cols` elements with a distance of their own; otherwise the n elements are one run.  The index that is
+// drawn for is the logical one (row * cols + column), so a tensor and its padded copy drop the same elements.
+template <typename T, bool PITCHED>
+__global__ __launch_bounds__(kThreads) void dropout_kernel(Args a) {
+  const uint2 key = advoc::drop_key_words(a.key);
+  const uint32_t thresh = a.key.thresh;
+  const float scale = a.key.scale;
+  const int64_t base = (int64_t)blockIdx.x * (kThreads * kPer);      // a multiple of 4, as the offset is
+  const int64_t i = base + threadIdx.x * kPer;
+  if (i >= a.n) return;
+  const uint32_t keep = thresh ? advoc::drop_keep8(a.key.offset + (uint64_t)i, true, key, thresh) : 0xffu;
+  const T* x = (const T*)a.x;
+  T* y = (T*)a.y;
+  uint32_t col = 0;
+  if constexpr (PITCHED) {
+    const uint64_t row0 = (uint64_t)base / a.cols;                   // uniform: one 64-bit division per workgroup
+    const uint32_t off = (uint32_t)((uint64_t)base - row0 * a.cols) + threadIdx.x * kPer;
+    const uint32_t r = off / a.cols;
+    col = off - r * a.cols;
+    x += (int64_t)(row0 + r) * a.x_pitch + col;
+    y += (int64_t)(row0 + r) * a.y_pitch + col;
+  } else {
+    x += i;
+    y += i;
+  }
+  if (i + kPer <= a.n && (!PITCHED || col + kPer <= a.cols)) {
+    const f32x8 v = advoc::load8(x);
+    f32x8 o;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) o[k] = (keep >> k & 1) ? v[k] * scale : 0.f;
+    advoc::store8(y, o);
+  } else {
+    for (int k = 0; k < kPer && i + k < a.n; ++k) {
+      *y = (T)((keep >> k & 1) ? (float)*x * scale : 0.f);
+      ++x, ++y;
+      if (PITCHED && ++col == a.cols) {
+        col = 0;
+        x += a.x_pitch - a.cols;
+        y += a.y_pitch - a.cols;
+      }
+    }
+  }
+}
+
+template <typename T>
+void launch(const Args& a, bool pitched, hipStream_t stream) {
+  const dim3 grid((unsigned)advoc::ceil_div(a.n, kThreads * kPer));
+  if (pitched)
+    hipLaunchKernelGGL((dropout_kernel<T, true>), grid, dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((dropout_kernel<T, false>), grid, dim3(kThreads), 0, stream, a);
+}
+
+}  // namespace
+
+extern "C" int advoc_dropout(const void* x, int64_t x_pitch, void* y, int64_t y_pitch, int64_t rows, int64_t cols, int32_t dtype,
+                             float keep_prob, uint64_t seed, uint64_t offset, const uint64_t* seed_dev, advoc_stream_t stream) {
+  if (rows < 0 || cols < 0 || !(keep_prob > 0.f && keep_prob <= 1.f)) return ADVOC_ERR_BAD_SHAPE;
+  if (rows == 0 || cols == 0) return ADVOC_OK;
+  if (!x || !y) return ADVOC_ERR_NULL;
+  if (rows > 1 && (x_pitch < cols || y_pitch < cols)) return ADVOC_ERR_BAD_SHAPE;
+  if (!advoc::dtype_ok(dtype) || (offset & 3)) return ADVOC_ERR_UNSUPPORTED;
+  if (cols > 0x7fffffffLL - 2 * kThreads * kPer && rows > 1 && (x_pitch != cols || y_pitch != cols)) return ADVOC_ERR_UNSUPPORTED;
+  if (rows > (1LL << 40) / cols) return ADVOC_ERR_UNSUPPORTED;         // the grid ends at 2^31 workgroups of 2048 elements
+  const bool pitched = rows > 1 && (x_pitch != cols || y_pitch != cols);
+  Args a = {x, y, rows * cols, x_pitch, y_pitch, pitched ? (uint32_t)cols : 0u,
+            advoc::make_drop_key(keep_prob, seed, offset, seed_dev)};
+  ADVOC_CLEAR_LAUNCH_ERROR();
+  if (dtype == ADVOC_F32)
+    launch<float>(a, pitched, advoc::as_stream(stream));
+  else if (dtype == ADVOC_BF16)
+    launch<__bf16>(a, pitched, advoc::as_stream(stream));
+  else
+    launch<_Float16>(a, pitched, advoc::as_stream(stream));
+  ADVOC_RETURN_IF_LAUNCH_FAILED();
+  return ADVOC_OK;
+}

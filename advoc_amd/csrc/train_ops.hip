@@ -7,6 +7,7 @@
 //   advoc_adam_tf_f32                   : tf.train.AdamOptimizer(0.0002, 0.5) ApplyAdam, :250-257
 //   advoc_dropout_mask_u8               : RandomUniform + Floor of tf.nn.dropout, :144-149
 #include "common.h"
+#include "philox.h"
 
 namespace {
 
@@ -122,21 +123,6 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, const 
   }
 }
 
-// Philox-4x32-10 counter RNG: element e of stream `seed` depends only on (seed, e), so masks are
-// reproducible and independent of how a global batch is sharded over GPUs.
-__device__ __forceinline__ uint4 philox4x32(uint4 ctr, uint2 key) {
-  const uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint32_t hi0 = __umulhi(M0, ctr.x), lo0 = M0 * ctr.x;
-    const uint32_t hi1 = __umulhi(M1, ctr.z), lo1 = M1 * ctr.z;
-    ctr = make_uint4(hi1 ^ ctr.y ^ key.x, lo1, hi0 ^ ctr.w ^ key.y, lo0);
-    key.x += W0;
-    key.y += W1;
-  }
-  return ctr;
-}
-
 // mask[i] = floor(keep + u) with u uniform in [0,1): 1 when u >= 1 - keep  (tf.nn.dropout)
 __global__ __launch_bounds__(256) void dropout_mask_kernel(uint8_t* __restrict__ mask, int64_t n,
                                                            uint64_t seed, uint64_t offset, float keep) {
@@ -145,8 +131,8 @@ __global__ __launch_bounds__(256) void dropout_mask_kernel(uint8_t* __restrict__
   const uint32_t thresh = (uint32_t)fminf(fmaxf((1.0f - keep) * 4294967296.0f, 0.f), 4294967295.f);
   for (int64_t q = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; q < quads; q += stride) {
     const uint64_t c = (offset >> 2) + (uint64_t)q;     // offset is a multiple of 4
-    const uint4 r = philox4x32(make_uint4((uint32_t)c, (uint32_t)(c >> 32), 0u, 0u),
-                               make_uint2((uint32_t)seed, (uint32_t)(seed >> 32)));
+    const uint4 r = advoc::philox4x32(make_uint4((uint32_t)c, (uint32_t)(c >> 32), 0u, 0u),
+                                      make_uint2((uint32_t)seed, (uint32_t)(seed >> 32)));
     const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
     const int64_t i = q * 4;
     if (i + 4 <= n) {

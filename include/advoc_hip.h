@@ -541,6 +541,121 @@ int advoc_zero_f32(float* dst, int64_t count, advoc_stream_t stream);
 int advoc_dropout_mask_u8(uint8_t* mask, int64_t count, uint64_t seed, uint64_t offset, float keep_prob,
                           advoc_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Residual blocks over frames: dropout without a stored mask, the norms around a block, 8-bit products.
+ * No reference op: the reference's networks are convolutions with batch norm; these are the same three ingredients
+ * -- dropout (advoc_model.py:144-149), normalisation (:77-84), a dense product (models/melspecgan/conv2d.py:82-150) --
+ * in the forms that blocks along the time axis need.
+ *   rows    frames of all clips; a row is `cols` channels (or bins) of unit stride, rows `pitch` ELEMENTS apart
+ *   dtypes  ADVOC_F32 | ADVOC_BF16 | ADVOC_F16; arithmetic, statistics and sums are fp32, each output rounded once
+ *   align   tensors need only be aligned to their elements
+ * ---------------------------------------------------------------------------------------- */
+#define ADVOC_F32 0
+#define ADVOC_BF16 1
+#define ADVOC_F16 2
+
+/* y[i] = keep_i ? x[i] / keep_prob : 0 with keep_i of advoc_dropout_mask_u8 at (seed, offset + i), i = row * cols + column
+ * (the LOGICAL index: a pitch does not change what is dropped).  The mask is never stored: the gradient is the same call on
+ * dy.  A dropped element is 0 whatever x holds (NaN and infinities included); keep_prob 1 copies.
+ *   seed_dev  NULL, or a device word that the kernel adds to `seed`: a captured graph whose program changes that word
+ *             between replays draws another mask each time
+ * y may be x (same pitch).  offset % 4 == 0. */
+int advoc_dropout(const void* x, int64_t x_pitch, void* y, int64_t y_pitch, int64_t rows, int64_t cols, int32_t dtype,
+                  float keep_prob, uint64_t seed, uint64_t offset, const uint64_t* seed_dev, advoc_stream_t stream);
+
+#define ADVOC_NORM_NONE 0
+#define ADVOC_NORM_RMS 1   /* a / sqrt(mean a^2 + eps)            */
+#define ADVOC_NORM_LAYER 2 /* (a - mean a) / sqrt(var a + eps), biased variance */
+#define ADVOC_GATE_NONE 0
+#define ADVOC_GATE_SIGMOID 1
+#define ADVOC_NORM_MAX_COLS 16384
+
+typedef struct advoc_rows {
+  void* p;       /* NULL: absent */
+  int64_t pitch; /* elements from one row to the next */
+} advoc_rows;
+
+/* The glue between two residual blocks, per row:
+ *   u = N_post(h) w_post + b_post                     norm behind the block whose output is h
+ *   r = x + alpha * scale * act(gate) * drop(u)       gate, per-channel residual scale, dropout, residual sum
+ *   z = N_pre(r) w_pre + b_pre                        norm before the next block
+ * and its gradients.  N_* of kind ADVOC_NORM_NONE is the identity without weight and bias (norm_pre: z is not written).
+ * Any of w_*, b_*, scale, gate may be absent (1, 0, 1, 1).  h absent (then no post norm, gate or scale): only
+ * z = N_pre(x), the norm before the first block.
+ *   gate [rows / gate_group, cols]: consecutive gate_group rows share one gate row (1: a gate per element; the frames of a
+ *        clip: a gate per clip); its gradient is summed over them
+ *   dropout draws at (seed (+ *seed_dev), offset + row * cols + column) like advoc_dropout; keep_prob 1 draws nothing
+ *   dtype is that of h, gate, z, dz, dh, dgate; res_dtype (dtype or ADVOC_F32) that of x, r, dr, dx
+ *   stats [rows][4] fp32 (mean, 1 / sqrt(var + eps) of the post norm, then of the pre norm; 0 where there is none; 16-byte
+ *        aligned): written by the forward pass when not NULL, read by the backward pass
+ * z and the statistics are those of r BEFORE it is rounded to res_dtype.
+ * An output may be the buffer of an input of the same type, rows and pitch (r over x, dx over dr, dh over h ...).
+ * A row of zeros gives zeros (plus the bias).  A NaN or infinity stays in its row. */
+typedef struct advoc_residual_norm {
+  int64_t rows;
+  int32_t cols;
+  int32_t dtype, res_dtype;
+  int32_t norm_post, norm_pre;
+  int32_t gate_act;
+  int64_t gate_group;
+  const float* w_post; /* [cols] each, or NULL */
+  const float* b_post;
+  const float* scale;
+  const float* w_pre;
+  const float* b_pre;
+  float alpha, eps, keep_prob;
+  int32_t accumulate; /* backward: != 0 adds to the five parameter gradients, 0 overwrites them */
+  uint64_t seed, offset;
+  const uint64_t* seed_dev;
+  advoc_rows h, x, gate;
+  advoc_rows r, z; /* forward: written; backward: r is read (the forward pass's; x of a call without h), z ignored */
+  float* stats;
+  /* backward: gradients of z and r (dz is required with a pre norm; dr may be absent then), and what is wanted of the
+   * gradients of h, x, gate (absent: not written) and of the parameters (NULL: not computed) */
+  advoc_rows dz, dr;
+  advoc_rows dh, dx, dgate;
+  float* dw_post;
+  float* db_post;
+  float* dscale;
+  float* dw_pre;
+  float* db_pre;
+  void* workspace; /* backward: advoc_residual_norm_workspace_bytes() of this descriptor, 4-byte aligned */
+  int64_t workspace_bytes;
+} advoc_residual_norm;
+
+int advoc_residual_norm_forward(const advoc_residual_norm* desc, advoc_stream_t stream);
+/* Scratch of the backward call (0: none); depends on which gradients are wanted.  Sums over rows are added in an order fixed
+ * by the shapes: two calls give the same bits.  ADVOC_ERR_NULL from the call when the scratch is missing or too small. */
+int64_t advoc_residual_norm_workspace_bytes(const advoc_residual_norm* desc);
+int advoc_residual_norm_backward(const advoc_residual_norm* desc, advoc_stream_t stream);
+
+/* 8-bit operands with a scale for each block of 128 along the contraction axis.  The scale is a power of two (one exponent
+ * byte: scale = 2^(byte - 127)), so scaling is exact and the matrix instruction applies it:
+ *   e = smallest integer >= -126 with max |x| of the block's finite values <= top 2^e     (top 448: E4M3, 57344: E5M2)
+ *   q = nearest 8-bit value to x 2^-e, ties to even;   infinities and NaN become NaN (E4M3) or stay what they are (E5M2)
+ * A quantised matrix of `rows` rows and `k` columns is
+ *   q     [rows][kp] bytes, kp = 128 ceil(k / 128), zero beyond k; 16-byte aligned
+ *   scale [rows][sp] bytes, sp =   4 ceil(kp / 512), zero beyond kp / 128; 4-byte aligned */
+#define ADVOC_E4M3 0
+#define ADVOC_E5M2 1
+
+/* x [rows, cols] (dtype, pitch in elements) -> q, scale: x quantised in blocks of its rows, and / or qt, scale_t: x^T (cols rows
+ * of `rows` columns) quantised in blocks of x's columns, for products that contract over x's rows (weight and input
+ * gradients).  Either pair may be NULL; both together read x once. */
+int advoc_f8_quantize(const void* x, int64_t x_pitch, int64_t rows, int64_t cols, int32_t dtype, int32_t format, uint8_t* q,
+                      uint8_t* scale, uint8_t* qt, uint8_t* scale_t, advoc_stream_t stream);
+
+/* out[i, j] = sum_k a[i, k] b[j, k] of two quantised matrices (m and n rows, the same k; formats may differ), like
+ * advoc_matmul_nt_f32.  ADVOC_F32 outputs are accumulated in fp32 throughout.  16-bit outputs take the 8-bit matrix instruction at
+ * twice the rate: it adds up in fp32 but for products below 2^-13 of the largest of eight neighbours, which it drops (1.5e-5 of
+ * the result in norm; their own rounding is 1.7e-3 or 2e-4).  out [m, n] dense; accumulate != 0 (out_dtype ADVOC_F32) adds to it.
+ * workspace: advoc_matmul_nt_f8_workspace_bytes(m, n, k) bytes, 4-byte aligned (0: may be NULL); with too little the product runs
+ * unsplit.  The order of every sum is fixed by the shapes: two calls give the same bits. */
+int64_t advoc_matmul_nt_f8_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int advoc_matmul_nt_f8(const uint8_t* a, const uint8_t* a_scale, int32_t a_format, const uint8_t* b, const uint8_t* b_scale,
+                       int32_t b_format, void* out, int32_t out_dtype, int32_t accumulate, int64_t m, int64_t n, int64_t k,
+                       void* workspace, int64_t workspace_bytes, advoc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
