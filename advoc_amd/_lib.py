@@ -143,7 +143,7 @@ PROTOTYPES = {
     'advoc_residual_norm_workspace_bytes': (_i64, [_p]),
     'advoc_residual_norm_backward': (ctypes.c_int, [_p, _p]),
     'advoc_f8_quantize': (ctypes.c_int, [_p, _i64, _i64, _i64, _i32, _i32, _p, _p, _p, _p, _p]),
-    'advoc_matmul_nt_f8_workspace_bytes': (_i64, [_i64, _i64, _i64]),
+    'advoc_matmul_nt_f8_workspace_bytes': (_i64, [_i64, _i64, _i64, _i32]),
     'advoc_matmul_nt_f8': (ctypes.c_int, [_p, _p, _i32, _p, _p, _i32, _p, _i32, _i32, _i64, _i64, _i64, _p, _i64, _p]),
 }
 

@@ -348,7 +348,7 @@ def matmul_nt_f8(a, b, out_dtype=torch.float32, out=None, accumulate=False):
     raise _lib.AdvocHipError('out must be a contiguous [{}, {}] tensor on {}'.format(m, n, device))
   code = _dtype(out, 'out')
   lib = _lib.load()
-  nbytes = lib.advoc_matmul_nt_f8_workspace_bytes(m, n, a.k)
+  nbytes = lib.advoc_matmul_nt_f8_workspace_bytes(m, n, a.k, code)
   work = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
   _call(lib.advoc_matmul_nt_f8, 'advoc_matmul_nt_f8', device, a.data.data_ptr(), a.scale.data_ptr(), a.format,
         b.data.data_ptr(), b.scale.data_ptr(), b.format, out.data_ptr(), code, int(bool(accumulate)), m, n, a.k,

@@ -84,13 +84,24 @@ __device__ __forceinline__ f32x4 mfma(const Frag<FB, true>& b, const Frag<FA, tr
   return c;
 }
 
-// c consecutive values of one output row
-template <typename O>
-__device__ __forceinline__ void store_run(const Args& g, int64_t row, int64_t col, const float* v, int c) {
+// C consecutive values of one output row
+template <typename O, int C>
+__device__ __forceinline__ void store_run(const Args& g, int64_t row, int64_t col, float (&v)[C]) {
   if (row >= g.m) return;
   O* p = (O*)g.out + row * g.n + col;
-  for (int k = 0; k < c; ++k)
-    if (col + k < g.n) p[k] = (O)((g.accumulate ? (float)p[k] : 0.f) + v[k]);
+  if (col + C <= g.n) {
+    if (g.accumulate)
+#pragma unroll
+      for (int k = 0; k < C; ++k) v[k] += (float)p[k];
+    O o[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) o[k] = (O)v[k];
+    __builtin_memcpy(p, o, sizeof(o));
+  } else {
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+      if (col + k < g.n) p[k] = (O)((g.accumulate ? (float)p[k] : 0.f) + v[k]);
+  }
 }
 
 // ---- few rows (m <= 64): the weights are read once, by whoever multiplies them ----
@@ -131,101 +142,152 @@ __global__ __launch_bounds__(1024) void f8_thin_kernel(Args g) {
     f32x4 v = red[e];
     for (int w = 1; w < waves; ++w) v += red[w * MF * 64 + e];
     const int l = e & 63;
-    const float o[4] = {v[0], v[1], v[2], v[3]};
-    store_run<O>(g, (e >> 6) * 16 + (l & 15), n0 + (l >> 4) * 4, o, 4);
+    float o[4] = {v[0], v[1], v[2], v[3]};
+    store_run<O, 4>(g, (e >> 6) * 16 + (l & 15), n0 + (l >> 4) * 4, o);
   }
 }
 
 // ---- tiles ----
 // BM x BN outputs per workgroup, WM x WN per wave.  A block of the contraction of both operands is a stage of LDS, fetched by
-// LDS-DMA while the stage before is multiplied.  A row's eight 16-byte pieces lie at piece ^ key(row): the 16 rows that a
-// fragment reads together have keys 0 ... 7 twice, so its reads spread over all banks.
+// LDS-DMA while the stage before is multiplied; the exponent bytes of four blocks (a dword per row) are fetched the same way every
+// fourth block.  (Loads that the compiler counts must not follow a DMA in the loop: memory counters retire in order, and waiting for
+// such a load waits for the next stage too.  That alone held the first form of this kernel at 0.8 PFLOP/s.)
+// A row's eight 16-byte pieces lie at piece ^ key(row): the 16 rows that a fragment reads together have keys 0 ... 7 twice, so its
+// reads spread over all banks.
+template <int BM, int BN, int WM, int WN>
+struct Tile {
+  static constexpr int kWaves = BM / WM * (BN / WN), kFm = WM / 16, kFn = WN / 16;
+  static constexpr int kShift = kFn == 4 ? 4 : 3;                // rows of b four apart in the instruction are 4 kFn apart
+  static constexpr int kRows = BM + BN, kStage = kRows * kBlock, kExp = kRows * 4;
+  static constexpr int kLds = 2 * (kStage + kExp);
+  static constexpr int kDma = kRows / 8 / kWaves;                // a DMA instruction fetches 8 rows
+  static constexpr int kExpDma = (kRows / 64 + kWaves - 1) / kWaves;      // or the exponents of 64 rows
+  static_assert(kFn == 2 || kFn == 4, "a wave is two or four fragments of b wide");
+  static_assert(kDma * 8 * kWaves == kRows && BM % (8 * kWaves) == 0, "whole DMA instructions per wave and operand");
+  static_assert(8 * kWaves % (2 << kShift) == 0, "rows fetched by one lane have one key");
+  static_assert(BM % 64 == 0 && BN % 64 == 0, "64 rows of one operand per exponent fetch");
+
+  advoc::u32x4s ra, rb, rea, reb;
+  const uint8_t* lds;
+  unsigned base;
+  int lane, wave, wm, wn, spitch;
+  int kp, voff_a, voff_b;                // what this lane fetches: its first row of a and of b, the others are 8 kWaves rows on
+  int off_a, off_b, piece0, piece1;      // this lane's first rows in a stage, its two pieces of a row
+
+  static __device__ __forceinline__ int key_a(int row) { return row & 7; }
+  static __device__ __forceinline__ int key_b(int row) { return (row & 3) | ((row >> kShift) & 1) << 2; }
+
+  __device__ __forceinline__ Tile(const Args& g, const uint8_t* lds_, int64_t m0, int64_t n0) : lds(lds_) {
+    lane = threadIdx.x & 63;
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wm = wave / (BN / WN) * WM;
+    wn = wave % (BN / WN) * WN;
+    // rows behind the last one read as zeros: their offsets are behind the descriptor's end
+    const int64_t mrows = g.m - m0 < BM ? g.m - m0 : BM, nrows = g.n - n0 < BN ? g.n - n0 : BN;
+    ra = advoc::dma_rsrc(g.a + m0 * g.kp, (unsigned)(mrows * g.kp));
+    rb = advoc::dma_rsrc(g.b + n0 * g.kp, (unsigned)(nrows * g.kp));
+    rea = advoc::dma_rsrc(g.a_scale + m0 * g.sp, (unsigned)(mrows * g.sp));
+    reb = advoc::dma_rsrc(g.b_scale + n0 * g.sp, (unsigned)(nrows * g.sp));
+    base = advoc::lds_address(lds);
+    spitch = (int)g.sp;
+    kp = (int)g.kp;
+    const int first = wave * 8 + (lane >> 3);
+    voff_a = first * kp + (((lane & 7) ^ key_a(first)) << 4);
+    voff_b = first * kp + (((lane & 7) ^ key_b(first)) << 4);
+    // fragment i of a: rows wm + 16 i + lane % 16; fragment j of b: rows wn + 4 kFn (lane % 16 / 4) + 4 j + lane % 4.  Their keys are
+    // lane % 8 for every fragment
+    off_a = wm + (lane & 15);
+    off_b = BM + wn + ((lane & 15) >> 2) * 4 * kFn + (lane & 3);
+    piece0 = (((lane >> 4) * 2) ^ (lane & 7)) << 4;
+    piece1 = (((lane >> 4) * 2 + 1) ^ (lane & 7)) << 4;
+  }
+
+  // block kb of the contraction into stage slot (kb - first) & 1, and with every fourth block the exponents of the next four
+  __device__ __forceinline__ void fetch(int kb, int slot) const {
+#pragma unroll
+    for (int t = 0; t < kDma; ++t) {
+      const unsigned to = base + slot * kStage + (t * kWaves + wave) * 1024;
+      if (t * 8 * kWaves < BM) advoc::dma16(ra, to, voff_a + t * 8 * kWaves * kp, kb * kBlock);
+      else advoc::dma16(rb, to, voff_b + (t * 8 * kWaves - BM) * kp, kb * kBlock);
+    }
+  }
+  __device__ __forceinline__ void fetch_exponents(int quad) const {
+#pragma unroll
+    for (int t = 0; t < kExpDma; ++t) {
+      const int first = (t * kWaves + wave) * 64;
+      if (first >= kRows) break;
+      const bool is_a = first < BM;
+      advoc::dma4(is_a ? rea : reb, base + 2 * kStage + (quad & 1) * kExp + first * 4, (first + lane - (is_a ? 0 : BM)) * spitch, quad * 4);
+    }
+  }
+
+  __device__ __forceinline__ i32x8 bytes(int row) const {      // slot * kRows + row of the stage
+    const uint8_t* p = lds + row * kBlock;
+    return join(*reinterpret_cast<const int4*>(p + piece0), *reinterpret_cast<const int4*>(p + piece1));
+  }
+  __device__ __forceinline__ i32x8 bytes_a(int slot, int i) const { return bytes(slot * kRows + off_a + i * 16); }
+  __device__ __forceinline__ i32x8 bytes_b(int slot, int j) const { return bytes(slot * kRows + off_b + j * 4); }
+  __device__ __forceinline__ int exponents(int quad, int row) const {
+    return *reinterpret_cast<const int*>(lds + 2 * kStage + ((quad & 1) * kRows + row) * 4);
+  }
+  __device__ __forceinline__ void exponents(int quad, int (&ea)[kFm], int (&eb)[kFn]) const {
+#pragma unroll
+    for (int i = 0; i < kFm; ++i) ea[i] = exponents(quad, off_a + i * 16);
+#pragma unroll
+    for (int j = 0; j < kFn; ++j) eb[j] = exponents(quad, off_b + j * 4);
+  }
+
+  template <typename O>
+  __device__ __forceinline__ void store(const Args& g, int64_t m0, int64_t n0, const f32x4 (&acc)[kFm][kFn]) const {
+#pragma unroll
+    for (int i = 0; i < kFm; ++i) {
+      float v[4 * kFn];
+#pragma unroll
+      for (int j = 0; j < kFn; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * j + e] = acc[i][j][e];
+      store_run<O, 4 * kFn>(g, m0 + off_a + i * 16, n0 + wn + (lane >> 4) * 4 * kFn, v);
+    }
+  }
+};
+
 template <typename O, bool EXACT, int FA, int FB, int BM, int BN, int WM, int WN, bool SPLIT>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void f8_tile_kernel(Args g) {
-  constexpr int kWaves = BM / WM * (BN / WN), kFm = WM / 16, kFn = WN / 16;
-  constexpr int kShift = kFn == 4 ? 4 : 3;                       // rows of b four apart in the instruction are 4 kFn apart
-  static_assert(kFn == 2 || kFn == 4, "a wave is two or four fragments of b wide");
-  constexpr int kStage = (BM + BN) * kBlock;
-  constexpr int kDma = (BM + BN) / 8 / kWaves;                   // a DMA instruction fetches 8 rows
-  static_assert(kDma * 8 * kWaves == BM + BN && BM % (8 * kWaves) == 0, "whole DMA instructions per wave and operand");
-  __shared__ __align__(1024) uint8_t lds[2 * kStage];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  using T = Tile<BM, BN, WM, WN>;
+  __shared__ __align__(1024) uint8_t lds[T::kLds];
   const int64_t m0 = (int64_t)blockIdx.x * BM, n0 = (int64_t)blockIdx.y * BN;
   const int kb0 = SPLIT ? blockIdx.z * g.per_split : 0;
   const int kb1 = SPLIT ? (kb0 + g.per_split < g.blocks ? kb0 + g.per_split : g.blocks) : g.blocks;
-  const int wm = (wave / (BN / WN)) * WM, wn = (wave % (BN / WN)) * WN;
+  const T t(g, lds, m0, n0);
 
-  // rows behind the last one read as zeros: their offsets are behind the descriptor's end
-  const int64_t mrows = g.m - m0 < BM ? g.m - m0 : BM, nrows = g.n - n0 < BN ? g.n - n0 : BN;
-  const advoc::u32x4s ra = advoc::dma_rsrc(g.a + m0 * g.kp, (unsigned)(mrows * g.kp));
-  const advoc::u32x4s rb = advoc::dma_rsrc(g.b + n0 * g.kp, (unsigned)(nrows * g.kp));
-  const unsigned base = advoc::lds_address(lds);
-  int voff[kDma];
+  f32x4 acc[T::kFm][T::kFn];
 #pragma unroll
-  for (int t = 0; t < kDma; ++t) {
-    const int row = (t * kWaves + wave) * 8 + (lane >> 3);       // of a, then of b
-    const int r = row < BM ? row : row - BM;
-    const int key = row < BM ? r & 7 : (r & 3) | ((r >> kShift) & 1) << 2;
-    voff[t] = r * (int)g.kp + (((lane & 7) ^ key) << 4);
-  }
-  auto fetch = [&](int kb, int stage) {
+  for (int i = 0; i < T::kFm; ++i)
 #pragma unroll
-    for (int t = 0; t < kDma; ++t) {
-      const bool is_a = t * 8 * kWaves < BM;
-      advoc::dma16(is_a ? ra : rb, base + stage * kStage + (t * kWaves + wave) * 1024, voff[t], kb * kBlock);
-    }
-  };
+    for (int j = 0; j < T::kFn; ++j) acc[i][j] = (f32x4)(0.f);
 
-  // exponents: a dword is four blocks of a row
-  const uint8_t *as[kFm], *bs[kFn];
-  int arow[kFm], brow[kFn];
-#pragma unroll
-  for (int i = 0; i < kFm; ++i) {
-    arow[i] = wm + i * 16 + (lane & 15);
-    const int64_t r = m0 + arow[i] < g.m ? m0 + arow[i] : g.m - 1;
-    as[i] = g.a_scale + r * g.sp;
-  }
-#pragma unroll
-  for (int j = 0; j < kFn; ++j) {
-    brow[j] = wn + ((lane & 15) >> 2) * 4 * kFn + j * 4 + (lane & 3);
-    const int64_t r = n0 + brow[j] < g.n ? n0 + brow[j] : g.n - 1;
-    bs[j] = g.b_scale + r * g.sp;
-  }
-
-  f32x4 acc[kFm][kFn];
-#pragma unroll
-  for (int i = 0; i < kFm; ++i)
-#pragma unroll
-    for (int j = 0; j < kFn; ++j) acc[i][j] = (f32x4)(0.f);
-
-  if (kb0 < kb1) fetch(kb0, 0);
+  int ea[T::kFm], eb[T::kFn];
+  t.fetch_exponents(kb0 >> 2);
+  t.fetch(kb0, 0);
   for (int kb = kb0; kb < kb1; ++kb) {
-    const int stage = (kb - kb0) & 1;
+    const int slot = (kb - kb0) & 1;
     advoc::dma_ring_barrier<0>();
-    int sa[kFm], sb[kFn];
-#pragma unroll
-    for (int i = 0; i < kFm; ++i) sa[i] = as[i][kb];
-#pragma unroll
-    for (int j = 0; j < kFn; ++j) sb[j] = bs[j][kb];
-    if (kb + 1 < kb1) fetch(kb + 1, stage ^ 1);
-    const uint8_t* s = lds + stage * kStage;
-    const int piece = (lane >> 4) * 2;
-    auto bytes = [&](int row, int key) {
-      const uint8_t* p = s + row * kBlock;
-      return join(*reinterpret_cast<const int4*>(p + ((piece ^ key) << 4)), *reinterpret_cast<const int4*>(p + (((piece + 1) ^ key) << 4)));
-    };
-    auto frag_b = [&](int j) {
-      return Frag<FB, EXACT>(bytes(BM + brow[j], (brow[j] & 3) | ((brow[j] >> kShift) & 1) << 2), sb[j]);
-    };
+    if (kb + 1 < kb1) {
+      if (((kb + 1) & 3) == 0) t.fetch_exponents((kb + 1) >> 2);
+      t.fetch(kb + 1, slot ^ 1);
+    }
+    if (kb == kb0 || (kb & 3) == 0) t.exponents(kb >> 2, ea, eb);
+    const int shift = (kb & 3) * 8;
+    auto frag_b = [&](int j) { return Frag<FB, EXACT>(t.bytes_b(slot, j), eb[j] >> shift & 255); };
     auto multiply = [&](const auto&... b) {
 #pragma unroll
-      for (int i = 0; i < kFm; ++i) {
-        const Frag<FA, EXACT> a(bytes(arow[i], arow[i] & 7), sa[i]);
+      for (int i = 0; i < T::kFm; ++i) {
+        const Frag<FA, EXACT> a(t.bytes_a(slot, i), ea[i] >> shift & 255);
         int j = 0;
         ((acc[i][j] = mfma<FA, FB>(b, a, acc[i][j]), ++j), ...);
       }
     };
-    if constexpr (kFn == 2) multiply(frag_b(0), frag_b(1));
+    if constexpr (T::kFn == 2) multiply(frag_b(0), frag_b(1));
     else multiply(frag_b(0), frag_b(1), frag_b(2), frag_b(3));
   }
 
@@ -234,15 +296,85 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void f8_tile_kernel(Args 
     o.out = g.part + (int64_t)blockIdx.z * g.m * g.n;
     o.accumulate = 0;
   }
+  t.template store<O>(o, m0, n0, acc);
+}
+
+// 256 x 256 outputs, eight waves of 128 x 64, the 8-bit instruction.  Two waves share a SIMD and take turns: while the waves of one
+// half of the workgroup read the fragments of a block from LDS (24 reads of 16 bytes a lane: 768 cycles of the CU's 128 bytes a
+// cycle for four waves), the other half multiplies the block before (32 instructions of 32 cycles), with a rendezvous between; the
+// matrix pipe has work in both halves of a block's time.
+template <typename O, int FA, int FB>
+__global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
+  using T = Tile<256, 256, 128, 64>;
+  __shared__ __align__(1024) uint8_t lds[T::kLds];
+  const int64_t m0 = (int64_t)blockIdx.x * 256, n0 = (int64_t)blockIdx.y * 256;
+  const T t(g, lds, m0, n0);
+
+  f32x4 acc[T::kFm][T::kFn];
 #pragma unroll
-  for (int i = 0; i < kFm; ++i) {
-    float v[4 * kFn];
+  for (int i = 0; i < T::kFm; ++i)
 #pragma unroll
-    for (int j = 0; j < kFn; ++j)
+    for (int j = 0; j < T::kFn; ++j) acc[i][j] = (f32x4)(0.f);
+  i32x8 a[T::kFm], b[T::kFn];
+  int ea[T::kFm], eb[T::kFn];
+
+  auto read = [&](int kb) {
+    const int slot = kb & 1;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * j + e] = acc[i][j][e];
-    store_run<O>(o, m0 + arow[i], n0 + wn + (lane >> 4) * 4 * kFn, v, 4 * kFn);
+    for (int j = 0; j < T::kFn; ++j) b[j] = t.bytes_b(slot, j);
+#pragma unroll
+    for (int i = 0; i < T::kFm; ++i) a[i] = t.bytes_a(slot, i);
+    if ((kb & 3) == 0) {
+      t.exponents(kb >> 2, ea, eb);
+    } else {
+#pragma unroll
+      for (int i = 0; i < T::kFm; ++i) ea[i] >>= 8;
+#pragma unroll
+      for (int j = 0; j < T::kFn; ++j) eb[j] >>= 8;
+    }
+  };
+  auto multiply = [&]() {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < T::kFm; ++i)
+#pragma unroll
+      for (int j = 0; j < T::kFn; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i], acc[i][j], FB, FA, 0, eb[j], 0, ea[i]);
+    __builtin_amdgcn_s_setprio(0);
+  };
+  auto fetch = [&](int kb) {
+    if (kb >= g.blocks) return;
+    if ((kb & 3) == 0) t.fetch_exponents(kb >> 2);
+    t.fetch(kb, kb & 1);
+  };
+  auto meet = [&](bool landed) {      // my reads have arrived and, with `landed`, what I fetched lies in LDS
+    __builtin_amdgcn_sched_barrier(0);
+    if (landed) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  // Both halves run one program, the second one rendezvous behind: rendezvous 2 kb + 1 ends the first half's reads of block kb and
+  // the second's multiplication of kb - 1, rendezvous 2 kb + 2 the second's reads of kb and the first's multiplication.  Behind
+  // rendezvous 2 kb nobody reads block kb - 1 any more, so both halves fetch kb + 1 into its place there, and it has to lie there
+  // at rendezvous 2 kb + 2.
+  const bool late = t.wave >= 4;      // waves w and w + 4 share a SIMD
+  fetch(0);
+  meet(true);
+  if (late) {
+    fetch(1);
+    meet(false);
   }
+  for (int kb = 0; kb < g.blocks; ++kb) {
+    if (!late) fetch(kb + 1);
+    read(kb);
+    meet(late);
+    if (late) fetch(kb + 2);
+    multiply();
+    meet(!late);
+  }
+  if (!late) meet(false);
+  t.template store<O>(g, m0, n0, acc);
 }
 
 // the parts of a split contraction, added in order
@@ -261,11 +393,11 @@ struct Plan {
   int form, splits, per_split;
 };
 
-Plan make_plan(int64_t m, int64_t n, int blocks) {
+Plan make_plan(int64_t m, int64_t n, int blocks, bool exact) {
   Plan p = {kThin, 1, blocks};
   if (m <= 64) return p;
   const int64_t t256 = ceil_div(m, 256) * ceil_div(n, 256), t128 = ceil_div(m, 128) * ceil_div(n, 128);
-  p.form = t256 >= 192 ? kTile256 : t128 >= 64 ? kTile128 : kTile64;
+  p.form = t256 >= 192 && !exact ? kTile256 : t128 >= 64 ? kTile128 : kTile64;
   const int64_t tiles = p.form == kTile256 ? t256 : p.form == kTile128 ? t128 : ceil_div(m, 64) * ceil_div(n, 64);
   int64_t splits = 512 / tiles;
   if (splits > blocks / 8) splits = blocks / 8;
@@ -299,7 +431,14 @@ int run(const Args& g, const Plan& p, hipStream_t stream) {
     ADVOC_RETURN_IF_LAUNCH_FAILED();
     return ADVOC_OK;
   }
-  if (p.form == kTile256) return run_tile<O, EXACT, FA, FB, 256, 256, 128, 64, false>(g, 1, stream);
+  if constexpr (!EXACT) {
+    if (p.form == kTile256) {
+      const dim3 grid((unsigned)ceil_div(g.m, 256), (unsigned)ceil_div(g.n, 256));
+      hipLaunchKernelGGL((f8_big_kernel<O, FA, FB>), grid, dim3(512), 0, stream, g);
+      ADVOC_RETURN_IF_LAUNCH_FAILED();
+      return ADVOC_OK;
+    }
+  }
   if (p.splits == 1)
     return p.form == kTile128 ? run_tile<O, EXACT, FA, FB, 128, 128, 64, 64, false>(g, 1, stream)
                               : run_tile<O, EXACT, FA, FB, 64, 64, 32, 32, false>(g, 1, stream);
@@ -324,9 +463,9 @@ int run_formats(const Args& g, const Plan& p, int fa, int fb, hipStream_t stream
 
 }  // namespace
 
-extern "C" int64_t advoc_matmul_nt_f8_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+extern "C" int64_t advoc_matmul_nt_f8_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t out_dtype) {
   if (m <= 0 || n <= 0 || k <= 0 || k > 0x7fffff00LL) return 0;
-  const Plan p = make_plan(m, n, (int)ceil_div(k, kBlock));
+  const Plan p = make_plan(m, n, (int)ceil_div(k, kBlock), out_dtype == ADVOC_F32);
   return p.splits > 1 ? 4 * p.splits * m * n : 0;
 }
 
@@ -347,7 +486,7 @@ extern "C" int advoc_matmul_nt_f8(const uint8_t* a, const uint8_t* a_scale, int3
   g.kp = (int64_t)g.blocks * kBlock;
   g.sp = ceil_div(g.blocks, 4) * 4;
   g.accumulate = accumulate != 0;
-  Plan p = make_plan(m, n, g.blocks);
+  Plan p = make_plan(m, n, g.blocks, out_dtype == ADVOC_F32);
   if (p.splits > 1 && (!workspace || workspace_bytes < 4 * p.splits * m * n)) p.splits = 1, p.per_split = g.blocks;
   if (p.splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 3)) return ADVOC_ERR_UNSUPPORTED;
   g.per_split = p.per_split;

@@ -44,6 +44,12 @@ __device__ __forceinline__ void dma16(u32x4s rsrc, unsigned lds_base, int voffse
                "s"(rsrc), "s"(soffset)
                : "memory", "m0");
 }
+// the same with 4 bytes per lane: lane l's land at lds_base + 4 l
+__device__ __forceinline__ void dma4(u32x4s rsrc, unsigned lds_base, int voffset, int soffset = 0) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(lds_base), "v"(voffset),
+               "s"(rsrc), "s"(soffset)
+               : "memory", "m0");
+}
 #pragma clang diagnostic pop
 
 // The rendezvous of an LDS-DMA ring: "my DMAs of the stage about to be read have landed (vmcnt <= VM), MY READS OF THE STAGE

@@ -413,7 +413,7 @@ def test_product_without_workspace_and_with(blocks):
   from advoc_amd import _lib
   lib = _lib.load()
   m, n, k = 200, 300, 5000
-  assert lib.advoc_matmul_nt_f8_workspace_bytes(m, n, k) > 0
+  assert lib.advoc_matmul_nt_f8_workspace_bytes(m, n, k, 0) > 0
   a, b = ints(m, k, 0), ints(n, k, 1)
   qa, qb = blocks.quantize_f8(a.cuda()), blocks.quantize_f8(b.cuda())
   out = torch.empty(m, n, device='cuda')
