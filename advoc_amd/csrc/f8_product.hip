@@ -2,8 +2,7 @@
 //
 // v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 128 by 128 x 16 values and applies an exponent byte per row and 32 values of k
 // to each operand: one instruction per block of 128, the block's byte in all four lane groups, accumulation in its fp32 registers
-// across blocks.  Which of the 128 positions of k a lane's 32 bytes are does not matter as long as both operands agree, so a lane
-// takes 32 consecutive bytes.
+// across blocks.  Which of the 128 positions of k a lane's 32 bytes are does not matter as long as both operands agree.
 // What that instruction adds up is not quite fp32: it aligns the products of eight consecutive k to the largest of them and drops
 // what is below 2^-13 of it (measured, also of the unscaled 16x16x32 form).  Against the definition the result is 1.5e-5 off in norm
 // -- 1/100 of the rounding of a 16-bit output, so those take it.  An fp32 output is computed EXACTly: the bytes become bf16 with the
@@ -152,8 +151,8 @@ __global__ __launch_bounds__(1024) void f8_thin_kernel(Args g) {
 // LDS-DMA while the stage before is multiplied; the exponent bytes of four blocks (a dword per row) are fetched the same way every
 // fourth block.  (Loads that the compiler counts must not follow a DMA in the loop: memory counters retire in order, and waiting for
 // such a load waits for the next stage too.  That alone held the first form of this kernel at 0.8 PFLOP/s.)
-// A row's eight 16-byte pieces lie at piece ^ key(row): the 16 rows that a fragment reads together have keys 0 ... 7 twice, so its
-// reads spread over all banks.
+// A row's eight 16-byte pieces lie at piece ^ key(row), and lane group g reads pieces g and g + 4: measured without bank conflicts, 4
+// cycles for a wave's 16 bytes a lane.  (Pieces 2 g and 2 g + 1 take 8.)
 template <int BM, int BN, int WM, int WN>
 struct Tile {
   static constexpr int kWaves = BM / WM * (BN / WN), kFm = WM / 16, kFn = WN / 16;
@@ -164,18 +163,19 @@ struct Tile {
   static constexpr int kExpDma = (kRows / 64 + kWaves - 1) / kWaves;      // or the exponents of 64 rows
   static_assert(kFn == 2 || kFn == 4, "a wave is two or four fragments of b wide");
   static_assert(kDma * 8 * kWaves == kRows && BM % (8 * kWaves) == 0, "whole DMA instructions per wave and operand");
-  static_assert(8 * kWaves % (2 << kShift) == 0, "rows fetched by one lane have one key");
+  static constexpr int kPer = kWaves < 8 && kFn == 4 ? 64 / (8 * kWaves) : 1;      // key_b repeats after 64 rows, or 32
+  static_assert(8 * kWaves * kPer % (4 << kShift) == 0 && 8 * kWaves % 16 == 0, "the keys of the rows that a lane fetches repeat");
   static_assert(BM % 64 == 0 && BN % 64 == 0, "64 rows of one operand per exponent fetch");
 
   advoc::u32x4s ra, rb, rea, reb;
   const uint8_t* lds;
   unsigned base;
   int lane, wave, wm, wn, spitch;
-  int kp, voff_a, voff_b;                // what this lane fetches: its first row of a and of b, the others are 8 kWaves rows on
+  int kp, voff_a, voff_b[kPer];          // what this lane fetches: its first row of a and of b, the others are 8 kWaves rows on
   int off_a, off_b, piece0, piece1;      // this lane's first rows in a stage, its two pieces of a row
 
-  static __device__ __forceinline__ int key_a(int row) { return row & 7; }
-  static __device__ __forceinline__ int key_b(int row) { return (row & 3) | ((row >> kShift) & 1) << 2; }
+  static __device__ __forceinline__ int key_a(int row) { return (row >> 1) & 7; }
+  static __device__ __forceinline__ int key_b(int row) { return ((row >> 1) & 1) | ((row >> kShift) & 3) << 1; }
 
   __device__ __forceinline__ Tile(const Args& g, const uint8_t* lds_, int64_t m0, int64_t n0) : lds(lds_) {
     lane = threadIdx.x & 63;
@@ -193,13 +193,14 @@ struct Tile {
     kp = (int)g.kp;
     const int first = wave * 8 + (lane >> 3);
     voff_a = first * kp + (((lane & 7) ^ key_a(first)) << 4);
-    voff_b = first * kp + (((lane & 7) ^ key_b(first)) << 4);
+#pragma unroll
+    for (int t = 0; t < kPer; ++t) voff_b[t] = first * kp + (((lane & 7) ^ key_b(first + t * 8 * kWaves)) << 4);
     // fragment i of a: rows wm + 16 i + lane % 16; fragment j of b: rows wn + 4 kFn (lane % 16 / 4) + 4 j + lane % 4.  Their keys are
-    // lane % 8 for every fragment
+    // lane / 2 % 8 for every fragment
     off_a = wm + (lane & 15);
     off_b = BM + wn + ((lane & 15) >> 2) * 4 * kFn + (lane & 3);
-    piece0 = (((lane >> 4) * 2) ^ (lane & 7)) << 4;
-    piece1 = (((lane >> 4) * 2 + 1) ^ (lane & 7)) << 4;
+    piece0 = ((lane >> 4) ^ ((lane >> 1) & 7)) << 4;
+    piece1 = piece0 ^ 64;
   }
 
   // block kb of the contraction into stage slot (kb - first) & 1, and with every fourth block the exponents of the next four
@@ -208,7 +209,7 @@ struct Tile {
     for (int t = 0; t < kDma; ++t) {
       const unsigned to = base + slot * kStage + (t * kWaves + wave) * 1024;
       if (t * 8 * kWaves < BM) advoc::dma16(ra, to, voff_a + t * 8 * kWaves * kp, kb * kBlock);
-      else advoc::dma16(rb, to, voff_b + (t * 8 * kWaves - BM) * kp, kb * kBlock);
+      else advoc::dma16(rb, to, voff_b[(t - BM / (8 * kWaves)) % kPer] + (t * 8 * kWaves - BM) * kp, kb * kBlock);
     }
   }
   __device__ __forceinline__ void fetch_exponents(int quad) const {
@@ -333,13 +334,19 @@ __global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
       for (int j = 0; j < T::kFn; ++j) eb[j] >>= 8;
     }
   };
+  // The instruction as assembly, so that it stays between its two rendezvous: the compiler sinks the builtin below the second one,
+  // out of its turn, and moves all accumulators once a block for it (349 against 314 us at 16384 x 4096 x 4096).  Each statement waits the two states that
+  // a vector instruction's result needs before a matrix instruction reads it; a fragment's accumulator comes round every 32
+  // instructions.
   auto multiply = [&]() {
     __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int i = 0; i < T::kFm; ++i)
 #pragma unroll
       for (int j = 0; j < T::kFn; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b[j], a[i], acc[i][j], FB, FA, 0, eb[j], 0, ea[i]);
+        asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
+                     : "+v"(acc[i][j])
+                     : "v"(b[j]), "v"(a[i]), "v"(eb[j]), "v"(ea[i]), "n"(FB), "n"(FA));
     __builtin_amdgcn_s_setprio(0);
   };
   auto fetch = [&](int kb) {
@@ -366,14 +373,19 @@ __global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
     meet(false);
   }
   for (int kb = 0; kb < g.blocks; ++kb) {
-    if (!late) fetch(kb + 1);
     read(kb);
+    if (!late) fetch(kb + 1);      // behind the reads: the address unit takes longer over these than LDS over those
     meet(late);
     if (late) fetch(kb + 2);
     multiply();
     meet(!late);
   }
   if (!late) meet(false);
+  asm volatile("s_nop 15\n\ts_nop 15");      // the last accumulators, before anything reads them
+#pragma unroll
+  for (int i = 0; i < T::kFm; ++i)
+#pragma unroll
+    for (int j = 0; j < T::kFn; ++j) asm volatile("" : "+v"(acc[i][j]));
   t.template store<O>(g, m0, n0, acc);
 }
 
