@@ -26,7 +26,7 @@ from advoc_amd import _lib
 NORMS = {'none': 0, 'rms': 1, 'layer': 2}
 GATE_ACTS = {'none': 0, 'sigmoid': 1}
 FORMATS = {'e4m3': 0, 'e5m2': 1}
-MAX_COLS = 16384
+MAX_COLS = 8192
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _MASK64 = 2 ** 64 - 1

@@ -5,8 +5,9 @@
 // A row of `cols` values is held by L lanes, V consecutive values at a time, NV times: value k of chunk j of lane l is column
 // (j L + l) V + k.  Up to 64 lanes a row is part of a wave and its sums are lane exchanges; wider rows are a workgroup's, whose
 // waves meet in LDS.  Everything a row needs is read once and stays in registers for both norms.
-// Where cols is no multiple of 8 the last chunk is moved back to end at the last column: it holds columns its neighbour holds
-// too (`dup` of them), computes the same values for them, stores the same values, and leaves them out of sums.
+// A chunk that would reach past the last column is moved back to end there: it holds columns its neighbour holds too (`dup` of them;
+// all V where the whole chunk lies behind the row), computes the same values for them, stores the same values, and leaves them out
+// of sums.  So no lane ever branches on where the row ends.
 #pragma once
 #include "philox.h"
 #include "rows.h"
@@ -90,7 +91,6 @@ static inline bool norm_dispatch(int cols, F&& f) {
   else if (cols <= 2048) f.template run<8, 256, 1, 256>();
   else if (cols <= 4096) f.template run<8, 256, 2, 256>();
   else if (cols <= 8192) f.template run<8, 512, 2, 512>();
-  else if (cols <= 16384) f.template run<8, 1024, 2, 1024>();
   else return false;
   return true;
 }
@@ -128,8 +128,33 @@ __device__ __forceinline__ uint32_t keep_chunk(uint64_t i, bool aligned, uint2 k
   return drop_keep1(i, key, thresh);
 }
 
-__device__ __forceinline__ float gate_act(float g, int act) {
-  return act == ADVOC_GATE_SIGMOID ? 1.f / (1.f + __expf(-g)) : g;
+// act(gate) in place
+template <int V>
+__device__ __forceinline__ void activate(f32x8& g, int act) {
+  if (act == ADVOC_GATE_SIGMOID)
+#pragma unroll
+    for (int k = 0; k < V; ++k) g[k] = 1.f / (1.f + expf(-g[k]));
+}
+
+// Sums over the columns that this lane owns: f(j, k) gives a term.  `ragged` (uniform) says whether a chunk can be owned in part.
+template <int V, int NV, typename F>
+__device__ __forceinline__ float own_sum(const int (&dup)[NV], bool ragged, F&& f) {
+  float sum = 0.f;
+  if (ragged) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < V; ++k) sum += k >= dup[j] ? f(j, k) : 0.f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float part = 0.f;
+#pragma unroll
+      for (int k = 0; k < V; ++k) part += f(j, k);
+      sum += dup[j] ? 0.f : part;
+    }
+  }
+  return sum;
 }
 
 }  // namespace advoc

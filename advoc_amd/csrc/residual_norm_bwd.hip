@@ -24,18 +24,12 @@ struct Sums {
   int slot[kSums];              // place in NormArgs.part, -1: not wanted
 };
 
-// g <- the gradient of a row given that of its normed values (times the weight): rstd (t - [mean t] - hat mean(t hat))
+// t <- the gradient of a row given that of its normed values (times the weight): rstd (t - [mean t] - hat mean(t hat))
 template <int V, int L, int NV, int WG>
-__device__ __forceinline__ void norm_back(f32x8 (&t)[NV], const f32x8 (&hat)[NV], const int (&dup)[NV], int kind, float inv_cols,
-                                          float rstd, float* red, int& turn) {
-  float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      s0 += k >= dup[j] ? t[j][k] : 0.f;
-      s1 += k >= dup[j] ? t[j][k] * hat[j][k] : 0.f;
-    }
+__device__ __forceinline__ void norm_back(f32x8 (&t)[NV], const f32x8 (&hat)[NV], const int (&dup)[NV], bool ragged, int kind,
+                                          float inv_cols, float rstd, float* red, int& turn) {
+  float s0 = advoc::own_sum<V>(dup, ragged, [&](int j, int k) { return t[j][k]; });
+  float s1 = advoc::own_sum<V>(dup, ragged, [&](int j, int k) { return t[j][k] * hat[j][k]; });
   Team<L, WG>::sum2(s0, s1, red, turn);
   s0 = kind == ADVOC_NORM_LAYER ? s0 * inv_cols : 0.f;
   s1 *= inv_cols;
@@ -43,17 +37,19 @@ __device__ __forceinline__ void norm_back(f32x8 (&t)[NV], const f32x8 (&hat)[NV]
   for (int j = 0; j < NV; ++j) t[j] = (t[j] - s0 - hat[j] * s1) * rstd;
 }
 
+// Two workgroups of 256 on a CU (256 registers a lane): the column vectors are read again for every row, from the caches -- held in
+// registers they left one wave to a SIMD.
 template <typename T, typename R, int V, int L, int NV, int WG>
-__global__ __launch_bounds__(WG) void norm_backward_kernel(NormArgs a, Sums sums) {
+__global__ __launch_bounds__(WG, 2) void norm_backward_kernel(NormArgs a, Sums sums) {
   using Row = Team<L, WG>;
   __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
   __shared__ float fold[L <= 64 ? Row::kRows * L * NV * V : 1];
   int turn = 0;
   const int lane = Row::lane();
   const uint2 key = advoc::drop_key_words(a.key);
-  const bool aligned = (a.cols & 3) == 0;
-  const int64_t group_rows = a.gate && a.gate_group > 1 ? a.gate_group : a.rows;
+  const bool aligned = (a.cols & 3) == 0, ragged = a.cols % V != 0;
   const bool shared_gate = a.gate && a.gate_group > 1;
+  const int group_rows = (int)(shared_gate ? a.gate_group : a.rows);
   int col[NV], dup[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, a.cols, col[j], dup[j]);
@@ -64,23 +60,26 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(NormArgs a, Sums sums
 #pragma unroll
     for (int j = 0; j < NV; ++j) acc[s][j] = (f32x8)(0.f);
 
-  const int64_t workers = (int64_t)gridDim.x * Row::kRows;
-  for (int64_t seg = (int64_t)blockIdx.x * Row::kRows + (L > 64 ? 0 : Row::slot()); seg < a.segments; seg += workers) {
-    const int64_t group = seg / a.splits, first = (seg - group * a.splits) * a.chunk;
-    const int64_t last = first + a.chunk < group_rows ? first + a.chunk : group_rows;
+  const int workers = (int)gridDim.x * Row::kRows;
+  for (int seg = (int)blockIdx.x * Row::kRows + (L > 64 ? 0 : Row::slot()); seg < a.segments; seg += workers) {
+    const int group = seg / a.splits, first = (seg - group * a.splits) * (int)a.chunk;
+    const int last = first + (int)a.chunk < group_rows ? first + (int)a.chunk : group_rows;
     f32x8 gacc[NV], gate[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       gacc[j] = (f32x8)(0.f);
       gate[j] = (f32x8)(1.f);
-      if (shared_gate && dup[j] < V) gate[j] = advoc::load_chunk<V>((const T*)a.gate + group * a.gate_pitch + col[j]);
+      if (shared_gate) {
+        gate[j] = advoc::load_chunk<V>((const T*)a.gate + group * a.gate_pitch + col[j]);
+        advoc::activate<V>(gate[j], a.act);
+      }
     }
-    for (int64_t row = group * group_rows + first; row < group * group_rows + last; ++row) {
+    for (int64_t row = (int64_t)group * group_rows + first; row < (int64_t)group * group_rows + last; ++row) {
+      asm volatile("" ::: "memory");            // (keeps the column vectors out of registers between rows)
       f32x8 hat[NV], t[NV], g[NV], u[NV];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         hat[j] = t[j] = g[j] = u[j] = (f32x8)(0.f);
-        if (dup[j] >= V) continue;
         if (a.pre != ADVOC_NORM_NONE) {
           t[j] = advoc::load_chunk<V>((const T*)a.dz + row * a.dz_pitch + col[j]);
           hat[j] = advoc::load_chunk<V>((const R*)a.x + row * a.x_pitch + col[j]);
@@ -94,64 +93,61 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(NormArgs a, Sums sums
       if (a.pre != ADVOC_NORM_NONE) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          if (dup[j] >= V) continue;
-          hat[j] = (hat[j] - st.z) * st.w;
+            hat[j] = (hat[j] - st.z) * st.w;
           acc[kDwPre][j] += t[j] * hat[j];
           acc[kDbPre][j] += t[j];
           t[j] *= advoc::cols_chunk<V>(a.w_pre, col[j], 1.f);
         }
-        norm_back<V, L, NV, WG>(t, hat, dup, a.pre, a.inv_cols, st.w, red, turn);
+        norm_back<V, L, NV, WG>(t, hat, dup, ragged, a.pre, a.inv_cols, st.w, red, turn);
 #pragma unroll
         for (int j = 0; j < NV; ++j) g[j] += t[j];
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (dup[j] < V && a.dx) advoc::store_chunk<V>((R*)a.dx + row * a.dx_pitch + col[j], g[j]);
+        if (a.dx) advoc::store_chunk<V>((R*)a.dx + row * a.dx_pitch + col[j], g[j]);
       if (!a.h) continue;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (dup[j] >= V) continue;
         hat[j] = u[j];
         if (a.post != ADVOC_NORM_NONE) {
           hat[j] = (u[j] - st.x) * st.y;
           u[j] = hat[j] * advoc::cols_chunk<V>(a.w_post, col[j], 1.f) + advoc::cols_chunk<V>(a.b_post, col[j], 0.f);
         }
         const uint32_t keep = advoc::keep_chunk<V>(a.key.offset + (uint64_t)(row * a.cols + col[j]), aligned, key, a.key.thresh);
-        const f32x8 s = advoc::cols_chunk<V>(a.scale, col[j], 1.f);
+        if (a.gate && !shared_gate) advoc::activate<V>(gate[j], a.act);
+        const f32x8 ks = advoc::cols_chunk<V>(a.scale, col[j], 1.f) * a.alpha;
         f32x8 dg;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float gt = a.gate ? advoc::gate_act(gate[j][k], a.act) : 1.f;
-          const float v = (keep >> k & 1) ? u[j][k] * a.key.scale : 0.f, ag = a.alpha * g[j][k];
-          acc[kDscale][j][k] += ag * gt * v;
-          dg[k] = ag * s[k] * v;
-          if (!shared_gate && a.act == ADVOC_GATE_SIGMOID) dg[k] *= gt * (1.f - gt);
-          t[j][k] = (keep >> k & 1) ? ag * s[k] * gt * a.key.scale : 0.f;
+          const float f = (keep >> k & 1) ? a.key.scale : 0.f;
+          const float v = (keep >> k & 1) ? u[j][k] * a.key.scale : 0.f, gv = g[j][k] * v;
+          acc[kDscale][j][k] += gv * gate[j][k];         // alpha is applied once, at the end
+          dg[k] = gv * ks[k];
+          t[j][k] = f * (ks[k] * gate[j][k] * g[j][k]);
+          if (!(keep >> k & 1)) t[j][k] = 0.f;
         }
-        if (shared_gate) gacc[j] += dg;
-        else if (a.gate && a.dgate) advoc::store_chunk<V>((T*)a.dgate + row * a.dgate_pitch + col[j], dg);
+        if (shared_gate) {
+          gacc[j] += dg;
+        } else if (a.gate && a.dgate) {
+          if (a.act == ADVOC_GATE_SIGMOID) dg *= gate[j] * (f32x8(1.f) - gate[j]);
+          advoc::store_chunk<V>((T*)a.dgate + row * a.dgate_pitch + col[j], dg);
+        }
         if (a.post != ADVOC_NORM_NONE) {
           acc[kDwPost][j] += t[j] * hat[j];
           acc[kDbPost][j] += t[j];
           t[j] *= advoc::cols_chunk<V>(a.w_post, col[j], 1.f);
         }
       }
-      if (a.post != ADVOC_NORM_NONE) norm_back<V, L, NV, WG>(t, hat, dup, a.post, a.inv_cols, st.y, red, turn);
+      if (a.post != ADVOC_NORM_NONE) norm_back<V, L, NV, WG>(t, hat, dup, ragged, a.post, a.inv_cols, st.y, red, turn);
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (dup[j] < V && a.dh) advoc::store_chunk<V>((T*)a.dh + row * a.dh_pitch + col[j], t[j]);
+        if (a.dh) advoc::store_chunk<V>((T*)a.dh + row * a.dh_pitch + col[j], t[j]);
     }
     if (shared_gate && a.dgate) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (dup[j] >= V) continue;
-        if (a.act == ADVOC_GATE_SIGMOID)
-#pragma unroll
-          for (int k = 0; k < V; ++k) {
-            const float gt = advoc::gate_act(gate[j][k], a.act);
-            gacc[j][k] *= gt * (1.f - gt);
-          }
-        if (a.gate_part) advoc::store_chunk<V>(a.gate_part + seg * a.cols + col[j], gacc[j]);
+        if (a.act == ADVOC_GATE_SIGMOID) gacc[j] *= gate[j] * (f32x8(1.f) - gate[j]);
+        if (a.gate_part) advoc::store_chunk<V>(a.gate_part + (int64_t)seg * a.cols + col[j], gacc[j]);
         else advoc::store_chunk<V>((T*)a.dgate + group * a.dgate_pitch + col[j], gacc[j]);
       }
     }
@@ -159,18 +155,20 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(NormArgs a, Sums sums
 
   // the workgroup's column sums: values of a column with two holders are equal, so either may store them
 #pragma unroll
+  for (int j = 0; j < NV; ++j) acc[kDscale][j] *= a.alpha;
+#pragma unroll
   for (int s = 0; s < kSums; ++s) {
     if (sums.slot[s] < 0) continue;
     float* out = a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * a.cols;
     if constexpr (L > 64) {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (dup[j] < V) advoc::store_chunk<V>(out + col[j], acc[s][j]);
+        advoc::store_chunk<V>(out + col[j], acc[s][j]);
     } else {
       __syncthreads();
 #pragma unroll
       for (int j = 0; j < NV; ++j)
-        if (dup[j] < V) advoc::store_chunk<V>(fold + Row::slot() * a.cols + col[j], acc[s][j]);
+        advoc::store_chunk<V>(fold + Row::slot() * a.cols + col[j], acc[s][j]);
       __syncthreads();
       for (int c = threadIdx.x; c < a.cols; c += WG) {
         float v = 0.f;
@@ -181,8 +179,8 @@ __global__ __launch_bounds__(WG) void norm_backward_kernel(NormArgs a, Sums sums
   }
 }
 
-// Adds up what the workgroups (column sums) and segments (shared gate rows) left, 64 columns to a block of four waves: wave w
-// takes entries w, w + 4, ...
+// Adds up what the workgroups (column sums) and segments (shared gate rows) left, 64 columns to a block of 16 waves: wave w takes
+// entries w, w + 16, ..., eight of them in flight.
 struct FoldArgs {
   const float *part, *gate_part;
   float* out[kSums];            // in the order of the slots
@@ -192,20 +190,32 @@ struct FoldArgs {
 };
 
 template <typename T>
-__global__ __launch_bounds__(256) void norm_fold_kernel(FoldArgs a) {
-  __shared__ float red[4][64];
-  const int item = blockIdx.x / a.col_blocks, c = (blockIdx.x - item * a.col_blocks) * 64 + (threadIdx.x & 63);
-  const int wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(1024) void norm_fold_kernel(FoldArgs a) {
+  constexpr int kWaves = 16, kDeep = 8;
+  __shared__ float red[kWaves][64];
+  const int item = blockIdx.x / a.col_blocks, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = (blockIdx.x - item * a.col_blocks) * 64 + lane;
   const bool is_gate = item >= a.sums;
   const int n = is_gate ? a.splits : a.entries;
   const float* p = is_gate ? a.gate_part + (int64_t)(item - a.sums) * n * a.cols : a.part + (int64_t)item * n * a.cols;
   float v = 0.f;
-  if (c < a.cols)
-    for (int e = wave; e < n; e += 4) v += p[(int64_t)e * a.cols + c];
-  red[wave][threadIdx.x & 63] = v;
+  if (c < a.cols) {
+    int e = wave;
+    for (; e + (kDeep - 1) * kWaves < n; e += kDeep * kWaves) {
+      float x[kDeep];
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) x[i] = p[(int64_t)(e + i * kWaves) * a.cols + c];
+#pragma unroll
+      for (int i = 0; i < kDeep; ++i) v += x[i];
+    }
+    for (; e < n; e += kWaves) v += p[(int64_t)e * a.cols + c];
+  }
+  red[wave][lane] = v;
   __syncthreads();
   if (wave == 0 && c < a.cols) {
-    v = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v += red[w][lane];
     if (is_gate) ((T*)a.dgate)[(int64_t)(item - a.sums) * a.dgate_pitch + c] = (T)v;
     else a.out[item][c] = a.accumulate ? a.out[item][c] + v : v;
   }
@@ -317,9 +327,9 @@ int launch_norm_backward(NormArgs a, int dtype, int res_dtype, float* const (&ou
   const int64_t items = p.sums + (p.gate_fold ? a.rows / a.gate_group : 0);
   const dim3 grid((unsigned)(items * f.col_blocks));
   ADVOC_CLEAR_LAUNCH_ERROR();
-  if (dtype == ADVOC_F32) hipLaunchKernelGGL(norm_fold_kernel<float>, grid, dim3(256), 0, stream, f);
-  else if (dtype == ADVOC_BF16) hipLaunchKernelGGL(norm_fold_kernel<__bf16>, grid, dim3(256), 0, stream, f);
-  else hipLaunchKernelGGL(norm_fold_kernel<_Float16>, grid, dim3(256), 0, stream, f);
+  if (dtype == ADVOC_F32) hipLaunchKernelGGL(norm_fold_kernel<float>, grid, dim3(1024), 0, stream, f);
+  else if (dtype == ADVOC_BF16) hipLaunchKernelGGL(norm_fold_kernel<__bf16>, grid, dim3(1024), 0, stream, f);
+  else hipLaunchKernelGGL(norm_fold_kernel<_Float16>, grid, dim3(1024), 0, stream, f);
   ADVOC_RETURN_IF_LAUNCH_FAILED();
   return ADVOC_OK;
 }

@@ -15,26 +15,19 @@ using advoc::Team;
 
 // mean and 1 / sqrt(var + eps) of a row
 template <int V, int L, int NV, int WG>
-__device__ __forceinline__ void row_stats(const f32x8 (&a)[NV], const int (&dup)[NV], int kind, float inv_cols, float eps,
+__device__ __forceinline__ void row_stats(const f32x8 (&a)[NV], const int (&dup)[NV], bool ragged, int kind, float inv_cols, float eps,
                                           float* red, int& turn, float& mean, float& rstd) {
   mean = 0.f;
   float none = 0.f;
   if (kind == ADVOC_NORM_LAYER) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int k = 0; k < V; ++k) mean += k >= dup[j] ? a[j][k] : 0.f;
+    mean = advoc::own_sum<V>(dup, ragged, [&](int j, int k) { return a[j][k]; });
     Team<L, WG>::sum2(mean, none, red, turn);
     mean *= inv_cols;
   }
-  float sq = 0.f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float d = a[j][k] - mean;
-      sq += k >= dup[j] ? d * d : 0.f;
-    }
+  float sq = advoc::own_sum<V>(dup, ragged, [&](int j, int k) {
+    const float d = a[j][k] - mean;
+    return d * d;
+  });
   Team<L, WG>::sum2(sq, none, red, turn);
   rstd = 1.f / sqrtf(sq * inv_cols + eps);
 }
@@ -46,7 +39,7 @@ __global__ __launch_bounds__(WG) void norm_forward_kernel(NormArgs a) {
   int turn = 0;
   const int lane = Row::lane();
   const uint2 key = advoc::drop_key_words(a.key);
-  const bool aligned = (a.cols & 3) == 0;
+  const bool aligned = (a.cols & 3) == 0, ragged = a.cols % V != 0;
   int col[NV], dup[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, a.cols, col[j], dup[j]);
@@ -55,38 +48,36 @@ __global__ __launch_bounds__(WG) void norm_forward_kernel(NormArgs a) {
        row += (int64_t)gridDim.x * Row::kRows) {
     f32x8 r[NV], u[NV], g[NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (dup[j] < V) {
+    for (int j = 0; j < NV; ++j) {
         r[j] = advoc::load_chunk<V>((const R*)a.x + row * a.x_pitch + col[j]);
         if (a.h) u[j] = advoc::load_chunk<V>((const T*)a.h + row * a.h_pitch + col[j]);
-        if (a.gate) g[j] = advoc::load_chunk<V>((const T*)a.gate + row / a.gate_group * a.gate_pitch + col[j]);
+        if (a.gate) g[j] = advoc::load_chunk<V>((const T*)a.gate + (int64_t)((uint32_t)row / (uint32_t)a.gate_group) * a.gate_pitch + col[j]);
       }
     if constexpr (L > 64) __syncthreads();      // outputs may be the inputs' own buffers, and a column may have two holders
     float mean0 = 0.f, rstd0 = 0.f, mean1 = 0.f, rstd1 = 0.f;
     if (a.h) {
-      if (a.post != ADVOC_NORM_NONE) row_stats<V, L, NV, WG>(u, dup, a.post, a.inv_cols, a.eps, red, turn, mean0, rstd0);
+      if (a.post != ADVOC_NORM_NONE) row_stats<V, L, NV, WG>(u, dup, ragged, a.post, a.inv_cols, a.eps, red, turn, mean0, rstd0);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (dup[j] >= V) continue;
         if (a.post != ADVOC_NORM_NONE) {
           const f32x8 w = advoc::cols_chunk<V>(a.w_post, col[j], 1.f), b = advoc::cols_chunk<V>(a.b_post, col[j], 0.f);
           u[j] = (u[j] - mean0) * rstd0 * w + b;
         }
         const uint32_t keep = advoc::keep_chunk<V>(a.key.offset + (uint64_t)(row * a.cols + col[j]), aligned, key, a.key.thresh);
-        const f32x8 s = advoc::cols_chunk<V>(a.scale, col[j], 1.f) * a.alpha;
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float gate = a.gate ? advoc::gate_act(g[j][k], a.act) : 1.f;
-          r[j][k] += s[k] * gate * ((keep >> k & 1) ? u[j][k] * a.key.scale : 0.f);
+        f32x8 s = advoc::cols_chunk<V>(a.scale, col[j], 1.f) * a.alpha;
+        if (a.gate) {
+          advoc::activate<V>(g[j], a.act);
+          s *= g[j];
         }
+#pragma unroll
+        for (int k = 0; k < V; ++k) r[j][k] += s[k] * ((keep >> k & 1) ? u[j][k] * a.key.scale : 0.f);
         advoc::store_chunk<V>((R*)a.r + row * a.r_pitch + col[j], r[j]);
       }
     }
     if (a.pre != ADVOC_NORM_NONE) {
-      row_stats<V, L, NV, WG>(r, dup, a.pre, a.inv_cols, a.eps, red, turn, mean1, rstd1);
+      row_stats<V, L, NV, WG>(r, dup, ragged, a.pre, a.inv_cols, a.eps, red, turn, mean1, rstd1);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (dup[j] >= V) continue;
         const f32x8 w = advoc::cols_chunk<V>(a.w_pre, col[j], 1.f), b = advoc::cols_chunk<V>(a.b_pre, col[j], 0.f);
         advoc::store_chunk<V>((T*)a.z + row * a.z_pitch + col[j], (r[j] - mean1) * rstd1 * w + b);
       }

@@ -6,7 +6,38 @@
 
 namespace advoc {
 
-typedef float f32x8 __attribute__((ext_vector_type(8)));
+// eight fp32 values in eight registers of their own (a 256-bit vector type would tie them together)
+struct f32x8 {
+  float v[8];
+  f32x8() = default;
+  __device__ __forceinline__ explicit f32x8(float x) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = x;
+  }
+  __device__ __forceinline__ float& operator[](int k) { return v[k]; }
+  __device__ __forceinline__ float operator[](int k) const { return v[k]; }
+};
+#define ADVOC_F32X8_OP(OP)                                                     \
+  __device__ __forceinline__ f32x8 operator OP(f32x8 a, const f32x8& b) {      \
+    _Pragma("unroll") for (int k = 0; k < 8; ++k) a.v[k] = a.v[k] OP b.v[k];   \
+    return a;                                                                  \
+  }                                                                            \
+  __device__ __forceinline__ f32x8 operator OP(f32x8 a, float b) {             \
+    _Pragma("unroll") for (int k = 0; k < 8; ++k) a.v[k] = a.v[k] OP b;        \
+    return a;                                                                  \
+  }                                                                            \
+  __device__ __forceinline__ f32x8& operator OP##=(f32x8& a, const f32x8& b) { \
+    _Pragma("unroll") for (int k = 0; k < 8; ++k) a.v[k] = a.v[k] OP b.v[k];   \
+    return a;                                                                  \
+  }                                                                            \
+  __device__ __forceinline__ f32x8& operator OP##=(f32x8& a, float b) {        \
+    _Pragma("unroll") for (int k = 0; k < 8; ++k) a.v[k] = a.v[k] OP b;        \
+    return a;                                                                  \
+  }
+ADVOC_F32X8_OP(+)
+ADVOC_F32X8_OP(-)
+ADVOC_F32X8_OP(*)
+#undef ADVOC_F32X8_OP
 
 template <typename T>
 struct vec8 {
@@ -17,13 +48,18 @@ template <typename T>
 __device__ __forceinline__ f32x8 load8(const T* p) {
   typename vec8<T>::type v;
   __builtin_memcpy(&v, p, sizeof(v));
-  return __builtin_convertvector(v, f32x8);
+  f32x8 f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) f.v[k] = (float)v[k];
+  return f;
 }
 
 // nearest, ties to even (v_cvt_pk_bf16_f32 and v_cvt_f16_f32 in the default mode)
 template <typename T>
-__device__ __forceinline__ void store8(T* p, f32x8 f) {
-  const typename vec8<T>::type v = __builtin_convertvector(f, typename vec8<T>::type);
+__device__ __forceinline__ void store8(T* p, const f32x8& f) {
+  typename vec8<T>::type v;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = (T)f.v[k];
   __builtin_memcpy(p, &v, sizeof(v));
 }
 

@@ -568,7 +568,7 @@ int advoc_dropout(const void* x, int64_t x_pitch, void* y, int64_t y_pitch, int6
 #define ADVOC_NORM_LAYER 2 /* (a - mean a) / sqrt(var a + eps), biased variance */
 #define ADVOC_GATE_NONE 0
 #define ADVOC_GATE_SIGMOID 1
-#define ADVOC_NORM_MAX_COLS 16384
+#define ADVOC_NORM_MAX_COLS 8192
 
 typedef struct advoc_rows {
   void* p;       /* NULL: absent */

@@ -132,7 +132,7 @@ def _norm_desc(**kw):
 @pytest.mark.parametrize('bad,code', [
     (dict(rows=-1), -1), (dict(cols=0), -1), (dict(eps=0.0), -1), (dict(eps=float('nan')), -1), (dict(keep_prob=0.0), -1),
     (dict(keep_prob=1.1), -1), (dict(norm_post=3), -2), (dict(norm_pre=-1), -2), (dict(gate_act=2), -2), (dict(dtype=3), -2),
-    (dict(dtype=1, res_dtype=2), -2), (dict(cols=16385), -2), (dict(rows=2 ** 31), -2), (dict(offset=1), -2),
+    (dict(dtype=1, res_dtype=2), -2), (dict(cols=8193), -2), (dict(rows=2 ** 31), -2), (dict(offset=1), -2),
     (dict(gate=(64, 8), gate_group=3), -1), (dict(gate=(64, 8), gate_group=0), -1), (dict(gate=(64, 7)), -1), (dict(h=(64, 7)), -1),
     (dict(x=(64, 7)), -1), (dict(z=(64, 7)), -1), (dict(r=(64, 7)), -1), (dict(h=(None, 0)), -1), (dict(stats=68), -2)])
 def test_norm_entries_refuse(lib, bad, code):
@@ -188,7 +188,7 @@ def test_binding_refuses_what_is_not_on_a_device():
 
 
 def test_binding_refuses_bad_options():
-  for kw in (dict(cols=0), dict(cols=16385), dict(cols=8, post='batch'), dict(cols=8, pre=None), dict(cols=8, gate_act='tanh'),
+  for kw in (dict(cols=0), dict(cols=8193), dict(cols=8, post='batch'), dict(cols=8, pre=None), dict(cols=8, gate_act='tanh'),
              dict(cols=8, eps=0.0), dict(cols=8, keep_prob=0.0), dict(cols=8, keep_prob=1.5),
              dict(cols=8, post='none', w_post=torch.zeros(8)), dict(cols=8, pre='none', b_pre=torch.zeros(8))):
     with pytest.raises(_lib.AdvocHipError):

@@ -1,7 +1,7 @@
 """GPU tests of advoc_amd.blocks against oracle/blocks_torch.py in float64.
 
 Tolerances, from the arithmetic alone.  u = 2^-24 is half a step of fp32; half a step of an output type is eps / 2 of the value.
-  * a row's sum is at most 16 terms in a lane, 6 exchanges and 16 waves: 38 roundings; two sums per norm, two norms, and under 100
+  * a row's sum is at most 16 terms in a lane, 6 exchanges and 8 waves: 30 roundings; two sums per norm, two norms, and under 100
     roundings of single operations around them (the sigmoid's exponential counts 4): a row output is within 256 u of the largest
     term of its row, before its own rounding;
   * a column sum adds a worker's rows, the workers of a workgroup (at most 16) and a quarter of the workgroups (at most 128) in turn:
@@ -186,8 +186,7 @@ def test_norm_types_and_options(blocks, dt, res, kind):
   check_norm(blocks, kind, (3, 37), 200, dt, res, *KINDS[kind])
 
 
-@pytest.mark.parametrize('cols', [1, 2, 7, 8, 9, 16, 80, 127, 128, 129, 256, 257, 512, 513, 1000, 1024, 1025, 2048, 2049, 4096, 4099, 8192, 8193,
-                                  16384])
+@pytest.mark.parametrize('cols', [1, 2, 7, 8, 9, 16, 80, 127, 128, 129, 256, 257, 512, 513, 1000, 1024, 1025, 2048, 2049, 4096, 4099, 8191, 8192])
 def test_norm_widths(blocks, cols):
   """Every instance of the kernels, at its edges, whole chunks and ragged ones."""
   check_norm(blocks, cols, (2, 5), cols, 'bf16', 'f32', *KINDS[1 + cols % 2])
