@@ -34,15 +34,31 @@ struct NormArgs {
   int64_t dh_pitch, dx_pitch, dgate_pitch;
   float* part;                  // [sum][workgroup][cols]
   float* gate_part;             // [gate row][splits][cols], NULL: a gate row's sum is complete in one worker
-  int64_t chunk;                // rows of a segment
+  float* carry;                 // per worker, where workers see several gate rows: see residual_norm_bwd.hip
   int64_t segments;
   int splits;                   // segments of a gate row
 };
 
-// 8 values of a column vector, or 8 times `otherwise`
-__device__ __forceinline__ f32x8 cols8(const float* p, int col, float otherwise) {
-  if (!p) return (f32x8)(otherwise);
-  return load8(p + col);
+// v of the lane that a data-parallel-primitive control names, within rows of 16 lanes
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_value(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
+// Sum over groups of N consecutive lanes, in every lane of the group.  Within 16 lanes the partners come with the addition itself
+// (eight cycles a step); a shuffle goes through LDS (over a hundred), and a row's sums are on the way of everything behind them.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += dpp<0xB1>(v);                       // quad_perm 1 0 3 2
+  v += dpp<0x4E>(v);                       // quad_perm 2 3 0 1
+  v += dpp<0x141>(v);                      // row_half_mirror: the other quad of eight
+  if constexpr (N >= 16) v += dpp<0x140>(v);      // row_mirror: the other eight of sixteen
+  if constexpr (N == 32) v += __shfl_xor(v, 16, 64);
+  if constexpr (N == 64) v = (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
+  return v;
 }
 
 // The lanes of one row.  WG lanes per workgroup, L per row.
@@ -50,16 +66,21 @@ template <int L, int WG>
 struct Team {
   static constexpr int kRows = WG / L;
   static __device__ __forceinline__ int lane() { return threadIdx.x % L; }
-  static __device__ __forceinline__ int slot() { return threadIdx.x / L; }
+  // (a wave's rows are said to be uniform: addresses are then a scalar base and a 32-bit offset that all tensors of a type share)
+  static __device__ __forceinline__ int slot() {
+    if constexpr (L > 64) return 0;
+    else if constexpr (L == 64) return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    else return threadIdx.x / L;
+  }
+
+  // A rendezvous of the workgroup that leaves loads in flight; LDS written before it can be read behind it.
+  static __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
   // sums over the row's lanes, in an order that depends on L alone; `red` is LDS for L > 64 (2 floats a wave, twice: a second
   // call may write while a slow wave still reads what the first left)
   static __device__ __forceinline__ void sum2(float& a, float& b, float* red, int& turn) {
-#pragma unroll
-    for (int off = (L < 64 ? L : 64) / 2; off > 0; off >>= 1) {
-      a += __shfl_xor(a, off, 64);
-      b += __shfl_xor(b, off, 64);
-    }
+    a = lanes_sum<(L < 64 ? L : 64)>(a);
+    b = lanes_sum<(L < 64 ? L : 64)>(b);
     if constexpr (L > 64) {
       constexpr int kWaves = L / 64;
       float* buf = red + turn * 2 * kWaves;
@@ -68,7 +89,7 @@ struct Team {
         buf[2 * (threadIdx.x >> 6)] = a;
         buf[2 * (threadIdx.x >> 6) + 1] = b;
       }
-      __syncthreads();
+      meet();
       a = b = 0.f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
@@ -83,14 +104,14 @@ struct Team {
 // (V = 1 only below 8 columns, where a chunk of 8 does not fit.)
 template <typename F>
 static inline bool norm_dispatch(int cols, F&& f) {
-  if (cols < 8) f.template run<1, 8, 1, 256>();
-  else if (cols <= 128) f.template run<8, 16, 1, 256>();
-  else if (cols <= 256) f.template run<8, 32, 1, 256>();
-  else if (cols <= 512) f.template run<8, 64, 1, 256>();
-  else if (cols <= 1024) f.template run<8, 64, 2, 256>();
-  else if (cols <= 2048) f.template run<8, 256, 1, 256>();
-  else if (cols <= 4096) f.template run<8, 256, 2, 256>();
-  else if (cols <= 8192) f.template run<8, 512, 2, 512>();
+  if (cols < 8) f.template run<1, 8, 1>();
+  else if (cols <= 128) f.template run<8, 16, 1>();
+  else if (cols <= 256) f.template run<8, 32, 1>();
+  else if (cols <= 512) f.template run<8, 64, 1>();
+  else if (cols <= 1024) f.template run<8, 64, 2>();
+  else if (cols <= 2048) f.template run<8, 256, 1>();
+  else if (cols <= 4096) f.template run<8, 256, 2>();
+  else if (cols <= 8192) f.template run<8, 512, 2>();
   else return false;
   return true;
 }
@@ -103,22 +124,55 @@ __device__ __forceinline__ void chunk_place(int j, int lane, int cols, int& col,
   dup = at < cols ? at - col : V;
 }
 
-template <int V, typename T>
-__device__ __forceinline__ f32x8 load_chunk(const T* p) {
-  if constexpr (V == 8) return load8(p);
-  f32x8 v = (f32x8)(0.f);
-  v[0] = (float)*p;
-  return v;
+// column `col` of the row that starts at element `at` of `base`
+template <typename T>
+__device__ __forceinline__ T* row_at(void* base, int64_t at, int col) {
+  return reinterpret_cast<T*>(static_cast<char*>(base) + at * (int64_t)sizeof(T) + (uint32_t)col * (uint32_t)sizeof(T));
 }
+template <typename T>
+__device__ __forceinline__ const T* row_at(const void* base, int64_t at, int col) {
+  return reinterpret_cast<const T*>(static_cast<const char*>(base) + at * (int64_t)sizeof(T) + (uint32_t)col * (uint32_t)sizeof(T));
+}
+
+// NV chunks of a row as they lie in memory: loaded early, converted when they are used
+template <typename T, int V, int NV>
+struct Raw {
+  typename vec8<T>::type v[NV];
+  __device__ __forceinline__ void load(const void* base, int64_t at, const int (&col)[NV]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const T* p = row_at<T>(base, at, col[j]);
+      if constexpr (V == 8) __builtin_memcpy(&v[j], p, sizeof(v[j]));
+      else v[j][0] = *p;
+    }
+  }
+  __device__ __forceinline__ f32x8 operator[](int j) const {
+    f32x8 f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = k < V ? (float)v[j][k] : 0.f;
+    return f;
+  }
+};
 template <int V, typename T>
-__device__ __forceinline__ void store_chunk(T* p, f32x8 v) {
+__device__ __forceinline__ void store_chunk(T* p, const f32x8& v) {
   if constexpr (V == 8) store8(p, v);
   else *p = (T)v[0];
 }
+
+// The column vectors of a call in LDS, [which][cols], an absent one as its neutral value: a lane reads its columns of them for every
+// row (kept in registers they cost the waves that hide the loads' latency; from the caches, a round trip per vector and row).
+// (the compiler would carry what it has read of them from row to row in registers, and spill)
+__device__ __forceinline__ void forget_lds() { asm volatile("" ::: "memory"); }
+template <int WG>
+__device__ __forceinline__ void stage_vector(float* lds, const float* p, float otherwise, int cols) {
+  for (int c = threadIdx.x; c < cols; c += WG) lds[c] = p ? p[c] : otherwise;
+}
 template <int V>
-__device__ __forceinline__ f32x8 cols_chunk(const float* p, int col, float otherwise) {
-  if (!p) return (f32x8)(otherwise);
-  return load_chunk<V>(p + col);
+__device__ __forceinline__ f32x8 cols_chunk(const float* p) {
+  f32x8 f(0.f);
+  if constexpr (V == 8) __builtin_memcpy(f.v, p, sizeof(f.v));
+  else f[0] = *p;
+  return f;
 }
 
 template <int V>

@@ -1,15 +1,17 @@
 // Backward pass of the residual norm (gfx950), with the statistics the forward pass left:
 //
 //   rhat = (r - mean1) rstd1;  t = dz w_pre;     g  = dr + rstd1 (t - [mean t] - rhat mean(t rhat))        ([..]: LAYER only)
-//   hhat = (h - mean0) rstd0;  v = drop(hhat w_post + b_post);   k = alpha scale act(gate)
-//   dx = g;   dscale = sum alpha act(gate) v g;   dgate = sum alpha scale v g act'(gate);   du = drop(k g)
-//   t = du w_post;             dh = rstd0 (t - [mean t] - hhat mean(t hhat))
-//   dw_post = sum du hhat, db_post = sum du;      dw_pre = sum dz rhat, db_pre = sum dz
+//   hhat = (h - mean0) rstd0;  e = drop(alpha g);   E0 = sum e act(gate),  E1 = sum e act(gate) hhat
+//   dx = g;   du = e scale act(gate);   t = du w_post;   dh = rstd0 (t - [mean t] - hhat mean(t hhat))
+//   dgate = sum e scale (hhat w_post + b_post) act'(gate)
+//   dw_post = scale E1,  db_post = scale E0,  dscale = w_post E1 + b_post E0;      dw_pre = sum dz rhat, db_pre = sum dz
 //
-// One pass: the five inputs of a row are read once and the three outputs written once; u and v are computed again instead of being
-// stored by the forward pass.  The column sums live in registers while a worker (the lanes of one row) walks over its rows, meet in
-// LDS per workgroup and in HBM once per workgroup; a second small launch adds those up in a fixed order (no atomics: two runs give
-// the same bits).  A gate row shared by the frames of a clip is summed the same way, a worker's rows never crossing a clip.
+// Four column sums give the five parameter gradients: what is constant in a column stays outside its sums.  One pass: the five
+// inputs of a row are read once and the three outputs written once; the mask is drawn again.  The sums live in registers while a
+// worker (the lanes of one row) walks over its rows, meet in LDS per workgroup and in HBM once per workgroup; a second small launch
+// adds those up in a fixed order (no atomics: two runs give the same bits).  A gate row shared by the frames of a clip is summed the
+// same way, a worker's rows never crossing a clip: G0 = sum e, G1 = sum e hhat over them give dgate = scale (w_post G1 + b_post G0)
+// act' and their part of E0, E1.
 #include "residual_norm.h"
 
 namespace {
@@ -24,6 +26,13 @@ struct Sums {
   int slot[kSums];              // place in NormArgs.part, -1: not wanted
 };
 
+// Lanes of a workgroup and waves per SIMD.  Rows of 16 columns a lane: 256 registers, a third of them sums, and 512 lanes to a
+// workgroup (half the partial column sums of 256); rows of 8: three waves to a SIMD.
+template <int L, int NV>
+constexpr int kLanes = L > 64 ? L : NV > 1 ? 512 : 256;
+template <int NV>
+constexpr int kWavesPerSimd = NV > 1 ? 2 : 3;
+
 // t <- the gradient of a row given that of its normed values (times the weight): rstd (t - [mean t] - hat mean(t hat))
 template <int V, int L, int NV, int WG>
 __device__ __forceinline__ void norm_back(f32x8 (&t)[NV], const f32x8 (&hat)[NV], const int (&dup)[NV], bool ragged, int kind,
@@ -37,143 +46,186 @@ __device__ __forceinline__ void norm_back(f32x8 (&t)[NV], const f32x8 (&hat)[NV]
   for (int j = 0; j < NV; ++j) t[j] = (t[j] - s0 - hat[j] * s1) * rstd;
 }
 
-// Two workgroups of 256 on a CU (256 registers a lane): the column vectors are read again for every row, from the caches -- held in
-// registers they left one wave to a SIMD.
-template <typename T, typename R, int V, int L, int NV, int WG>
-__global__ __launch_bounds__(WG, 2) void norm_backward_kernel(NormArgs a, Sums sums) {
+// H: there is a block output (otherwise only the pre norm is differentiated); PRE: there is a pre norm.  Everything else that may be
+// absent is not a branch (register allocation around those cost more than the work they save): an absent dr or gate is read from
+// where r or h lies and replaced by its neutral value, absent vectors are staged as theirs.
+template <typename T, typename R, int V, int L, int NV, int WG, bool H, bool PRE>
+__global__ __launch_bounds__(WG, kWavesPerSimd<NV>) void norm_backward_kernel(NormArgs a, Sums sums) {
   using Row = Team<L, WG>;
   __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
-  __shared__ float fold[L <= 64 ? Row::kRows * L * NV * V : 1];
+  extern __shared__ float vec[];                // w_pre, w_post, b_post, scale; afterwards the column sums of the workgroup's rows
   int turn = 0;
-  const int lane = Row::lane();
+  const int lane = Row::lane(), cols = a.cols;
   const uint2 key = advoc::drop_key_words(a.key);
-  const bool aligned = (a.cols & 3) == 0, ragged = a.cols % V != 0;
-  const bool shared_gate = a.gate && a.gate_group > 1;
+  const bool aligned = (cols & 3) == 0, ragged = cols % V != 0;
+  const bool has_dr = a.dr, has_gate = a.gate, shared_gate = has_gate && a.gate_group > 1, row_gate = has_gate && !shared_gate;
+  const bool post = a.post != ADVOC_NORM_NONE;
   const int group_rows = (int)(shared_gate ? a.gate_group : a.rows);
+  const void* dr = has_dr ? a.dr : a.x;
+  const void* gate_base = has_gate ? a.gate : a.h;
+  const int64_t dr_pitch = has_dr ? a.dr_pitch : a.x_pitch, gate_pitch = has_gate ? a.gate_pitch : a.h_pitch;
   int col[NV], dup[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, a.cols, col[j], dup[j]);
+  for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, cols, col[j], dup[j]);
 
-  f32x8 acc[kSums][NV];
+  advoc::stage_vector<WG>(vec, a.w_pre, 1.f, cols);
+  advoc::stage_vector<WG>(vec + cols, a.w_post, 1.f, cols);
+  advoc::stage_vector<WG>(vec + 2 * cols, a.b_post, 0.f, cols);
+  advoc::stage_vector<WG>(vec + 3 * cols, a.scale, 1.f, cols);
+  auto w_pre = [&](int j) { return advoc::cols_chunk<V>(vec + col[j]); };
+  auto w_post = [&](int j) { return advoc::cols_chunk<V>(vec + cols + col[j]); };
+  auto b_post = [&](int j) { return advoc::cols_chunk<V>(vec + 2 * cols + col[j]); };
+  auto scale = [&](int j) { return advoc::cols_chunk<V>(vec + 3 * cols + col[j]); };
+  Row::meet();
+
+  // sums over rows.  g0, g1 are E0, E1 but for the gate where rows share one
+  f32x8 dw_pre[NV], db_pre[NV], g0[NV], g1[NV];
 #pragma unroll
-  for (int s = 0; s < kSums; ++s)
-#pragma unroll
-    for (int j = 0; j < NV; ++j) acc[s][j] = (f32x8)(0.f);
+  for (int j = 0; j < NV; ++j) dw_pre[j] = db_pre[j] = g0[j] = g1[j] = f32x8(0.f);
+  // a worker with several clips carries E0, E1 of those before in memory of its own
+  constexpr int kOwn = NV * L * V;
+  float* const carry = a.carry ? a.carry + ((int64_t)blockIdx.x * Row::kRows + Row::slot()) * 2 * kOwn + lane * V : nullptr;
 
   const int workers = (int)gridDim.x * Row::kRows;
-  for (int seg = (int)blockIdx.x * Row::kRows + (L > 64 ? 0 : Row::slot()); seg < a.segments; seg += workers) {
-    const int group = seg / a.splits, first = (seg - group * a.splits) * (int)a.chunk;
-    const int last = first + (int)a.chunk < group_rows ? first + (int)a.chunk : group_rows;
-    f32x8 gacc[NV], gate[NV];
+  const float kept = a.alpha * a.key.scale;
+  bool again = false;
+  for (int seg = (int)blockIdx.x * Row::kRows + Row::slot(); seg < a.segments; seg += workers) {
+    // part p of a group takes rows p, p + splits, ...: what runs together lies together
+    const int group = seg / a.splits, first = seg - group * a.splits;
+    const int64_t end = (int64_t)(group + 1) * group_rows;
+    if (H && carry)
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      gacc[j] = (f32x8)(0.f);
-      gate[j] = (f32x8)(1.f);
-      if (shared_gate) {
-        gate[j] = advoc::load_chunk<V>((const T*)a.gate + group * a.gate_pitch + col[j]);
-        advoc::activate<V>(gate[j], a.act);
+      for (int j = 0; j < NV; ++j) g0[j] = g1[j] = f32x8(0.f);
+    advoc::Raw<T, V, NV> raw_gate, raw_dz, raw_h;
+    advoc::Raw<R, V, NV> raw_r, raw_dr;
+    auto load = [&](int64_t row) {
+      if constexpr (PRE) {
+        raw_dz.load(a.dz, row * a.dz_pitch, col);
+        raw_r.load(a.x, row * a.x_pitch, col);
       }
-    }
-    for (int64_t row = (int64_t)group * group_rows + first; row < (int64_t)group * group_rows + last; ++row) {
-      asm volatile("" ::: "memory");            // (keeps the column vectors out of registers between rows)
-      f32x8 hat[NV], t[NV], g[NV], u[NV];
+      raw_dr.load(dr, row * dr_pitch, col);
+      if constexpr (H) {
+        raw_h.load(a.h, row * a.h_pitch, col);
+        raw_gate.load(gate_base, (shared_gate ? group : row) * gate_pitch, col);
+      }
+    };
+    for (int64_t row = end - group_rows + first; row < end; row += a.splits) {
+      advoc::forget_lds();
+      load(row);
+      f32x8 hat[NV], t[NV], g[NV], gate[NV];
+      const float4 st = PRE || post ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        hat[j] = t[j] = g[j] = u[j] = (f32x8)(0.f);
-        if (a.pre != ADVOC_NORM_NONE) {
-          t[j] = advoc::load_chunk<V>((const T*)a.dz + row * a.dz_pitch + col[j]);
-          hat[j] = advoc::load_chunk<V>((const R*)a.x + row * a.x_pitch + col[j]);
-        }
-        if (a.dr) g[j] = advoc::load_chunk<V>((const R*)a.dr + row * a.dr_pitch + col[j]);
-        if (a.h) u[j] = advoc::load_chunk<V>((const T*)a.h + row * a.h_pitch + col[j]);
-        if (a.gate && !shared_gate) gate[j] = advoc::load_chunk<V>((const T*)a.gate + row * a.gate_pitch + col[j]);
-      }
-      if constexpr (L > 64) __syncthreads();    // outputs may be the inputs' own buffers, and a column may have two holders
-      const float4 st = a.stats ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
-      if (a.pre != ADVOC_NORM_NONE) {
+        g[j] = raw_dr[j];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            hat[j] = (hat[j] - st.z) * st.w;
-          acc[kDwPre][j] += t[j] * hat[j];
-          acc[kDbPre][j] += t[j];
-          t[j] *= advoc::cols_chunk<V>(a.w_pre, col[j], 1.f);
+        for (int k = 0; k < V; ++k) g[j][k] = has_dr ? g[j][k] : 0.f;
+        if constexpr (PRE) {
+          t[j] = raw_dz[j];
+          hat[j] = (raw_r[j] - st.z) * st.w;
+          dw_pre[j] += t[j] * hat[j];
+          db_pre[j] += t[j];
+          t[j] *= w_pre(j);
         }
+      }
+      if constexpr (PRE) {
         norm_back<V, L, NV, WG>(t, hat, dup, ragged, a.pre, a.inv_cols, st.w, red, turn);
 #pragma unroll
         for (int j = 0; j < NV; ++j) g[j] += t[j];
       }
+      if constexpr (H) {
+        const float mean = post ? st.x : 0.f, rstd = post ? st.y : 1.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (a.dx) advoc::store_chunk<V>((R*)a.dx + row * a.dx_pitch + col[j], g[j]);
-      if (!a.h) continue;
+        for (int j = 0; j < NV; ++j) {
+          hat[j] = (raw_h[j] - mean) * rstd;
+          gate[j] = raw_gate[j];
+        }
+      }
+      if constexpr (L > 64) Row::meet();        // outputs may be the inputs' own buffers, and a column may have two holders
+      if (a.dx)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) advoc::store_chunk<V>(advoc::row_at<R>(a.dx, row * a.dx_pitch, col[j]), g[j]);
+      if constexpr (!H) continue;
+      advoc::forget_lds();
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        hat[j] = u[j];
-        if (a.post != ADVOC_NORM_NONE) {
-          hat[j] = (u[j] - st.x) * st.y;
-          u[j] = hat[j] * advoc::cols_chunk<V>(a.w_post, col[j], 1.f) + advoc::cols_chunk<V>(a.b_post, col[j], 0.f);
-        }
-        const uint32_t keep = advoc::keep_chunk<V>(a.key.offset + (uint64_t)(row * a.cols + col[j]), aligned, key, a.key.thresh);
-        if (a.gate && !shared_gate) advoc::activate<V>(gate[j], a.act);
-        const f32x8 ks = advoc::cols_chunk<V>(a.scale, col[j], 1.f) * a.alpha;
-        f32x8 dg;
+        const uint32_t keep = advoc::keep_chunk<V>(a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
+        advoc::activate<V>(gate[j], a.act);
+        const f32x8 s = scale(j);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float f = (keep >> k & 1) ? a.key.scale : 0.f;
-          const float v = (keep >> k & 1) ? u[j][k] * a.key.scale : 0.f, gv = g[j][k] * v;
-          acc[kDscale][j][k] += gv * gate[j][k];         // alpha is applied once, at the end
-          dg[k] = gv * ks[k];
-          t[j][k] = f * (ks[k] * gate[j][k] * g[j][k]);
-          if (!(keep >> k & 1)) t[j][k] = 0.f;
+          gate[j][k] = has_gate ? gate[j][k] : 1.f;
+          t[j][k] = (keep >> k & 1) ? g[j][k] * kept : 0.f;
         }
-        if (shared_gate) {
-          gacc[j] += dg;
-        } else if (a.gate && a.dgate) {
+        if (row_gate && a.dgate) {
+          f32x8 dg = t[j] * s * (hat[j] * w_post(j) + b_post(j));
           if (a.act == ADVOC_GATE_SIGMOID) dg *= gate[j] * (f32x8(1.f) - gate[j]);
-          advoc::store_chunk<V>((T*)a.dgate + row * a.dgate_pitch + col[j], dg);
+          advoc::store_chunk<V>(advoc::row_at<T>(a.dgate, row * a.dgate_pitch, col[j]), dg);
         }
-        if (a.post != ADVOC_NORM_NONE) {
-          acc[kDwPost][j] += t[j] * hat[j];
-          acc[kDbPost][j] += t[j];
-          t[j] *= advoc::cols_chunk<V>(a.w_post, col[j], 1.f);
-        }
+        const f32x8 e = t[j] * gate[j];
+        f32x8 sum = shared_gate ? t[j] : e;
+        g0[j] += sum;
+        g1[j] += sum * hat[j];
+        t[j] = e * s * w_post(j);               // (w_post is staged as ones without a post norm)
       }
-      if (a.post != ADVOC_NORM_NONE) norm_back<V, L, NV, WG>(t, hat, dup, ragged, a.post, a.inv_cols, st.y, red, turn);
+      if (post) norm_back<V, L, NV, WG>(t, hat, dup, ragged, a.post, a.inv_cols, st.y, red, turn);
+      if (a.dh)
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (a.dh) advoc::store_chunk<V>((T*)a.dh + row * a.dh_pitch + col[j], t[j]);
+        for (int j = 0; j < NV; ++j) advoc::store_chunk<V>(advoc::row_at<T>(a.dh, row * a.dh_pitch, col[j]), t[j]);
     }
-    if (shared_gate && a.dgate) {
+    if (H && shared_gate) {
+      raw_gate.load(gate_base, group * gate_pitch, col);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (a.act == ADVOC_GATE_SIGMOID) gacc[j] *= gate[j] * (f32x8(1.f) - gate[j]);
-        if (a.gate_part) advoc::store_chunk<V>(a.gate_part + (int64_t)seg * a.cols + col[j], gacc[j]);
-        else advoc::store_chunk<V>((T*)a.dgate + group * a.dgate_pitch + col[j], gacc[j]);
+        f32x8 gate = raw_gate[j];
+        advoc::activate<V>(gate, a.act);
+        if (a.dgate) {
+          f32x8 dg = scale(j) * (w_post(j) * g1[j] + b_post(j) * g0[j]);
+          if (a.act == ADVOC_GATE_SIGMOID) dg *= gate * (f32x8(1.f) - gate);
+          if (a.gate_part) advoc::store_chunk<V>(a.gate_part + (int64_t)seg * cols + col[j], dg);
+          else advoc::store_chunk<V>(advoc::row_at<T>(a.dgate, group * a.dgate_pitch, col[j]), dg);
+        }
+        g0[j] *= gate;
+        g1[j] *= gate;
+        if (carry) {
+          float *c0 = carry + j * L * V, *c1 = c0 + kOwn;
+          if (again) {
+            g0[j] += advoc::cols_chunk<V>(c0);
+            g1[j] += advoc::cols_chunk<V>(c1);
+          }
+          advoc::store_chunk<V>(c0, g0[j]);
+          advoc::store_chunk<V>(c1, g1[j]);
+        }
       }
+      again = true;
     }
   }
 
   // the workgroup's column sums: values of a column with two holders are equal, so either may store them
+  f32x8 out[kSums][NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) acc[kDscale][j] *= a.alpha;
+  for (int j = 0; j < NV; ++j) {
+    out[kDwPost][j] = scale(j) * g1[j];
+    out[kDbPost][j] = scale(j) * g0[j];
+    out[kDscale][j] = w_post(j) * g1[j] + b_post(j) * g0[j];
+    out[kDwPre][j] = dw_pre[j];
+    out[kDbPre][j] = db_pre[j];
+  }
 #pragma unroll
   for (int s = 0; s < kSums; ++s) {
     if (sums.slot[s] < 0) continue;
-    float* out = a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * a.cols;
+    float* to = a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * cols;
     if constexpr (L > 64) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        advoc::store_chunk<V>(out + col[j], acc[s][j]);
+      for (int j = 0; j < NV; ++j) advoc::store_chunk<V>(to + col[j], out[s][j]);
     } else {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-        advoc::store_chunk<V>(fold + Row::slot() * a.cols + col[j], acc[s][j]);
+      for (int j = 0; j < NV; ++j) advoc::store_chunk<V>(vec + Row::slot() * cols + col[j], out[s][j]);
       __syncthreads();
-      for (int c = threadIdx.x; c < a.cols; c += WG) {
+      for (int c = threadIdx.x; c < cols; c += WG) {
         float v = 0.f;
-        for (int w = 0; w < Row::kRows; ++w) v += fold[w * a.cols + c];
-        out[c] = v;
+        for (int w = 0; w < Row::kRows; ++w) v += vec[w * cols + c];
+        to[c] = v;
       }
     }
   }
@@ -223,27 +275,26 @@ __global__ __launch_bounds__(1024) void norm_fold_kernel(FoldArgs a) {
 
 // How the rows are cut: workgroups, and for a shared gate how many workers share a gate row.
 struct Plan {
-  int64_t blocks = 0, chunk = 0, segments = 0;
+  int64_t blocks = 0, segments = 0;
   int splits = 0, sums = 0;
   bool gate_fold = false;
-  int64_t part_floats = 0, gate_floats = 0;
+  int64_t part_floats = 0, gate_floats = 0, carry_floats = 0;
 };
 
 struct MakePlan {
   const NormArgs& a;
   const Sums& sums;
   Plan& p;
-  template <int V, int L, int NV, int WG>
+  template <int V, int L, int NV>
   void run() const {
-    constexpr int kRows = Team<L, WG>::kRows;
-    const int64_t most = 512 * 256 / WG;
+    constexpr int kRows = Team<L, kLanes<L, NV>>::kRows;
+    const int64_t most = 256 * 4 * 64 * kWavesPerSimd<NV> / kLanes<L, NV>;      // what is resident together
     const bool shared_gate = a.gate && a.gate_group > 1;
     const int64_t rows = shared_gate ? a.gate_group : a.rows, groups = a.rows / rows;
     int64_t splits = most * kRows / groups;
     if (splits > rows) splits = rows;
     if (splits < 1) splits = 1;
-    p.chunk = advoc::ceil_div(rows, splits);
-    p.splits = (int)advoc::ceil_div(rows, p.chunk);
+    p.splits = (int)splits;
     p.segments = groups * p.splits;
     p.blocks = advoc::ceil_div(p.segments, kRows);
     if (p.blocks > most) p.blocks = most;
@@ -251,6 +302,7 @@ struct MakePlan {
     p.gate_fold = shared_gate && a.dgate && p.splits > 1;
     p.part_floats = p.sums * p.blocks * a.cols;
     p.gate_floats = p.gate_fold ? p.segments * a.cols : 0;
+    if (shared_gate && p.segments > p.blocks * kRows) p.carry_floats = p.blocks * kRows * 2 * NV * L * V;
   }
 };
 
@@ -260,9 +312,14 @@ struct Launch {
   const Sums& sums;
   int64_t blocks;
   hipStream_t stream;
-  template <int V, int L, int NV, int WG>
+  template <int V, int L, int NV>
   void run() const {
-    hipLaunchKernelGGL((norm_backward_kernel<T, R, V, L, NV, WG>), dim3((unsigned)blocks), dim3(WG), 0, stream, a, sums);
+    constexpr int WG = kLanes<L, NV>, kRows = Team<L, WG>::kRows;
+    const dim3 grid((unsigned)blocks), block(WG);
+    const unsigned lds = 4u * a.cols * (kRows > 4 ? kRows : 4);
+    if (!a.h) hipLaunchKernelGGL((norm_backward_kernel<T, R, V, L, NV, WG, false, true>), grid, block, lds, stream, a, sums);
+    else if (a.pre == ADVOC_NORM_NONE) hipLaunchKernelGGL((norm_backward_kernel<T, R, V, L, NV, WG, true, false>), grid, block, lds, stream, a, sums);
+    else hipLaunchKernelGGL((norm_backward_kernel<T, R, V, L, NV, WG, true, true>), grid, block, lds, stream, a, sums);
   }
 };
 
@@ -286,7 +343,7 @@ int64_t norm_backward_workspace(const NormArgs& a, float* const (&out)[5]) {
   const Sums sums = wanted_sums(out, packed);
   Plan p;
   if (!norm_dispatch(a.cols, MakePlan{a, sums, p})) return 0;
-  return 4 * (p.part_floats + p.gate_floats);
+  return 4 * (p.part_floats + p.gate_floats + p.carry_floats);
 }
 
 int launch_norm_backward(NormArgs a, int dtype, int res_dtype, float* const (&out)[5], int accumulate, void* workspace,
@@ -295,10 +352,10 @@ int launch_norm_backward(NormArgs a, int dtype, int res_dtype, float* const (&ou
   const Sums sums = wanted_sums(out, f.out);
   Plan p;
   if (!norm_dispatch(a.cols, MakePlan{a, sums, p})) return ADVOC_ERR_UNSUPPORTED;
-  if (4 * (p.part_floats + p.gate_floats) > workspace_bytes) return ADVOC_ERR_NULL;
+  if (4 * (p.part_floats + p.gate_floats + p.carry_floats) > workspace_bytes) return ADVOC_ERR_NULL;
   a.part = (float*)workspace;
   a.gate_part = p.gate_fold ? (float*)workspace + p.part_floats : nullptr;
-  a.chunk = p.chunk;
+  a.carry = p.carry_floats ? (float*)workspace + p.part_floats + p.gate_floats : nullptr;
   a.segments = p.segments;
   a.splits = p.splits;
   ADVOC_CLEAR_LAUNCH_ERROR();

@@ -32,54 +32,78 @@ __device__ __forceinline__ void row_stats(const f32x8 (&a)[NV], const int (&dup)
   rstd = 1.f / sqrtf(sq * inv_cols + eps);
 }
 
+template <int V, int L, int NV>
+constexpr bool kFiveVectors = V * L * NV <= 4096;
+
+// The next row's loads are in flight while a row is computed.
 template <typename T, typename R, int V, int L, int NV, int WG>
 __global__ __launch_bounds__(WG) void norm_forward_kernel(NormArgs a) {
   using Row = Team<L, WG>;
+  extern __shared__ float vec[];                // scale, w_post, b_post, w_pre and, where five fit into LDS, b_pre
+  constexpr bool kFive = kFiveVectors<V, L, NV>;
   __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
   int turn = 0;
-  const int lane = Row::lane();
+  const int lane = Row::lane(), cols = a.cols;
   const uint2 key = advoc::drop_key_words(a.key);
-  const bool aligned = (a.cols & 3) == 0, ragged = a.cols % V != 0;
+  const bool aligned = (cols & 3) == 0, ragged = cols % V != 0;
   int col[NV], dup[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, a.cols, col[j], dup[j]);
-  // a workgroup-wide row must take every lane through the same number of rows (the sums meet at barriers)
-  for (int64_t row = (int64_t)blockIdx.x * Row::kRows + (L > 64 ? 0 : Row::slot()); row < a.rows;
-       row += (int64_t)gridDim.x * Row::kRows) {
+  for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, cols, col[j], dup[j]);
+
+  advoc::Raw<T, V, NV> h, gate;
+  advoc::Raw<R, V, NV> x;
+  auto load = [&](int64_t row) {
+    if (row >= a.rows) row = a.rows - 1;        // (the lanes of a wave leave the loop together)
+    x.load(a.x, row * a.x_pitch, col);
+    if (a.h) h.load(a.h, row * a.h_pitch, col);
+    if (a.gate) gate.load(a.gate, (int64_t)((uint32_t)row / (uint32_t)a.gate_group) * a.gate_pitch, col);
+  };
+  const int64_t step = (int64_t)gridDim.x * Row::kRows;
+  int64_t row = (int64_t)blockIdx.x * Row::kRows + Row::slot();
+  load(row);
+  advoc::stage_vector<WG>(vec, a.scale, 1.f, cols);
+  advoc::stage_vector<WG>(vec + cols, a.w_post, 1.f, cols);
+  advoc::stage_vector<WG>(vec + 2 * cols, a.b_post, 0.f, cols);
+  advoc::stage_vector<WG>(vec + 3 * cols, a.w_pre, 1.f, cols);
+  if constexpr (kFive) advoc::stage_vector<WG>(vec + 4 * cols, a.b_pre, 0.f, cols);
+  Row::meet();
+  for (; row < a.rows; row += step) {
+    advoc::forget_lds();
     f32x8 r[NV], u[NV], g[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        r[j] = advoc::load_chunk<V>((const R*)a.x + row * a.x_pitch + col[j]);
-        if (a.h) u[j] = advoc::load_chunk<V>((const T*)a.h + row * a.h_pitch + col[j]);
-        if (a.gate) g[j] = advoc::load_chunk<V>((const T*)a.gate + (int64_t)((uint32_t)row / (uint32_t)a.gate_group) * a.gate_pitch + col[j]);
-      }
-    if constexpr (L > 64) __syncthreads();      // outputs may be the inputs' own buffers, and a column may have two holders
+      r[j] = x[j];
+      u[j] = h[j];
+      g[j] = gate[j];
+    }
+    if constexpr (L > 64) Row::meet();          // outputs may be the inputs' own buffers, and a column may have two holders
+    load(row + step);
     float mean0 = 0.f, rstd0 = 0.f, mean1 = 0.f, rstd1 = 0.f;
     if (a.h) {
       if (a.post != ADVOC_NORM_NONE) row_stats<V, L, NV, WG>(u, dup, ragged, a.post, a.inv_cols, a.eps, red, turn, mean0, rstd0);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (a.post != ADVOC_NORM_NONE) {
-          const f32x8 w = advoc::cols_chunk<V>(a.w_post, col[j], 1.f), b = advoc::cols_chunk<V>(a.b_post, col[j], 0.f);
-          u[j] = (u[j] - mean0) * rstd0 * w + b;
-        }
-        const uint32_t keep = advoc::keep_chunk<V>(a.key.offset + (uint64_t)(row * a.cols + col[j]), aligned, key, a.key.thresh);
-        f32x8 s = advoc::cols_chunk<V>(a.scale, col[j], 1.f) * a.alpha;
+        if (a.post != ADVOC_NORM_NONE)
+          u[j] = (u[j] - mean0) * rstd0 * advoc::cols_chunk<V>(vec + cols + col[j]) + advoc::cols_chunk<V>(vec + 2 * cols + col[j]);
+        const uint32_t keep = advoc::keep_chunk<V>(a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
+        f32x8 s = advoc::cols_chunk<V>(vec + col[j]) * a.alpha;
         if (a.gate) {
           advoc::activate<V>(g[j], a.act);
           s *= g[j];
         }
 #pragma unroll
         for (int k = 0; k < V; ++k) r[j][k] += s[k] * ((keep >> k & 1) ? u[j][k] * a.key.scale : 0.f);
-        advoc::store_chunk<V>((R*)a.r + row * a.r_pitch + col[j], r[j]);
+        advoc::store_chunk<V>(advoc::row_at<R>(a.r, row * a.r_pitch, col[j]), r[j]);
       }
     }
     if (a.pre != ADVOC_NORM_NONE) {
       row_stats<V, L, NV, WG>(r, dup, ragged, a.pre, a.inv_cols, a.eps, red, turn, mean1, rstd1);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const f32x8 w = advoc::cols_chunk<V>(a.w_pre, col[j], 1.f), b = advoc::cols_chunk<V>(a.b_pre, col[j], 0.f);
-        advoc::store_chunk<V>((T*)a.z + row * a.z_pitch + col[j], (r[j] - mean1) * rstd1 * w + b);
+        f32x8 z = (r[j] - mean1) * rstd1 * advoc::cols_chunk<V>(vec + 3 * cols + col[j]);
+        if constexpr (kFive) z += advoc::cols_chunk<V>(vec + 4 * cols + col[j]);
+        else if (a.b_pre) z += advoc::cols_chunk<V>(a.b_pre + col[j]);
+        advoc::store_chunk<V>(advoc::row_at<T>(a.z, row * a.z_pitch, col[j]), z);
       }
     }
     if (a.stats && lane == 0) a.stats[row] = make_float4(mean0, rstd0, mean1, rstd1);
@@ -90,12 +114,14 @@ template <typename T, typename R>
 struct Launch {
   const NormArgs& a;
   hipStream_t stream;
-  template <int V, int L, int NV, int WG>
+  template <int V, int L, int NV>
   void run() const {
+    constexpr int WG = L > 64 ? L : 256;
     int64_t blocks = advoc::ceil_div(a.rows, Team<L, WG>::kRows);
-    const int64_t most = 256 * (2048 / WG);      // every resident workgroup of the chip, then rows in turn
+    const int64_t most = 256 * (1024 / WG);      // the workgroups that are resident together, then rows in turn
     if (blocks > most) blocks = most;
-    hipLaunchKernelGGL((norm_forward_kernel<T, R, V, L, NV, WG>), dim3((unsigned)blocks), dim3(WG), 0, stream, a);
+    hipLaunchKernelGGL((norm_forward_kernel<T, R, V, L, NV, WG>), dim3((unsigned)blocks), dim3(WG),
+                       (kFiveVectors<V, L, NV> ? 20 : 16) * a.cols, stream, a);
   }
 };
 
