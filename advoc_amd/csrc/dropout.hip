@@ -29,7 +29,8 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(Args a) {
   const int64_t base = (int64_t)blockIdx.x * (kThreads * kPer);      // a multiple of 4, as the offset is
   const int64_t i = base + threadIdx.x * kPer;
   if (i >= a.n) return;
-  const uint32_t keep = thresh ? advoc::drop_keep8(a.key.offset + (uint64_t)i, true, key, thresh) : 0xffu;
+  uint32_t words[kPer] = {};
+  if (thresh) advoc::drop_words8(words, a.key.offset + (uint64_t)i, true, key);
   const T* x = (const T*)a.x;
   T* y = (T*)a.y;
   uint32_t col = 0;
@@ -48,11 +49,13 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(Args a) {
     const f32x8 v = advoc::load8(x);
     f32x8 o;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) o[k] = (keep >> k & 1) ? v[k] * scale : 0.f;
+    for (int k = 0; k < kPer; ++k) o[k] = words[k] >= thresh ? v[k] * scale : 0.f;
     advoc::store8(y, o);
   } else {
-    for (int k = 0; k < kPer && i + k < a.n; ++k) {
-      *y = (T)((keep >> k & 1) ? (float)*x * scale : 0.f);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      if (i + k >= a.n) break;
+      *y = (T)(words[k] >= thresh ? (float)*x * scale : 0.f);
       ++x, ++y;
       if (PITCHED && ++col == a.cols) {
         col = 0;

@@ -15,16 +15,19 @@ __device__ __forceinline__ void mul64(uint64_t& p, uint32_t a, uint32_t b) {
   asm("v_mad_u64_u32 %0, %1, %2, %3, 0" : "=v"(p), "=s"(carry) : "s"(a), "v"(b));
 }
 
-__device__ __forceinline__ uint4 philox4x32(uint4 ctr, uint2 key) {
+// Counter (c, 0): the first round multiplies one word only.
+__device__ __forceinline__ uint4 philox4x32(uint64_t c, uint2 key) {
   const uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
+  uint64_t p0, p1;
+  mul64(p0, M0, (uint32_t)c);
+  uint4 ctr = make_uint4((uint32_t)(c >> 32) ^ key.x, 0u, (uint32_t)(p0 >> 32) ^ key.y, (uint32_t)p0);
 #pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    uint64_t p0, p1;
+  for (int r = 1; r < 10; ++r) {
+    key.x += W0;
+    key.y += W1;
     mul64(p0, M0, ctr.x);
     mul64(p1, M1, ctr.z);
     ctr = make_uint4((uint32_t)(p1 >> 32) ^ ctr.y ^ key.x, (uint32_t)p1, (uint32_t)(p0 >> 32) ^ ctr.w ^ key.y, (uint32_t)p0);
-    key.x += W0;
-    key.y += W1;
   }
   return ctr;
 }
@@ -55,30 +58,28 @@ __device__ __forceinline__ uint2 drop_key_words(const DropKey& k) {
   return make_uint2((uint32_t)s, (uint32_t)(s >> 32));
 }
 
-// words 4 q .. 4 q + 3
-__device__ __forceinline__ uint4 drop_quad(uint64_t q, uint2 key) {
-  return philox4x32(make_uint4((uint32_t)q, (uint32_t)(q >> 32), 0u, 0u), key);
-}
-
-// bit k set: element i + k of the stream is kept, k < 8.  i = offset + index; any alignment (a third block only where i is no
-// multiple of 4, and `aligned` -- uniform over the launch -- says that none is).
-__device__ __forceinline__ uint32_t drop_keep8(uint64_t i, bool aligned, uint2 key, uint32_t thresh) {
+// The words of elements i ... i + 7 of the stream: element k is kept when words[k] >= thresh.  i = offset + index, of any
+// alignment: a third block is drawn only where i is no multiple of 4, which `aligned` -- uniform over the launch -- rules out.
+__device__ __forceinline__ void drop_words8(uint32_t (&words)[8], uint64_t i, bool aligned, uint2 key) {
   const uint64_t q = i >> 2;
-  const uint4 a = drop_quad(q, key), b = drop_quad(q + 1, key);
-  uint32_t bits = (a.x >= thresh) | (a.y >= thresh) << 1 | (a.z >= thresh) << 2 | (a.w >= thresh) << 3 |
-                  (b.x >= thresh) << 4 | (b.y >= thresh) << 5 | (b.z >= thresh) << 6 | (b.w >= thresh) << 7;
-  if (!aligned) {
-    const uint4 c = drop_quad(q + 2, key);
-    bits |= (c.x >= thresh) << 8 | (c.y >= thresh) << 9 | (c.z >= thresh) << 10 | (c.w >= thresh) << 11;
-    bits >>= (uint32_t)i & 3u;
+  const uint4 a = philox4x32(q, key), b = philox4x32(q + 1, key);
+  if (aligned) {
+    words[0] = a.x, words[1] = a.y, words[2] = a.z, words[3] = a.w;
+    words[4] = b.x, words[5] = b.y, words[6] = b.z, words[7] = b.w;
+  } else {
+    const uint4 c = philox4x32(q + 2, key);
+    const uint32_t w[11] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z};
+    uint32_t v[10];
+#pragma unroll
+    for (int k = 0; k < 10; ++k) v[k] = (i & 1) ? w[k + 1] : w[k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) words[k] = (i & 2) ? v[k + 2] : v[k];
   }
-  return bits;
 }
 
-__device__ __forceinline__ uint32_t drop_keep1(uint64_t i, uint2 key, uint32_t thresh) {
-  const uint4 a = drop_quad(i >> 2, key);
-  const uint32_t w = (i & 2) ? ((i & 1) ? a.w : a.z) : ((i & 1) ? a.y : a.x);
-  return w >= thresh;
+__device__ __forceinline__ uint32_t drop_word(uint64_t i, uint2 key) {
+  const uint4 a = philox4x32(i >> 2, key);
+  return (i & 2) ? ((i & 1) ? a.w : a.z) : ((i & 1) ? a.y : a.x);
 }
 
 }  // namespace advoc

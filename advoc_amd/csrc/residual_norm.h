@@ -175,11 +175,14 @@ __device__ __forceinline__ f32x8 cols_chunk(const float* p) {
   return f;
 }
 
+// what a chunk's elements draw (all kept where nothing is drawn: thresh 0)
 template <int V>
-__device__ __forceinline__ uint32_t keep_chunk(uint64_t i, bool aligned, uint2 key, uint32_t thresh) {
-  if (!thresh) return 0xffu;
-  if constexpr (V == 8) return drop_keep8(i, aligned, key, thresh);
-  return drop_keep1(i, key, thresh);
+__device__ __forceinline__ void draw_chunk(uint32_t (&words)[8], uint64_t i, bool aligned, uint2 key, uint32_t thresh) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) words[k] = 0;
+  if (!thresh) return;
+  if constexpr (V == 8) drop_words8(words, i, aligned, key);
+  else words[0] = drop_word(i, key);
 }
 
 // act(gate) in place

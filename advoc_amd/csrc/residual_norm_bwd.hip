@@ -148,13 +148,14 @@ __global__ __launch_bounds__(WG, kWavesPerSimd<NV>) void norm_backward_kernel(No
       advoc::forget_lds();
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const uint32_t keep = advoc::keep_chunk<V>(a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
+        uint32_t words[8];
+        advoc::draw_chunk<V>(words, a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
         advoc::activate<V>(gate[j], a.act);
         const f32x8 s = scale(j);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           gate[j][k] = has_gate ? gate[j][k] : 1.f;
-          t[j][k] = (keep >> k & 1) ? g[j][k] * kept : 0.f;
+          t[j][k] = words[k] >= a.key.thresh ? g[j][k] * kept : 0.f;
         }
         if (row_gate && a.dgate) {
           f32x8 dg = t[j] * s * (hat[j] * w_post(j) + b_post(j));

@@ -59,6 +59,7 @@ __global__ __launch_bounds__(WG) void norm_forward_kernel(NormArgs a) {
     if (a.gate) gate.load(a.gate, (int64_t)((uint32_t)row / (uint32_t)a.gate_group) * a.gate_pitch, col);
   };
   const int64_t step = (int64_t)gridDim.x * Row::kRows;
+  const float kept = a.alpha * a.key.scale;
   int64_t row = (int64_t)blockIdx.x * Row::kRows + Row::slot();
   load(row);
   advoc::stage_vector<WG>(vec, a.scale, 1.f, cols);
@@ -85,14 +86,15 @@ __global__ __launch_bounds__(WG) void norm_forward_kernel(NormArgs a) {
       for (int j = 0; j < NV; ++j) {
         if (a.post != ADVOC_NORM_NONE)
           u[j] = (u[j] - mean0) * rstd0 * advoc::cols_chunk<V>(vec + cols + col[j]) + advoc::cols_chunk<V>(vec + 2 * cols + col[j]);
-        const uint32_t keep = advoc::keep_chunk<V>(a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
-        f32x8 s = advoc::cols_chunk<V>(vec + col[j]) * a.alpha;
+        uint32_t words[8];
+        advoc::draw_chunk<V>(words, a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
+        f32x8 s = advoc::cols_chunk<V>(vec + col[j]) * kept;
         if (a.gate) {
           advoc::activate<V>(g[j], a.act);
           s *= g[j];
         }
 #pragma unroll
-        for (int k = 0; k < V; ++k) r[j][k] += s[k] * ((keep >> k & 1) ? u[j][k] * a.key.scale : 0.f);
+        for (int k = 0; k < V; ++k) r[j][k] += s[k] * (words[k] >= a.key.thresh ? u[j][k] : 0.f);
         advoc::store_chunk<V>(advoc::row_at<R>(a.r, row * a.r_pitch, col[j]), r[j]);
       }
     }

@@ -131,8 +131,7 @@ __global__ __launch_bounds__(256) void dropout_mask_kernel(uint8_t* __restrict__
   const uint32_t thresh = (uint32_t)fminf(fmaxf((1.0f - keep) * 4294967296.0f, 0.f), 4294967295.f);
   for (int64_t q = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; q < quads; q += stride) {
     const uint64_t c = (offset >> 2) + (uint64_t)q;     // offset is a multiple of 4
-    const uint4 r = advoc::philox4x32(make_uint4((uint32_t)c, (uint32_t)(c >> 32), 0u, 0u),
-                                      make_uint2((uint32_t)seed, (uint32_t)(seed >> 32)));
+    const uint4 r = advoc::philox4x32(c, make_uint2((uint32_t)seed, (uint32_t)(seed >> 32)));
     const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
     const int64_t i = q * 4;
     if (i + 4 <= n) {
