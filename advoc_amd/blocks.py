@@ -46,13 +46,13 @@ def _dtype(t, name):
   return code
 
 
-def _rows(t, name, device=None):
-  """(address, rows, cols, elements from row to row) of a tensor as rows of its last dimension."""
+def _rows(t, name, index=None):
+  """(address, rows, cols, elements from row to row) of a tensor as rows of its last dimension; index: the device it must be on."""
   if not isinstance(t, torch.Tensor) or not t.is_cuda:
     raise _lib.AdvocHipError('{} must be a torch tensor on a HIP device (no CPU path exists)'.format(name))
-  if device is not None and t.device != device:
-    raise _lib.AdvocHipError('{} is on {}, the other tensors on {}'.format(name, t.device, device))
-  if t.dim() == 0:
+  if index is not None and t.get_device() != index:
+    raise _lib.AdvocHipError('{} is on {}, the other tensors on device {}'.format(name, t.device, index))
+  if not t.dim():
     raise _lib.AdvocHipError('{} must have at least one dimension'.format(name))
   cols = t.shape[-1]
   if t.is_contiguous():
@@ -73,22 +73,30 @@ def _rows(t, name, device=None):
   return t.data_ptr(), rows, cols, pitch
 
 
-def _seed_word(seed_dev, device):
+def _seed_word(seed_dev, index):
   if seed_dev is None:
     return None
-  if not isinstance(seed_dev, torch.Tensor) or seed_dev.device != device or seed_dev.numel() != 1 or seed_dev.dtype not in (
-      torch.int64, torch.uint64):
-    raise _lib.AdvocHipError('seed_dev must be one int64 or uint64 on {}'.format(device))
+  if not isinstance(seed_dev, torch.Tensor) or not seed_dev.is_cuda or seed_dev.get_device() != index or (
+      seed_dev.numel() != 1) or seed_dev.dtype not in (torch.int64, torch.uint64):
+    raise _lib.AdvocHipError('seed_dev must be one int64 or uint64 on device {}'.format(index))
   return seed_dev.data_ptr()
 
 
-def _call(fn, what, device, *args):
-  """One library call on the current stream of `device`, with that device current."""
-  if device.index == torch.cuda.current_device():
-    rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+# (torch.cuda.current_stream() and current_device() spend 9 us in Python per call, several times what the smallest kernels take)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_devices = None
+
+
+def _call(fn, what, index, *args):
+  """One library call on the current stream of device `index`, with that device current."""
+  global _devices
+  if _devices is None:
+    _devices = torch.cuda.device_count()
+  if _devices == 1 or torch.cuda.current_device() == index:
+    rc = fn(*args, _raw_stream(index))
   else:
-    with torch.cuda.device(device):
-      rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(index):
+      rc = fn(*args, _raw_stream(index))
   if rc:
     _lib.check(rc, what)
 
@@ -103,15 +111,16 @@ def dropout(x, keep_prob, seed, offset=0, seed_dev=None, out=None):
   graphs whose replays must not repeat a mask.  out: a tensor of x's shape and dtype, or x itself."""
   px, rows, cols, pitch = _rows(x, 'x')
   code = _dtype(x, 'x')
+  index = x.get_device()
   if out is None:
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     py, out_pitch = out.data_ptr(), cols
   else:
-    py, _, _, out_pitch = _rows(out, 'out', x.device)
+    py, _, _, out_pitch = _rows(out, 'out', index)
     if out.shape != x.shape or out.dtype != x.dtype:
       raise _lib.AdvocHipError('out must have the shape and dtype of x')
-  _call(_lib.load().advoc_dropout, 'advoc_dropout', x.device, px, pitch, py, out_pitch, rows, cols, code, keep_prob,
-        seed & _MASK64, offset & _MASK64, _seed_word(seed_dev, x.device))
+  _call(_lib.load().advoc_dropout, 'advoc_dropout', index, px, pitch, py, out_pitch, rows, cols, code, keep_prob,
+        seed & _MASK64, offset & _MASK64, _seed_word(seed_dev, index))
   return out
 
 
@@ -144,56 +153,59 @@ class ResidualNorm(object):
     if not self.post and (w_post is not None or b_post is not None) or not self.pre and (w_pre is not None or b_pre is not None):
       raise _lib.AdvocHipError('a norm of kind none takes no weight or bias')
 
-  def _vector(self, t, name, device):
+  def _vector(self, t, name, index):
     if t is None:
       return None
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.float32 or t.shape != (self.cols,) or not (
-        t.is_contiguous()):
-      raise _lib.AdvocHipError('{} must be a contiguous float32 tensor of {} on {}'.format(name, self.cols, device))
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != index or t.dtype != torch.float32 or (
+        t.dim() != 1 or t.shape[0] != self.cols or not t.is_contiguous()):
+      raise _lib.AdvocHipError('{} must be a contiguous float32 tensor of {} on device {}'.format(name, self.cols, index))
     return t.data_ptr()
 
-  def _bind(self, d, name, t, rows, device, dtype=None):
-    p, n, cols, pitch = _rows(t, name, device)
+  def _bind(self, field, name, t, rows, index, dtype=None):
+    field.p, n, cols, field.pitch = _rows(t, name, index)
     if n != rows or cols != self.cols:
       raise _lib.AdvocHipError('{} has shape {}: {} rows of {} wanted'.format(name, tuple(t.shape), rows, self.cols))
     if dtype is not None and t.dtype != dtype:
       raise _lib.AdvocHipError('{} is {}, {} wanted'.format(name, t.dtype, dtype))
-    field = getattr(d, name)
-    field.p, field.pitch = p, pitch
 
   def _descriptor(self, x, name, dtype, gate, seed, offset, seed_dev, has_h):
     """What both directions share; x (r in the backward pass) sets rows, device and residual dtype."""
     px, rows, cols, pitch = _rows(x, name)
     if cols != self.cols:
       raise _lib.AdvocHipError('{} has {} columns, {} wanted'.format(name, cols, self.cols))
-    device = x.device
-    d = _lib.ResidualNorm()
-    d.rows, d.cols, d.dtype, d.res_dtype = rows, cols, _DTYPES.get(dtype, -1), _dtype(x, name)
-    if d.dtype < 0 or d.res_dtype not in (d.dtype, 0):
+    index = x.get_device()
+    code, res_code = _DTYPES.get(dtype, -1), _dtype(x, name)
+    if code < 0 or res_code not in (code, 0):
       raise _lib.AdvocHipError('{} is {}: it must be float32 or the dtype of the block ({})'.format(name, x.dtype, dtype))
-    d.norm_pre, d.alpha, d.eps, d.keep_prob = self.pre, self.alpha, self.eps, self.keep_prob
-    d.w_pre, d.b_pre = self._vector(self.w_pre, 'w_pre', device), self._vector(self.b_pre, 'b_pre', device)
-    if has_h:
-      d.norm_post, d.gate_act = self.post, self.gate_act
-      d.w_post, d.b_post = self._vector(self.w_post, 'w_post', device), self._vector(self.b_post, 'b_post', device)
-      d.scale = self._vector(self.scale, 'scale', device)
-      d.seed, d.offset, d.seed_dev = seed & _MASK64, offset & _MASK64, _seed_word(seed_dev, device)
+    if not has_h:
       if gate is not None:
-        p, n, cols, gate_pitch = _rows(gate, 'gate', device)
+        raise _lib.AdvocHipError('a gate needs a block output h')
+      d = _lib.ResidualNorm(rows, cols, code, res_code, 0, self.pre, 0, 1, None, None, None,
+                            self._vector(self.w_pre, 'w_pre', index), self._vector(self.b_pre, 'b_pre', index), self.alpha,
+                            self.eps, self.keep_prob)
+    else:
+      d = _lib.ResidualNorm(rows, cols, code, res_code, self.post, self.pre, self.gate_act, 1,
+                            self._vector(self.w_post, 'w_post', index), self._vector(self.b_post, 'b_post', index),
+                            self._vector(self.scale, 'scale', index), self._vector(self.w_pre, 'w_pre', index),
+                            self._vector(self.b_pre, 'b_pre', index), self.alpha, self.eps, self.keep_prob, 0, seed & _MASK64,
+                            offset & _MASK64, _seed_word(seed_dev, index))
+      if gate is not None:
+        field = d.gate
+        field.p, n, cols, field.pitch = _rows(gate, 'gate', index)
         if cols != self.cols or gate.dtype != dtype or (rows % n if n else rows):
           raise _lib.AdvocHipError('gate {} {} does not divide {} rows of {} {}'.format(
               gate.dtype, tuple(gate.shape), rows, self.cols, dtype))
         self._check_gate_shape(gate, x)
-        d.gate.p, d.gate.pitch, d.gate_group = p, gate_pitch, rows // n if n else 1
-    elif gate is not None:
-      raise _lib.AdvocHipError('a gate needs a block output h')
+        d.gate_group = rows // n if n else 1
     field = getattr(d, name)
     field.p, field.pitch = px, pitch
-    return d, rows, device
+    return d, rows, index
 
   def _check_gate_shape(self, gate, x):
     """A gate has x's shape, with ones for trailing row dimensions that share it: [clips, 1, cols] for [clips, frames, cols]."""
-    lead, want = list(gate.shape[:-1]), list(x.shape[:-1])
+    if gate.shape == x.shape:
+      return
+    lead, want = gate.shape[:-1], x.shape[:-1]
     if len(lead) == len(want):
       i = 0
       while i < len(lead) and lead[i] == want[i]:
@@ -205,28 +217,34 @@ class ResidualNorm(object):
   def forward(self, h, x, gate=None, seed=0, offset=0, seed_dev=None, save=False, r=None, z=None):
     """(r, z, stats).  h None: only z = N_pre(x), the norm before the first block (r is x).  z is None without a pre norm,
     stats [rows, 4] is None unless `save` (a later backward needs it).  r, z: buffers to write into; r may be x."""
-    dtype = h.dtype if isinstance(h, torch.Tensor) else z.dtype if z is not None else x.dtype
-    d, rows, device = self._descriptor(x, 'x', dtype, gate, seed, offset, seed_dev, h is not None)
+    like = h if h is not None else z if z is not None else x
+    if not isinstance(like, torch.Tensor):
+      raise _lib.AdvocHipError('h and x must be torch tensors')
+    dtype = like.dtype
+    d, rows, index = self._descriptor(x, 'x', dtype, gate, seed, offset, seed_dev, h is not None)
     if h is None:
       if not self.pre:
         raise _lib.AdvocHipError('neither h nor a pre norm: nothing to compute')
       r = x
     else:
-      self._bind(d, 'h', h, rows, device)
+      self._bind(d.h, 'h', h, rows, index)
       if r is None:
-        r = torch.empty(x.shape, dtype=x.dtype, device=device)
-      self._bind(d, 'r', r, rows, device, x.dtype)
-    if self.pre:
-      if z is None:
-        z = torch.empty(x.shape, dtype=dtype, device=device)
-      self._bind(d, 'z', z, rows, device, dtype)
-    else:
+        r = torch.empty_like(x, memory_format=torch.contiguous_format)
+        d.r.p, d.r.pitch = r.data_ptr(), self.cols
+      else:
+        self._bind(d.r, 'r', r, rows, index, x.dtype)
+    if not self.pre:
       z = None
+    elif z is None:
+      z = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
+      d.z.p, d.z.pitch = z.data_ptr(), self.cols
+    else:
+      self._bind(d.z, 'z', z, rows, index, dtype)
     stats = None
     if save:
-      stats = torch.empty(rows, 4, dtype=torch.float32, device=device)
+      stats = torch.empty(rows, 4, dtype=torch.float32, device=x.device)
       d.stats = stats.data_ptr()
-    _call(_lib.load().advoc_residual_norm_forward, 'advoc_residual_norm_forward', device, ctypes.byref(d))
+    _call(_lib.load().advoc_residual_norm_forward, 'advoc_residual_norm_forward', index, ctypes.byref(d))
     return r, z, stats
 
   def backward(self, dz, dr, h, r, stats, gate=None, seed=0, offset=0, seed_dev=None, into=None, accumulate=False):
@@ -236,30 +254,29 @@ class ResidualNorm(object):
     like = h if h is not None else dz
     if not isinstance(like, torch.Tensor):
       raise _lib.AdvocHipError('h or dz is needed')
-    d, rows, device = self._descriptor(r, 'r', like.dtype, gate, seed, offset, seed_dev, h is not None)
+    d, rows, index = self._descriptor(r, 'r', like.dtype, gate, seed, offset, seed_dev, h is not None)
     if (dz is None) != (not self.pre) or (dz is None and dr is None):
       raise _lib.AdvocHipError('dz goes with a pre norm, and dz or dr must be given')
     if dz is not None:
-      self._bind(d, 'dz', dz, rows, device, like.dtype)
+      self._bind(d.dz, 'dz', dz, rows, index, like.dtype)
     if dr is not None:
-      self._bind(d, 'dr', dr, rows, device, r.dtype)
+      self._bind(d.dr, 'dr', dr, rows, index, r.dtype)
     if h is not None:
-      self._bind(d, 'h', h, rows, device)
+      self._bind(d.h, 'h', h, rows, index)
     if self.pre or h is not None and self.post:
-      if not isinstance(stats, torch.Tensor) or stats.device != device or stats.dtype != torch.float32 or (
-          stats.shape != (rows, 4)) or not stats.is_contiguous():
+      if not isinstance(stats, torch.Tensor) or not stats.is_cuda or stats.get_device() != index or (
+          stats.dtype != torch.float32 or stats.shape != (rows, 4) or not stats.is_contiguous()):
         raise _lib.AdvocHipError('stats must be the contiguous float32 [rows, 4] tensor of forward(..., save=True)')
       d.stats = stats.data_ptr()
     g = dict.fromkeys(ResidualNormGrads._fields)
-    g['dx'] = torch.empty(r.shape, dtype=r.dtype, device=device)
+    g['dx'] = torch.empty_like(r, memory_format=torch.contiguous_format)
+    d.dx.p, d.dx.pitch = g['dx'].data_ptr(), self.cols
     if h is not None:
-      g['dh'] = torch.empty(r.shape, dtype=h.dtype, device=device)
+      g['dh'] = torch.empty_like(r, dtype=h.dtype, memory_format=torch.contiguous_format)
+      d.dh.p, d.dh.pitch = g['dh'].data_ptr(), self.cols
     if gate is not None:
-      g['dgate'] = torch.empty(gate.shape, dtype=gate.dtype, device=device)
-    for name in ('dh', 'dx', 'dgate'):
-      if g[name] is not None:
-        field = getattr(d, name)
-        field.p, field.pitch = g[name].data_ptr(), self.cols
+      g['dgate'] = torch.empty_like(gate, memory_format=torch.contiguous_format)
+      d.dgate.p, d.dgate.pitch = g['dgate'].data_ptr(), self.cols
     into = into or {}
     for name in ('w_post', 'b_post', 'scale', 'w_pre', 'b_pre'):
       if getattr(self, name) is None or h is None and name in ('w_post', 'b_post', 'scale'):
@@ -270,40 +287,51 @@ class ResidualNorm(object):
       if t is None:
         if accumulate:
           raise _lib.AdvocHipError('accumulate needs a buffer for d{}'.format(name))
-        t = torch.empty(self.cols, dtype=torch.float32, device=device)
+        t = torch.empty(self.cols, dtype=torch.float32, device=r.device)
       g['d' + name] = t
-      setattr(d, 'd' + name, self._vector(t, 'd' + name, device))
-    unknown = set(into) - {k for k in g if k[1:] in ('w_post', 'b_post', 'scale', 'w_pre', 'b_pre')}
-    if unknown:
-      raise _lib.AdvocHipError('no such parameter gradients: {}'.format(sorted(unknown)))
+      setattr(d, 'd' + name, self._vector(t, 'd' + name, index))
+    if into:
+      unknown = set(into) - {'dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre'}
+      if unknown:
+        raise _lib.AdvocHipError('no such parameter gradients: {}'.format(sorted(unknown)))
     d.accumulate = int(bool(accumulate))
     lib = _lib.load()
     nbytes = lib.advoc_residual_norm_workspace_bytes(ctypes.byref(d))
     if nbytes:
-      work = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+      work = torch.empty(nbytes // 4, dtype=torch.float32, device=r.device)
       d.workspace, d.workspace_bytes = work.data_ptr(), nbytes
     if rows == 0 and not accumulate:
       for name in ('dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre'):
         if g[name] is not None:
           g[name].zero_()
-    _call(lib.advoc_residual_norm_backward, 'advoc_residual_norm_backward', device, ctypes.byref(d))
+    _call(lib.advoc_residual_norm_backward, 'advoc_residual_norm_backward', index, ctypes.byref(d))
     return ResidualNormGrads(**g)
 
 
 class F8Matrix(object):
-  """A matrix held in 8 bits with a power of two for each block of 128 along its rows: `data` [rows, kp] and `scale`
-  [rows, sp] (uint8; layout in include/advoc_hip.h), made by the quantize_f8 functions."""
-  __slots__ = ('data', 'scale', 'rows', 'k', 'format')
+  """A matrix held in 8 bits with a power of two for each block of 128 along its rows, made by the quantize_f8 functions:
+  `data` [rows, kp] and `scale` [rows, sp] (uint8; layout in include/advoc_hip.h) are two parts of one buffer."""
+  __slots__ = ('buffer', 'rows', 'k', 'format', 'data_ptr', 'scale_ptr')
 
   def __init__(self, rows, k, format, device):
     kp = -(-k // 128) * 128
     self.rows, self.k, self.format = rows, k, format
-    self.data = torch.empty(rows, kp, dtype=torch.uint8, device=device)
-    self.scale = torch.empty(rows, -(-kp // 512) * 4, dtype=torch.uint8, device=device)
+    self.buffer = torch.empty(rows * (kp + -(-kp // 512) * 4), dtype=torch.uint8, device=device)
+    self.data_ptr = self.buffer.data_ptr()
+    self.scale_ptr = self.data_ptr + rows * kp
 
   @property
   def shape(self):
     return (self.rows, self.k)
+
+  @property
+  def data(self):
+    kp = -(-self.k // 128) * 128
+    return self.buffer[:self.rows * kp].view(self.rows, kp)
+
+  @property
+  def scale(self):
+    return self.buffer[self.rows * (-(-self.k // 128) * 128):].view(self.rows, -1)
 
 
 def _quantize(x, fmt, want_rows, want_cols):
@@ -313,9 +341,8 @@ def _quantize(x, fmt, want_rows, want_cols):
     raise _lib.AdvocHipError('x of shape {} holds nothing to quantise'.format(tuple(x.shape)))
   a = F8Matrix(rows, cols, code, x.device) if want_rows else None
   t = F8Matrix(cols, rows, code, x.device) if want_cols else None
-  _call(_lib.load().advoc_f8_quantize, 'advoc_f8_quantize', x.device, p, pitch, rows, cols, _dtype(x, 'x'), code,
-        a.data.data_ptr() if a else None, a.scale.data_ptr() if a else None,
-        t.data.data_ptr() if t else None, t.scale.data_ptr() if t else None)
+  _call(_lib.load().advoc_f8_quantize, 'advoc_f8_quantize', x.get_device(), p, pitch, rows, cols, _dtype(x, 'x'), code,
+        a and a.data_ptr, a and a.scale_ptr, t and t.data_ptr, t and t.scale_ptr)
   return a, t
 
 
@@ -335,11 +362,11 @@ def quantize_f8_both(x, fmt='e4m3'):
 
 
 def matmul_nt_f8(a, b, out_dtype=torch.float32, out=None, accumulate=False):
-  """a b^T of two F8Matrix operands with the same k -> [a.rows, b.rows], accumulated in fp32 (``advoc_matmul_nt_f8``).
-  accumulate: add to `out` (float32), e.g. a gradient arena's slice."""
-  if not isinstance(a, F8Matrix) or not isinstance(b, F8Matrix) or a.k != b.k or a.data.device != b.data.device:
+  """a b^T of two F8Matrix operands with the same k -> [a.rows, b.rows] (``advoc_matmul_nt_f8``); a float32 result is
+  accumulated in fp32 throughout.  accumulate: add to `out` (float32), e.g. a gradient arena's slice."""
+  if not isinstance(a, F8Matrix) or not isinstance(b, F8Matrix) or a.k != b.k or a.buffer.device != b.buffer.device:
     raise _lib.AdvocHipError('two F8Matrix operands with the same k on one device are needed')
-  device, m, n = a.data.device, a.rows, b.rows
+  device, m, n = a.buffer.device, a.rows, b.rows
   if out is None:
     if accumulate:
       raise _lib.AdvocHipError('accumulate needs out')
@@ -348,9 +375,9 @@ def matmul_nt_f8(a, b, out_dtype=torch.float32, out=None, accumulate=False):
     raise _lib.AdvocHipError('out must be a contiguous [{}, {}] tensor on {}'.format(m, n, device))
   code = _dtype(out, 'out')
   lib = _lib.load()
-  nbytes = lib.advoc_matmul_nt_f8_workspace_bytes(m, n, a.k, code)
+  nbytes = lib.advoc_matmul_nt_f8_workspace_bytes(m, n, a.k, code) if m > 64 else 0
   work = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
-  _call(lib.advoc_matmul_nt_f8, 'advoc_matmul_nt_f8', device, a.data.data_ptr(), a.scale.data_ptr(), a.format,
-        b.data.data_ptr(), b.scale.data_ptr(), b.format, out.data_ptr(), code, int(bool(accumulate)), m, n, a.k,
+  _call(lib.advoc_matmul_nt_f8, 'advoc_matmul_nt_f8', device.index, a.data_ptr, a.scale_ptr, a.format, b.data_ptr, b.scale_ptr,
+        b.format, out.data_ptr(), code, int(bool(accumulate)), m, n, a.k,
         work.data_ptr() if nbytes else None, nbytes)
   return out

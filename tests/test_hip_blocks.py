@@ -416,7 +416,7 @@ def test_product_without_workspace_and_with(blocks):
   a, b = ints(m, k, 0), ints(n, k, 1)
   qa, qb = blocks.quantize_f8(a.cuda()), blocks.quantize_f8(b.cuda())
   out = torch.empty(m, n, device='cuda')
-  _lib.check(lib.advoc_matmul_nt_f8(_lib.ptr(qa.data), _lib.ptr(qa.scale), 0, _lib.ptr(qb.data), _lib.ptr(qb.scale), 0, _lib.ptr(out), 0, 0, m, n,
+  _lib.check(lib.advoc_matmul_nt_f8(qa.data_ptr, qa.scale_ptr, 0, qb.data_ptr, qb.scale_ptr, 0, _lib.ptr(out), 0, 0, m, n,
                                     k, None, 0, _lib.stream()))
   assert torch.equal(out, blocks.matmul_nt_f8(qa, qb)) and torch.equal(out.cpu().double(), a.double() @ b.double().t())
 
