@@ -9,8 +9,10 @@
 // block's power of two applied (v_cvt_scalef32_pk_bf16_fp8; every 8-bit value is a bf16 value) and go through
 // v_mfma_f32_16x16x32_bf16, whose sums are fp32's: 4e-8 off in norm, at half the rate.
 // The operand with n rows is the instruction's first: the four accumulators of a lane are then four consecutive n of one output
-// row, and the n that a wave's fragments stand for are dealt so that a lane's fragments continue them (16 consecutive n with four
-// fragments): the output leaves in 32- or 64-byte pieces without a turn through LDS.
+// row, and for 16-bit outputs the n that two fragments stand for are dealt so that one continues the other: a lane stores 16 bytes,
+// four of them 64 consecutive ones, without a turn through LDS.
+#include <utility>
+
 #include "rows.h"
 #include "lds_dma.h"
 
@@ -83,24 +85,14 @@ __device__ __forceinline__ f32x4 mfma(const Frag<FB, true>& b, const Frag<FA, tr
   return c;
 }
 
-// C consecutive values of one output row
+// C consecutive values of one output row, those inside the matrix
 template <typename O, int C>
-__device__ __forceinline__ void store_run(const Args& g, int64_t row, int64_t col, float (&v)[C]) {
+__device__ __forceinline__ void store_part(const Args& g, int64_t row, int64_t col, const float (&v)[C]) {
   if (row >= g.m) return;
   O* p = (O*)g.out + row * g.n + col;
-  if (col + C <= g.n) {
-    if (g.accumulate)
 #pragma unroll
-      for (int k = 0; k < C; ++k) v[k] += (float)p[k];
-    O o[C];
-#pragma unroll
-    for (int k = 0; k < C; ++k) o[k] = (O)v[k];
-    __builtin_memcpy(p, o, sizeof(o));
-  } else {
-#pragma unroll
-    for (int k = 0; k < C; ++k)
-      if (col + k < g.n) p[k] = (O)((g.accumulate ? (float)p[k] : 0.f) + v[k]);
-  }
+  for (int k = 0; k < C; ++k)
+    if (col + k < g.n) p[k] = (O)((g.accumulate ? (float)p[k] : 0.f) + v[k]);
 }
 
 // ---- few rows (m <= 64): the weights are read once, by whoever multiplies them ----
@@ -142,40 +134,42 @@ __global__ __launch_bounds__(1024) void f8_thin_kernel(Args g) {
     for (int w = 1; w < waves; ++w) v += red[w * MF * 64 + e];
     const int l = e & 63;
     float o[4] = {v[0], v[1], v[2], v[3]};
-    store_run<O, 4>(g, (e >> 6) * 16 + (l & 15), n0 + (l >> 4) * 4, o);
+    store_part<O, 4>(g, (e >> 6) * 16 + (l & 15), n0 + (l >> 4) * 4, o);
   }
 }
 
 // ---- tiles ----
-// BM x BN outputs per workgroup, WM x WN per wave.  A block of the contraction of both operands is a stage of LDS, fetched by
-// LDS-DMA while the stage before is multiplied; the exponent bytes of four blocks (a dword per row) are fetched the same way every
-// fourth block.  (Loads that the compiler counts must not follow a DMA in the loop: memory counters retire in order, and waiting for
+// BM x BN outputs per workgroup, WM x WN per wave.  A block of the contraction of both operands, with the dword that holds its
+// exponent byte for every row, is one of S stages in LDS, fetched by LDS-DMA while those before are multiplied.  (Loads that the compiler counts must not follow a DMA in the loop: memory counters retire in order, and waiting for
 // such a load waits for the next stage too.  That alone held the first form of this kernel at 0.8 PFLOP/s.)
 // A row's eight 16-byte pieces lie at piece ^ key(row), and lane group g reads pieces g and g + 4: measured without bank conflicts, 4
 // cycles for a wave's 16 bytes a lane.  (Pieces 2 g and 2 g + 1 take 8.)
-template <int BM, int BN, int WM, int WN>
+template <typename O, int BM, int BN, int WM, int WN, int S>
 struct Tile {
   static constexpr int kWaves = BM / WM * (BN / WN), kFm = WM / 16, kFn = WN / 16;
-  static constexpr int kShift = kFn == 4 ? 4 : 3;                // rows of b four apart in the instruction are 4 kFn apart
+  static constexpr int kRun = sizeof(O) == 4 ? 1 : 2;            // fragments of b that give a lane 16 consecutive bytes of output
   static constexpr int kRows = BM + BN, kStage = kRows * kBlock, kExp = kRows * 4;
-  static constexpr int kLds = 2 * (kStage + kExp);
-  static constexpr int kDma = kRows / 8 / kWaves;                // a DMA instruction fetches 8 rows
-  static constexpr int kExpDma = (kRows / 64 + kWaves - 1) / kWaves;      // or the exponents of 64 rows
-  static_assert(kFn == 2 || kFn == 4, "a wave is two or four fragments of b wide");
+  static constexpr int kLds = S * (kStage + kExp);
+  static constexpr int kDma = kRows / 8 / kWaves;                // a DMA instruction fetches 8 rows, or the exponents of 64
+  static constexpr int kInFlight = kDma + 1;                     // DMA instructions of a wave per stage
+  static_assert(kFn % kRun == 0, "whole runs");
   static_assert(kDma * 8 * kWaves == kRows && BM % (8 * kWaves) == 0, "whole DMA instructions per wave and operand");
-  static constexpr int kPer = kWaves < 8 && kFn == 4 ? 64 / (8 * kWaves) : 1;      // key_b repeats after 64 rows, or 32
-  static_assert(8 * kWaves * kPer % (4 << kShift) == 0 && 8 * kWaves % 16 == 0, "the keys of the rows that a lane fetches repeat");
-  static_assert(BM % 64 == 0 && BN % 64 == 0, "64 rows of one operand per exponent fetch");
+  static_assert(8 * kWaves % 32 == 0, "the keys of the rows that a lane fetches repeat");
+  static_assert(BM % 64 == 0 && BN % 64 == 0 && kWaves % (kRows / 64) == 0, "64 rows of one operand per wave's exponent fetch");
 
   advoc::u32x4s ra, rb, rea, reb;
   const uint8_t* lds;
   unsigned base;
   int lane, wave, wm, wn, spitch;
-  int kp, voff_a, voff_b[kPer];          // what this lane fetches: its first row of a and of b, the others are 8 kWaves rows on
+  int kp, voff_a, voff_b;                // what this lane fetches: its first row of a and of b, the others are 8 kWaves rows on
   int off_a, off_b, piece0, piece1;      // this lane's first rows in a stage, its two pieces of a row
 
+  // which column of a wave's part of the output is row `row` of the matrix instruction's operand for fragment j
+  static __device__ __forceinline__ constexpr int place_b(int j, int row) {
+    return j / kRun * 16 * kRun + (row >> 2) * 4 * kRun + j % kRun * 4 + (row & 3);
+  }
   static __device__ __forceinline__ int key_a(int row) { return (row >> 1) & 7; }
-  static __device__ __forceinline__ int key_b(int row) { return ((row >> 1) & 1) | ((row >> kShift) & 3) << 1; }
+  static __device__ __forceinline__ int key_b(int row) { return kRun == 1 ? key_a(row) : ((row >> 1) & 1) | ((row >> 3) & 3) << 1; }
 
   __device__ __forceinline__ Tile(const Args& g, const uint8_t* lds_, int64_t m0, int64_t n0) : lds(lds_) {
     lane = threadIdx.x & 63;
@@ -193,33 +187,26 @@ struct Tile {
     kp = (int)g.kp;
     const int first = wave * 8 + (lane >> 3);
     voff_a = first * kp + (((lane & 7) ^ key_a(first)) << 4);
-#pragma unroll
-    for (int t = 0; t < kPer; ++t) voff_b[t] = first * kp + (((lane & 7) ^ key_b(first + t * 8 * kWaves)) << 4);
-    // fragment i of a: rows wm + 16 i + lane % 16; fragment j of b: rows wn + 4 kFn (lane % 16 / 4) + 4 j + lane % 4.  Their keys are
-    // lane / 2 % 8 for every fragment
+    voff_b = first * kp + (((lane & 7) ^ key_b(first)) << 4);
+    // fragment i of a: rows wm + 16 i + lane % 16; fragment j of b: rows wn + place_b(j, lane % 16).  Their keys are lane / 2 % 8 for
+    // every fragment
     off_a = wm + (lane & 15);
-    off_b = BM + wn + ((lane & 15) >> 2) * 4 * kFn + (lane & 3);
+    off_b = BM + wn + place_b(0, lane & 15);
     piece0 = ((lane >> 4) ^ ((lane >> 1) & 7)) << 4;
     piece1 = piece0 ^ 64;
   }
 
-  // block kb of the contraction into stage slot (kb - first) & 1, and with every fourth block the exponents of the next four
+  // block kb of the contraction into stage `slot`
   __device__ __forceinline__ void fetch(int kb, int slot) const {
 #pragma unroll
     for (int t = 0; t < kDma; ++t) {
       const unsigned to = base + slot * kStage + (t * kWaves + wave) * 1024;
       if (t * 8 * kWaves < BM) advoc::dma16(ra, to, voff_a + t * 8 * kWaves * kp, kb * kBlock);
-      else advoc::dma16(rb, to, voff_b[(t - BM / (8 * kWaves)) % kPer] + (t * 8 * kWaves - BM) * kp, kb * kBlock);
+      else advoc::dma16(rb, to, voff_b + (t * 8 * kWaves - BM) * kp, kb * kBlock);
     }
-  }
-  __device__ __forceinline__ void fetch_exponents(int quad) const {
-#pragma unroll
-    for (int t = 0; t < kExpDma; ++t) {
-      const int first = (t * kWaves + wave) * 64;
-      if (first >= kRows) break;
-      const bool is_a = first < BM;
-      advoc::dma4(is_a ? rea : reb, base + 2 * kStage + (quad & 1) * kExp + first * 4, (first + lane - (is_a ? 0 : BM)) * spitch, quad * 4);
-    }
+    const int first = wave % (kRows / 64) * 64;                  // (waves beyond the rows fetch the same dwords again)
+    const bool is_a = first < BM;
+    advoc::dma4(is_a ? rea : reb, base + S * kStage + slot * kExp + first * 4, (first + lane - (is_a ? 0 : BM)) * spitch, kb & ~3);
   }
 
   __device__ __forceinline__ i32x8 bytes(int row) const {      // slot * kRows + row of the stage
@@ -227,37 +214,68 @@ struct Tile {
     return join(*reinterpret_cast<const int4*>(p + piece0), *reinterpret_cast<const int4*>(p + piece1));
   }
   __device__ __forceinline__ i32x8 bytes_a(int slot, int i) const { return bytes(slot * kRows + off_a + i * 16); }
-  __device__ __forceinline__ i32x8 bytes_b(int slot, int j) const { return bytes(slot * kRows + off_b + j * 4); }
-  __device__ __forceinline__ int exponents(int quad, int row) const {
-    return *reinterpret_cast<const int*>(lds + 2 * kStage + ((quad & 1) * kRows + row) * 4);
-  }
-  __device__ __forceinline__ void exponents(int quad, int (&ea)[kFm], int (&eb)[kFn]) const {
-#pragma unroll
-    for (int i = 0; i < kFm; ++i) ea[i] = exponents(quad, off_a + i * 16);
-#pragma unroll
-    for (int j = 0; j < kFn; ++j) eb[j] = exponents(quad, off_b + j * 4);
-  }
+  __device__ __forceinline__ i32x8 bytes_b(int slot, int j) const { return bytes(slot * kRows + off_b + place_b(j, 0)); }
+  __device__ __forceinline__ int exponent_a(int slot, int kb, int i) const { return exponent(slot * kRows + off_a + i * 16, kb); }
+  __device__ __forceinline__ int exponent_b(int slot, int kb, int j) const { return exponent(slot * kRows + off_b + place_b(j, 0), kb); }
+  __device__ __forceinline__ int exponent(int row, int kb) const { return lds[S * kStage + row * 4 + (kb & 3)]; }
 
-  template <typename O>
+  // Four lane groups store 64 consecutive bytes of a row together.  Tiles inside the matrix have a loop of their own: next to the
+  // element-wise form the compiler cut their 16-byte stores in two (34 -> 46 us for a 16 MB output).
   __device__ __forceinline__ void store(const Args& g, int64_t m0, int64_t n0, const f32x4 (&acc)[kFm][kFn]) const {
+    constexpr int C = 4 * kRun;
+    typedef O run __attribute__((ext_vector_type(C)));
+    const bool whole = m0 + BM <= g.m && n0 + BN <= g.n && !g.accumulate;
+    if (whole) {
+      O* p = (O*)g.out + (m0 + off_a) * g.n + n0 + wn + place_b(0, (lane >> 4) * 4);
 #pragma unroll
-    for (int i = 0; i < kFm; ++i) {
-      float v[4 * kFn];
+      for (int i = 0; i < kFm; ++i, p += 16 * g.n)
 #pragma unroll
-      for (int j = 0; j < kFn; ++j)
+        for (int j = 0; j < kFn; j += kRun) {
+          run v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * j + e] = acc[i][j][e];
-      store_run<O, 4 * kFn>(g, m0 + off_a + i * 16, n0 + wn + (lane >> 4) * 4 * kFn, v);
+          for (int q = 0; q < C; ++q) v[q] = (O)acc[i][j + q / 4][q % 4];
+          __builtin_memcpy(p + place_b(j, 0), &v, sizeof(v));
+        }
+      return;
     }
+#pragma unroll
+    for (int i = 0; i < kFm; ++i)
+#pragma unroll
+      for (int j = 0; j < kFn; j += kRun) {
+        float v[C];
+#pragma unroll
+        for (int q = 0; q < C; ++q) v[q] = acc[i][j + q / 4][q % 4];
+        store_part<O, C>(g, m0 + off_a + i * 16, n0 + wn + place_b(j, (lane >> 4) * 4), v);
+      }
   }
 };
 
-template <typename O, bool EXACT, int FA, int FB, int BM, int BN, int WM, int WN, bool SPLIT>
+// A workgroup's tile.  Workgroups go to the eight XCDs in turn; each XCD gets a run of the tiles instead, those of one part of a split
+// contraction behind one another and within it eight tiles of m for one of n after the other: what runs on an XCD together shares
+// its rows in that L2.
+struct Place {
+  int64_t m0, n0;
+  int z;
+  __device__ __forceinline__ Place(const Args& g, int bm, int bn) {
+    const unsigned total = gridDim.x, q = total / 8, r = total % 8, xcd = blockIdx.x % 8;
+    unsigned at = xcd * q + (xcd < r ? xcd : r) + blockIdx.x / 8;
+    const unsigned mt = (unsigned)((g.m + bm - 1) / bm), nt = (unsigned)((g.n + bn - 1) / bn);
+    z = at / (mt * nt);
+    at -= z * mt * nt;
+    const unsigned band = at / (8 * nt), first = band * 8, rows = mt - first < 8 ? mt - first : 8;
+    at -= band * 8 * nt;
+    m0 = (int64_t)(first + at % rows) * bm;
+    n0 = (int64_t)(at / rows) * bn;
+  }
+};
+
+template <typename O, bool EXACT, int FA, int FB, int BM, int BN, int WM, int WN, int S, bool SPLIT>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void f8_tile_kernel(Args g) {
-  using T = Tile<BM, BN, WM, WN>;
+  using T = Tile<O, BM, BN, WM, WN, S>;
   __shared__ __align__(1024) uint8_t lds[T::kLds];
-  const int64_t m0 = (int64_t)blockIdx.x * BM, n0 = (int64_t)blockIdx.y * BN;
-  const int kb0 = SPLIT ? blockIdx.z * g.per_split : 0;
+  const Place at(g, BM, BN);
+  const int64_t m0 = at.m0, n0 = at.n0;
+  const int kb0 = SPLIT ? at.z * g.per_split : 0;
   const int kb1 = SPLIT ? (kb0 + g.per_split < g.blocks ? kb0 + g.per_split : g.blocks) : g.blocks;
   const T t(g, lds, m0, n0);
 
@@ -267,38 +285,70 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void f8_tile_kernel(Args 
 #pragma unroll
     for (int j = 0; j < T::kFn; ++j) acc[i][j] = (f32x4)(0.f);
 
+  // Block kb is in registers when its turn comes: the reads of kb + 1 go out in front of the multiplications of kb, and with them the
+  // fetch of kb + S into the stage that kb has left.
+  i32x8 qa[T::kFm], qb[T::kFn];
   int ea[T::kFm], eb[T::kFn];
-  t.fetch_exponents(kb0 >> 2);
-  t.fetch(kb0, 0);
+  auto read = [&](int slot, int kb) {
+#pragma unroll
+    for (int j = 0; j < T::kFn; ++j) qb[j] = t.bytes_b(slot, j), eb[j] = t.exponent_b(slot, kb, j);
+#pragma unroll
+    for (int i = 0; i < T::kFm; ++i) qa[i] = t.bytes_a(slot, i), ea[i] = t.exponent_a(slot, kb, i);
+  };
+  for (int kb = kb0; kb < kb0 + S && kb < kb1; ++kb) t.fetch(kb, kb - kb0);
+  if (kb0 + S - 1 < kb1) advoc::dma_ring_barrier<(S - 1) * T::kInFlight>();
+  else advoc::dma_ring_barrier<0>();
+  read(0, kb0);
+  int slot = 0;
+#pragma unroll 2
   for (int kb = kb0; kb < kb1; ++kb) {
-    const int slot = (kb - kb0) & 1;
-    advoc::dma_ring_barrier<0>();
-    if (kb + 1 < kb1) {
-      if (((kb + 1) & 3) == 0) t.fetch_exponents((kb + 1) >> 2);
-      t.fetch(kb + 1, slot ^ 1);
-    }
-    if (kb == kb0 || (kb & 3) == 0) t.exponents(kb >> 2, ea, eb);
-    const int shift = (kb & 3) * 8;
-    auto frag_b = [&](int j) { return Frag<FB, EXACT>(t.bytes_b(slot, j), eb[j] >> shift & 255); };
+    // everyone holds block kb, block kb + 1 has landed; S - 2 younger stages may be in flight, the last ones are waited for
+    if (kb + S - 1 < kb1) advoc::dma_ring_barrier<(S - 2) * T::kInFlight>();
+    else advoc::dma_ring_barrier<0>();
+    if (kb + S < kb1) t.fetch(kb + S, slot);
+    slot = slot == S - 1 ? 0 : slot + 1;
     auto multiply = [&](const auto&... b) {
+      const Frag<FA, EXACT> fa[] = {{qa[0], ea[0]}, {qa[1], ea[1]}, {qa[T::kFm - 2], ea[T::kFm - 2]}, {qa[T::kFm - 1], ea[T::kFm - 1]}};
+      read(slot, kb + 1);      // (behind the last block: what lies there, unused)
 #pragma unroll
       for (int i = 0; i < T::kFm; ++i) {
-        const Frag<FA, EXACT> a(t.bytes_a(slot, i), ea[i] >> shift & 255);
         int j = 0;
-        ((acc[i][j] = mfma<FA, FB>(b, a, acc[i][j]), ++j), ...);
+        ((acc[i][j] = mfma<FA, FB>(b, fa[i < 2 ? i : i + 4 - T::kFm], acc[i][j]), ++j), ...);
       }
     };
-    if constexpr (T::kFn == 2) multiply(frag_b(0), frag_b(1));
-    else multiply(frag_b(0), frag_b(1), frag_b(2), frag_b(3));
+    static_assert(T::kFm == 2 || T::kFm == 4, "two or four fragments of a");
+    if constexpr (T::kFn == 2) multiply(Frag<FB, EXACT>(qb[0], eb[0]), Frag<FB, EXACT>(qb[1], eb[1]));
+    else multiply(Frag<FB, EXACT>(qb[0], eb[0]), Frag<FB, EXACT>(qb[1], eb[1]), Frag<FB, EXACT>(qb[2], eb[2]), Frag<FB, EXACT>(qb[3], eb[3]));
   }
 
   Args o = g;
   if constexpr (SPLIT) {
-    o.out = g.part + (int64_t)blockIdx.z * g.m * g.n;
+    o.out = g.part + (int64_t)at.z * g.m * g.n;
     o.accumulate = 0;
   }
-  t.template store<O>(o, m0, n0, acc);
+  t.store(o, m0, n0, acc);
 }
+
+// The instruction as assembly, so that it stays between two rendezvous: the compiler sinks the builtin below the second one, out of
+// its turn, and moves all accumulators once a block for it (349 against 314 us at 16384 x 4096 x 4096).  It waits the two states that
+// a vector instruction's result needs before a matrix instruction reads it.  Whoever reads an accumulator by other means waits for
+// the instruction himself and then says settled().
+// BYTE_B, BYTE_A: which byte of the exponent registers.
+template <int FA, int FB, int BYTE_B, int BYTE_A>
+__device__ __forceinline__ void mfma_in_place(f32x4& c, const i32x8& b, const i32x8& a, int bytes_b, int bytes_a) {
+  asm volatile(
+      "s_nop 1\n\t"
+      "v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel:[%7,%8,0] op_sel_hi:[%9,%10,0] cbsz:%5 blgp:%6"
+      : "+v"(c)
+      : "v"(b), "v"(a), "v"(bytes_b), "v"(bytes_a), "n"(FB), "n"(FA), "n"(BYTE_B & 1), "n"(BYTE_A & 1), "n"(BYTE_B >> 1), "n"(BYTE_A >> 1));
+}
+// acc[i][j] += b[j] a[i] for every i, j; the exponents of four fragments are the bytes of one register
+template <int FA, int FB, int FM, int FN, int... K>
+__device__ __forceinline__ void mfma_all(f32x4 (&acc)[FM][FN], const i32x8 (&b)[FN], const i32x8 (&a)[FM], const int (&eb)[FN / 4],
+                                         const int (&ea)[FM / 4], std::integer_sequence<int, K...>) {
+  (mfma_in_place<FA, FB, K % FN % 4, K / FN % 4>(acc[K / FN][K % FN], b[K % FN], a[K / FN], eb[K % FN / 4], ea[K / FN / 4]), ...);
+}
+__device__ __forceinline__ void settled(f32x4& c) { asm volatile("" : "+v"(c)); }
 
 // 256 x 256 outputs, eight waves of 128 x 64, the 8-bit instruction.  Two waves share a SIMD and take turns: while the waves of one
 // half of the workgroup read the fragments of a block from LDS (24 reads of 16 bytes a lane: 768 cycles of the CU's 128 bytes a
@@ -306,9 +356,10 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void f8_tile_kernel(Args 
 // matrix pipe has work in both halves of a block's time.
 template <typename O, int FA, int FB>
 __global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
-  using T = Tile<256, 256, 128, 64>;
+  using T = Tile<O, 256, 256, 128, 64, 2>;
   __shared__ __align__(1024) uint8_t lds[T::kLds];
-  const int64_t m0 = (int64_t)blockIdx.x * 256, n0 = (int64_t)blockIdx.y * 256;
+  const Place at(g, 256, 256);
+  const int64_t m0 = at.m0, n0 = at.n0;
   const T t(g, lds, m0, n0);
 
   f32x4 acc[T::kFm][T::kFn];
@@ -317,7 +368,7 @@ __global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
 #pragma unroll
     for (int j = 0; j < T::kFn; ++j) acc[i][j] = (f32x4)(0.f);
   i32x8 a[T::kFm], b[T::kFn];
-  int ea[T::kFm], eb[T::kFn];
+  int ea[T::kFm / 4], eb[T::kFn / 4];
 
   auto read = [&](int kb) {
     const int slot = kb & 1;
@@ -325,33 +376,20 @@ __global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
     for (int j = 0; j < T::kFn; ++j) b[j] = t.bytes_b(slot, j);
 #pragma unroll
     for (int i = 0; i < T::kFm; ++i) a[i] = t.bytes_a(slot, i);
-    if ((kb & 3) == 0) {
-      t.exponents(kb >> 2, ea, eb);
-    } else {
 #pragma unroll
-      for (int i = 0; i < T::kFm; ++i) ea[i] >>= 8;
+    for (int i = 0; i < T::kFm; i += 4)
+      ea[i / 4] = t.exponent_a(slot, kb, i) | t.exponent_a(slot, kb, i + 1) << 8 | t.exponent_a(slot, kb, i + 2) << 16 | t.exponent_a(slot, kb, i + 3) << 24;
 #pragma unroll
-      for (int j = 0; j < T::kFn; ++j) eb[j] >>= 8;
-    }
+    for (int j = 0; j < T::kFn; j += 4)
+      eb[j / 4] = t.exponent_b(slot, kb, j) | t.exponent_b(slot, kb, j + 1) << 8 | t.exponent_b(slot, kb, j + 2) << 16 | t.exponent_b(slot, kb, j + 3) << 24;
   };
-  // The instruction as assembly, so that it stays between its two rendezvous: the compiler sinks the builtin below the second one,
-  // out of its turn, and moves all accumulators once a block for it (349 against 314 us at 16384 x 4096 x 4096).  Each statement waits the two states that
-  // a vector instruction's result needs before a matrix instruction reads it; a fragment's accumulator comes round every 32
-  // instructions.
   auto multiply = [&]() {
     __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-    for (int i = 0; i < T::kFm; ++i)
-#pragma unroll
-      for (int j = 0; j < T::kFn; ++j)
-        asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:%5 blgp:%6"
-                     : "+v"(acc[i][j])
-                     : "v"(b[j]), "v"(a[i]), "v"(eb[j]), "v"(ea[i]), "n"(FB), "n"(FA));
+    mfma_all<FA, FB>(acc, b, a, eb, ea, std::make_integer_sequence<int, T::kFm * T::kFn>());
     __builtin_amdgcn_s_setprio(0);
   };
   auto fetch = [&](int kb) {
     if (kb >= g.blocks) return;
-    if ((kb & 3) == 0) t.fetch_exponents(kb >> 2);
     t.fetch(kb, kb & 1);
   };
   auto meet = [&](bool landed) {      // my reads have arrived and, with `landed`, what I fetched lies in LDS
@@ -385,8 +423,8 @@ __global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
 #pragma unroll
   for (int i = 0; i < T::kFm; ++i)
 #pragma unroll
-    for (int j = 0; j < T::kFn; ++j) asm volatile("" : "+v"(acc[i][j]));
-  t.template store<O>(g, m0, n0, acc);
+    for (int j = 0; j < T::kFn; ++j) settled(acc[i][j]);
+  t.store(g, m0, n0, acc);
 }
 
 // the parts of a split contraction, added in order
@@ -411,7 +449,7 @@ Plan make_plan(int64_t m, int64_t n, int blocks, bool exact) {
   const int64_t t256 = ceil_div(m, 256) * ceil_div(n, 256), t128 = ceil_div(m, 128) * ceil_div(n, 128);
   p.form = t256 >= 192 && !exact ? kTile256 : t128 >= 64 ? kTile128 : kTile64;
   const int64_t tiles = p.form == kTile256 ? t256 : p.form == kTile128 ? t128 : ceil_div(m, 64) * ceil_div(n, 64);
-  int64_t splits = 512 / tiles;
+  int64_t splits = (p.form == kTile64 ? 512 : 256) / tiles;
   if (splits > blocks / 8) splits = blocks / 8;
   if (splits > 1 && p.form != kTile256) {
     p.per_split = (int)ceil_div(blocks, splits);
@@ -420,11 +458,11 @@ Plan make_plan(int64_t m, int64_t n, int blocks, bool exact) {
   return p;
 }
 
-template <typename O, bool EXACT, int FA, int FB, int BM, int BN, int WM, int WN, bool SPLIT>
+template <typename O, bool EXACT, int FA, int FB, int BM, int BN, int WM, int WN, int S, bool SPLIT>
 int run_tile(const Args& g, int splits, hipStream_t stream) {
   constexpr int kThreads = BM / WM * (BN / WN) * 64;
-  const dim3 grid((unsigned)ceil_div(g.m, BM), (unsigned)ceil_div(g.n, BN), (unsigned)splits);
-  hipLaunchKernelGGL((f8_tile_kernel<O, EXACT, FA, FB, BM, BN, WM, WN, SPLIT>), grid, dim3(kThreads), 0, stream, g);
+  const dim3 grid((unsigned)(ceil_div(g.m, BM) * ceil_div(g.n, BN) * splits));
+  hipLaunchKernelGGL((f8_tile_kernel<O, EXACT, FA, FB, BM, BN, WM, WN, S, SPLIT>), grid, dim3(kThreads), 0, stream, g);
   ADVOC_RETURN_IF_LAUNCH_FAILED();
   return ADVOC_OK;
 }
@@ -445,17 +483,17 @@ int run(const Args& g, const Plan& p, hipStream_t stream) {
   }
   if constexpr (!EXACT) {
     if (p.form == kTile256) {
-      const dim3 grid((unsigned)ceil_div(g.m, 256), (unsigned)ceil_div(g.n, 256));
+      const dim3 grid((unsigned)(ceil_div(g.m, 256) * ceil_div(g.n, 256)));
       hipLaunchKernelGGL((f8_big_kernel<O, FA, FB>), grid, dim3(512), 0, stream, g);
       ADVOC_RETURN_IF_LAUNCH_FAILED();
       return ADVOC_OK;
     }
   }
   if (p.splits == 1)
-    return p.form == kTile128 ? run_tile<O, EXACT, FA, FB, 128, 128, 64, 64, false>(g, 1, stream)
-                              : run_tile<O, EXACT, FA, FB, 64, 64, 32, 32, false>(g, 1, stream);
-  const int rc = p.form == kTile128 ? run_tile<float, EXACT, FA, FB, 128, 128, 64, 64, true>(g, p.splits, stream)
-                                    : run_tile<float, EXACT, FA, FB, 64, 64, 32, 32, true>(g, p.splits, stream);
+    return p.form == kTile128 ? run_tile<O, EXACT, FA, FB, 128, 128, 64, 32, 4, false>(g, 1, stream)
+                              : run_tile<O, EXACT, FA, FB, 64, 64, 32, 32, 4, false>(g, 1, stream);
+  const int rc = p.form == kTile128 ? run_tile<float, EXACT, FA, FB, 128, 128, 64, 32, 4, true>(g, p.splits, stream)
+                                    : run_tile<float, EXACT, FA, FB, 64, 64, 32, 32, 4, true>(g, p.splits, stream);
   if (rc != ADVOC_OK) return rc;
   const int64_t count = g.m * g.n, blocks = ceil_div(count, 256);
   ADVOC_CLEAR_LAUNCH_ERROR();
@@ -491,8 +529,8 @@ extern "C" int advoc_matmul_nt_f8(const uint8_t* a, const uint8_t* a_scale, int3
     return ADVOC_ERR_UNSUPPORTED;
   if (!advoc::dtype_ok(out_dtype) || (accumulate && out_dtype != ADVOC_F32)) return ADVOC_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) return ADVOC_ERR_UNSUPPORTED;
-  // 256 rows of an operand lie behind one 32-bit descriptor; tiles of n are a grid's second dimension
-  if (k > 8000000 || m > 64LL * 0x7fffffff || n > 64LL * 65535) return ADVOC_ERR_UNSUPPORTED;
+  // 256 rows of an operand lie behind one 32-bit descriptor; tiles are numbered in 31 bits
+  if (k > 8000000 || m > (1LL << 31) || n > (1LL << 31) || ceil_div(m, 64) * ceil_div(n, 64) > 0x3fffffff) return ADVOC_ERR_UNSUPPORTED;
   Args g = {a, a_scale, b, b_scale, out, static_cast<float*>(workspace), m, n};
   g.blocks = (int)ceil_div(k, kBlock);
   g.kp = (int64_t)g.blocks * kBlock;

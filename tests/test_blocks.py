@@ -173,7 +173,7 @@ def test_f8_entries_refuse(lib):
   for k in ('a', 'sa', 'b', 'sb', 'out'):
     assert mul(**{k: None}) == -4
   assert mul(m=-1) == -1 and mul(k=0) == -1 and mul(fa=2) == -2 and mul(fb=-1) == -2 and mul(dtype=5) == -2
-  assert mul(acc=1, dtype=1) == -2 and mul(a=72) == -2 and mul(k=2 ** 24) == -2 and mul(n=2 ** 23) == -2
+  assert mul(acc=1, dtype=1) == -2 and mul(a=72) == -2 and mul(k=2 ** 24) == -2 and mul(n=2 ** 32) == -2 and mul(m=2 ** 24, n=2 ** 24) == -2
   assert mul(m=0) == 0 and mul(n=0, out=None) == 0
   assert lib.advoc_matmul_nt_f8_workspace_bytes(0, 4, 4, 0) == 0 and lib.advoc_matmul_nt_f8_workspace_bytes(1, 4, 4, 0) == 0
 
