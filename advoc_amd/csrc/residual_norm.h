@@ -110,7 +110,7 @@ static inline bool norm_dispatch(int cols, F&& f) {
   else if (cols <= 512) f.template run<8, 64, 1>();
   else if (cols <= 1024) f.template run<8, 64, 2>();
   else if (cols <= 2048) f.template run<8, 256, 1>();
-  else if (cols <= 4096) f.template run<8, 256, 2>();
+  else if (cols <= 4096) f.template run<8, 512, 1>();
   else if (cols <= 8192) f.template run<8, 512, 2>();
   else return false;
   return true;

@@ -27,11 +27,13 @@ struct Sums {
 };
 
 // Lanes of a workgroup and waves per SIMD.  Rows of 16 columns a lane: 256 registers, a third of them sums, and 512 lanes to a
-// workgroup (half the partial column sums of 256); rows of 8: three waves to a SIMD.
+// workgroup (half the partial column sums of 256); rows of 8: three waves to a SIMD (8192 x 2048 fp32: 90.5 us, two 92.4).  A row of
+// 4096 columns is 512 lanes of 8, one workgroup to a CU: 4096 rows take 88 us, with registers for three waves 115 (they spill),
+// 256 lanes of 16 97.
 template <int L, int NV>
 constexpr int kLanes = L > 64 ? L : NV > 1 ? 512 : 256;
-template <int NV>
-constexpr int kWavesPerSimd = NV > 1 ? 2 : 3;
+template <int L, int NV>
+constexpr int kWavesPerSimd = NV > 1 || L > 256 ? 2 : 3;
 
 // t <- the gradient of a row given that of its normed values (times the weight): rstd (t - [mean t] - hat mean(t hat))
 template <int V, int L, int NV, int WG>
@@ -50,7 +52,7 @@ __device__ __forceinline__ void norm_back(f32x8 (&t)[NV], const f32x8 (&hat)[NV]
 // absent is not a branch (register allocation around those cost more than the work they save): an absent dr or gate is read from
 // where r or h lies and replaced by its neutral value, absent vectors are staged as theirs.
 template <typename T, typename R, int V, int L, int NV, int WG, bool H, bool PRE>
-__global__ __launch_bounds__(WG, kWavesPerSimd<NV>) void norm_backward_kernel(NormArgs a, Sums sums) {
+__global__ __launch_bounds__(WG, (kWavesPerSimd<L, NV>)) void norm_backward_kernel(NormArgs a, Sums sums) {
   using Row = Team<L, WG>;
   __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
   extern __shared__ float vec[];                // w_pre, w_post, b_post, scale; afterwards the column sums of the workgroup's rows
@@ -289,7 +291,7 @@ struct MakePlan {
   template <int V, int L, int NV>
   void run() const {
     constexpr int kRows = Team<L, kLanes<L, NV>>::kRows;
-    const int64_t most = 256 * 4 * 64 * kWavesPerSimd<NV> / kLanes<L, NV>;      // what is resident together
+    const int64_t most = 256 * 4 * 64 * kWavesPerSimd<L, NV> / kLanes<L, NV>;      // what is resident together
     const bool shared_gate = a.gate && a.gate_group > 1;
     const int64_t rows = shared_gate ? a.gate_group : a.rows, groups = a.rows / rows;
     int64_t splits = most * kRows / groups;

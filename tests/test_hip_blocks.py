@@ -198,6 +198,12 @@ def test_norm_rows_and_clips(blocks, lead):
   check_norm(blocks, 1, lead, 72, 'f16', 'f32', *KINDS[1])
 
 
+@pytest.mark.parametrize('lead,cols', [((13000, 2), 16), ((2500, 2), 1000), ((900, 3), 1100), ((300, 2), 2500), ((130, 2), 4100)])
+def test_norm_more_clips_than_workers(blocks, lead, cols):
+  """A worker that passes through several gate rows carries the sums of those before, at every width that holds rows its own way."""
+  check_norm(blocks, 3, lead, cols, 'bf16', 'bf16', *KINDS[1])
+
+
 def test_norm_many_rows(blocks):
   check_norm(blocks, 2, (3, 5001), 16, 'bf16', 'bf16', *KINDS[3])
 
