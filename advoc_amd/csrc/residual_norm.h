@@ -116,10 +116,11 @@ static inline bool norm_dispatch(int cols, F&& f) {
   return true;
 }
 
-// One chunk's place: first column, how many leading values a neighbour holds too (V: none are this lane's own).
+// One chunk's place: which one it is, its first column, how many leading values a neighbour holds too (V: none are this lane's own).
 template <int V, int L>
-__device__ __forceinline__ void chunk_place(int j, int lane, int cols, int& col, int& dup) {
-  const int at = (j * L + lane) * V;
+__device__ __forceinline__ void chunk_place(int j, int lane, int cols, int& chunk, int& col, int& dup) {
+  const int last = (cols + V - 1) / V - 1, at = (j * L + lane) * V;
+  chunk = j * L + lane < last ? j * L + lane : last;
   col = at <= cols - V ? at : cols - V;
   dup = at < cols ? at - col : V;
 }
@@ -159,16 +160,64 @@ __device__ __forceinline__ void store_chunk(T* p, const f32x8& v) {
   else *p = (T)v[0];
 }
 
-// The column vectors of a call in LDS, [which][cols], an absent one as its neutral value: a lane reads its columns of them for every
-// row (kept in registers they cost the waves that hide the loads' latency; from the caches, a round trip per vector and row).
-// (the compiler would carry what it has read of them from row to row in registers, and spill)
-__device__ __forceinline__ void forget_lds() { asm volatile("" ::: "memory"); }
-template <int WG>
-__device__ __forceinline__ void stage_vector(float* lds, const float* p, float otherwise, int cols) {
-  for (int c = threadIdx.x; c < cols; c += WG) lds[c] = p ? p[c] : otherwise;
-}
+// Column vectors in LDS: the lanes' chunks side by side, so that 64 lanes read or write theirs without a bank twice.  The first four
+// values of every chunk lie together, then the last four (V = 1: value by value).  The moved-back chunk at the row's end is the last
+// one.  A lane reads its columns of the call's vectors for every row (kept in registers they cost the waves that hide the loads'
+// latency; from the caches, a round trip per vector and row); an absent vector is staged as its neutral value.
 template <int V>
-__device__ __forceinline__ f32x8 cols_chunk(const float* p) {
+struct Chunks {
+  int count;                    // V = 8: of chunks;  V = 1: of columns
+  __host__ __device__ __forceinline__ explicit Chunks(int cols) : count(V == 8 ? (cols + 7) / 8 : cols) {}
+  __host__ __device__ __forceinline__ int floats() const { return count * V; }
+  __device__ __forceinline__ f32x8 get(const float* vec, int chunk) const {
+    f32x8 f(0.f);
+    if constexpr (V == 8) {
+      const float4 a = reinterpret_cast<const float4*>(vec)[chunk], b = reinterpret_cast<const float4*>(vec)[count + chunk];
+      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    } else f[0] = vec[chunk];
+    return f;
+  }
+  __device__ __forceinline__ void put(float* vec, int chunk, const f32x8& f) const {
+    if constexpr (V == 8) {
+      reinterpret_cast<float4*>(vec)[chunk] = make_float4(f[0], f[1], f[2], f[3]);
+      reinterpret_cast<float4*>(vec)[count + chunk] = make_float4(f[4], f[5], f[6], f[7]);
+    } else vec[chunk] = f[0];
+  }
+  // the columns that four values (V = 1: one) at `at` of such a vector stand for
+  static constexpr int kPiece = V == 8 ? 4 : 1;
+  __device__ __forceinline__ int pieces() const { return V == 8 ? 2 * count : count; }
+  __device__ __forceinline__ int piece_col(int piece, int cols) const {
+    if constexpr (V == 1) return piece;
+    const int half = piece >= count, at = 8 * (piece - half * count);
+    return (at <= cols - 8 ? at : cols - 8) + 4 * half;
+  }
+};
+
+// (the compiler would carry what it has read of LDS from row to row in registers, and spill)
+__device__ __forceinline__ void forget_lds() { asm volatile("" ::: "memory"); }
+
+// Stages N vectors p[i] (where absent: otherwise[i]), a piece of each a lane, all in flight before the first is written.
+template <int WG, int V, int N>
+__device__ __forceinline__ void stage_vectors(float* lds, const float* const (&p)[N], const float (&otherwise)[N], int cols) {
+  const Chunks<V> chunks(cols);
+  constexpr int kPiece = Chunks<V>::kPiece;
+  for (int q = threadIdx.x; q < chunks.pieces(); q += WG) {
+    const int col = chunks.piece_col(q, cols);
+    float v[N][kPiece];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int k = 0; k < kPiece; ++k) v[i][k] = otherwise[i];
+      if (p[i]) __builtin_memcpy(v[i], p[i] + col, sizeof(v[i]));
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) __builtin_memcpy(__builtin_assume_aligned(lds + i * chunks.floats() + q * kPiece, 4 * kPiece), v[i], sizeof(v[i]));
+  }
+}
+
+// V consecutive floats in global memory
+template <int V>
+__device__ __forceinline__ f32x8 floats_at(const float* p) {
   f32x8 f(0.f);
   if constexpr (V == 8) __builtin_memcpy(f.v, p, sizeof(f.v));
   else f[0] = *p;

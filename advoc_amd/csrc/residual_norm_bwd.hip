@@ -27,13 +27,17 @@ struct Sums {
 };
 
 // Lanes of a workgroup and waves per SIMD.  Rows of 16 columns a lane: 256 registers, a third of them sums, and 512 lanes to a
-// workgroup (half the partial column sums of 256); rows of 8: three waves to a SIMD (8192 x 2048 fp32: 90.5 us, two 92.4).  A row of
+// workgroup (half the partial column sums of 256); rows of 8: three waves to a SIMD (8192 x 2048: 90.5 us, two 92.4).  A row of
 // 4096 columns is 512 lanes of 8, one workgroup to a CU: 4096 rows take 88 us, with registers for three waves 115 (they spill),
 // 256 lanes of 16 97.
 template <int L, int NV>
 constexpr int kLanes = L > 64 ? L : NV > 1 ? 512 : 256;
 template <int L, int NV>
 constexpr int kWavesPerSimd = NV > 1 || L > 256 ? 2 : 3;
+
+// Column sums that go through LDS together at the end of a workgroup: 40 KB with three workgroups to a CU, 128 KB with one.
+template <int NV>
+constexpr int kSumsTogether = NV > 1 ? 4 : 5;
 
 // t <- the gradient of a row given that of its normed values (times the weight): rstd (t - [mean t] - hat mean(t hat))
 template <int V, int L, int NV, int WG>
@@ -55,7 +59,7 @@ template <typename T, typename R, int V, int L, int NV, int WG, bool H, bool PRE
 __global__ __launch_bounds__(WG, (kWavesPerSimd<L, NV>)) void norm_backward_kernel(NormArgs a, Sums sums) {
   using Row = Team<L, WG>;
   __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
-  extern __shared__ float vec[];                // w_pre, w_post, b_post, scale; afterwards the column sums of the workgroup's rows
+  extern __shared__ __align__(16) float vec[];                // w_pre, w_post, b_post, scale; afterwards the column sums of the workgroup's rows
   int turn = 0;
   const int lane = Row::lane(), cols = a.cols;
   const uint2 key = advoc::drop_key_words(a.key);
@@ -66,18 +70,18 @@ __global__ __launch_bounds__(WG, (kWavesPerSimd<L, NV>)) void norm_backward_kern
   const void* dr = has_dr ? a.dr : a.x;
   const void* gate_base = has_gate ? a.gate : a.h;
   const int64_t dr_pitch = has_dr ? a.dr_pitch : a.x_pitch, gate_pitch = has_gate ? a.gate_pitch : a.h_pitch;
-  int col[NV], dup[NV];
+  int chunk[NV], col[NV], dup[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, cols, col[j], dup[j]);
+  for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, cols, chunk[j], col[j], dup[j]);
 
-  advoc::stage_vector<WG>(vec, a.w_pre, 1.f, cols);
-  advoc::stage_vector<WG>(vec + cols, a.w_post, 1.f, cols);
-  advoc::stage_vector<WG>(vec + 2 * cols, a.b_post, 0.f, cols);
-  advoc::stage_vector<WG>(vec + 3 * cols, a.scale, 1.f, cols);
-  auto w_pre = [&](int j) { return advoc::cols_chunk<V>(vec + col[j]); };
-  auto w_post = [&](int j) { return advoc::cols_chunk<V>(vec + cols + col[j]); };
-  auto b_post = [&](int j) { return advoc::cols_chunk<V>(vec + 2 * cols + col[j]); };
-  auto scale = [&](int j) { return advoc::cols_chunk<V>(vec + 3 * cols + col[j]); };
+  const advoc::Chunks<V> chunks(cols);
+  const int floats = chunks.floats();
+  auto w_pre = [&](int j) { return chunks.get(vec, chunk[j]); };
+  auto w_post = [&](int j) { return chunks.get(vec + floats, chunk[j]); };
+  auto b_post = [&](int j) { return chunks.get(vec + 2 * floats, chunk[j]); };
+  auto scale = [&](int j) { return chunks.get(vec + 3 * floats, chunk[j]); };
+
+  advoc::stage_vectors<WG, V, 4>(vec, {a.w_pre, a.w_post, a.b_post, a.scale}, {1.f, 1.f, 0.f, 1.f}, cols);
   Row::meet();
 
   // sums over rows.  g0, g1 are E0, E1 but for the gate where rows share one
@@ -192,8 +196,8 @@ __global__ __launch_bounds__(WG, (kWavesPerSimd<L, NV>)) void norm_backward_kern
         if (carry) {
           float *c0 = carry + j * L * V, *c1 = c0 + kOwn;
           if (again) {
-            g0[j] += advoc::cols_chunk<V>(c0);
-            g1[j] += advoc::cols_chunk<V>(c1);
+            g0[j] += advoc::floats_at<V>(c0);
+            g1[j] += advoc::floats_at<V>(c1);
           }
           advoc::store_chunk<V>(c0, g0[j]);
           advoc::store_chunk<V>(c1, g1[j]);
@@ -213,22 +217,42 @@ __global__ __launch_bounds__(WG, (kWavesPerSimd<L, NV>)) void norm_backward_kern
     out[kDwPre][j] = dw_pre[j];
     out[kDbPre][j] = db_pre[j];
   }
+  if constexpr (L > 64) {
 #pragma unroll
-  for (int s = 0; s < kSums; ++s) {
-    if (sums.slot[s] < 0) continue;
-    float* to = a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * cols;
-    if constexpr (L > 64) {
+    for (int s = 0; s < kSums; ++s)
+      if (sums.slot[s] >= 0)
 #pragma unroll
-      for (int j = 0; j < NV; ++j) advoc::store_chunk<V>(to + col[j], out[s][j]);
-    } else {
+        for (int j = 0; j < NV; ++j)
+          advoc::store_chunk<V>(a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * cols + col[j], out[s][j]);
+  } else {
+    // kTogether sums at a time: [sum][row of the workgroup] in LDS
+    constexpr int kTogether = kSumsTogether<NV>, kPiece = advoc::Chunks<V>::kPiece;
+#pragma unroll
+    for (int first = 0; first < kSums; first += kTogether) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < NV; ++j) advoc::store_chunk<V>(vec + Row::slot() * cols + col[j], out[s][j]);
+      for (int s = first; s < kSums && s < first + kTogether; ++s)
+        if (sums.slot[s] >= 0)
+#pragma unroll
+          for (int j = 0; j < NV; ++j) chunks.put(vec + ((s - first) * Row::kRows + Row::slot()) * floats, chunk[j], out[s][j]);
       __syncthreads();
-      for (int c = threadIdx.x; c < cols; c += WG) {
-        float v = 0.f;
-        for (int w = 0; w < Row::kRows; ++w) v += vec[w * cols + c];
-        to[c] = v;
+      for (int q = threadIdx.x; q < chunks.pieces(); q += WG) {
+        const int c = chunks.piece_col(q, cols);
+#pragma unroll
+        for (int s = first; s < kSums && s < first + kTogether; ++s) {
+          if (sums.slot[s] < 0) continue;
+          const float* from = vec + (s - first) * Row::kRows * floats + q * kPiece;
+          float v[kPiece];
+#pragma unroll
+          for (int k = 0; k < kPiece; ++k) v[k] = 0.f;
+          for (int w = 0; w < Row::kRows; ++w) {
+            float x[kPiece];
+            __builtin_memcpy(x, __builtin_assume_aligned(from + w * floats, 4 * kPiece), sizeof(x));
+#pragma unroll
+            for (int k = 0; k < kPiece; ++k) v[k] += x[k];
+          }
+          __builtin_memcpy(a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * cols + c, v, sizeof(v));
+        }
       }
     }
   }
@@ -319,7 +343,7 @@ struct Launch {
   void run() const {
     constexpr int WG = kLanes<L, NV>, kRows = Team<L, WG>::kRows;
     const dim3 grid((unsigned)blocks), block(WG);
-    const unsigned lds = 4u * a.cols * (kRows > 4 ? kRows : 4);
+    const unsigned lds = 4u * advoc::Chunks<V>(a.cols).floats() * (L > 64 ? 4 : kRows * kSumsTogether<NV>);
     if (!a.h) hipLaunchKernelGGL((norm_backward_kernel<T, R, V, L, NV, WG, false, true>), grid, block, lds, stream, a, sums);
     else if (a.pre == ADVOC_NORM_NONE) hipLaunchKernelGGL((norm_backward_kernel<T, R, V, L, NV, WG, true, false>), grid, block, lds, stream, a, sums);
     else hipLaunchKernelGGL((norm_backward_kernel<T, R, V, L, NV, WG, true, true>), grid, block, lds, stream, a, sums);

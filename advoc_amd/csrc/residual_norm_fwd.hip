@@ -35,76 +35,89 @@ __device__ __forceinline__ void row_stats(const f32x8 (&a)[NV], const int (&dup)
 template <int V, int L, int NV>
 constexpr bool kFiveVectors = V * L * NV <= 4096;
 
-// The next row's loads are in flight while a row is computed.
-template <typename T, typename R, int V, int L, int NV, int WG>
-__global__ __launch_bounds__(WG) void norm_forward_kernel(NormArgs a) {
+// H: there is a block output; PRE: there is a pre norm.  Nothing else that may be absent is a branch around memory: an absent gate is
+// read from where h lies and replaced by ones.
+// The next row's loads are in flight while a row is computed.  A wave waits for its loads and stores in the order of their issue, so
+// that holds only while the number of stores behind the loads is known where the loads are waited for.
+template <typename T, typename R, int V, int L, int NV, int WG, bool H, bool PRE>
+__global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
   using Row = Team<L, WG>;
-  extern __shared__ float vec[];                // scale, w_post, b_post, w_pre and, where five fit into LDS, b_pre
+  extern __shared__ __align__(16) float vec[];                // scale, w_post, b_post, w_pre and, where five fit into LDS, b_pre
+  constexpr bool kAhead = NV == 1;
   constexpr bool kFive = kFiveVectors<V, L, NV>;
   __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
   int turn = 0;
   const int lane = Row::lane(), cols = a.cols;
   const uint2 key = advoc::drop_key_words(a.key);
-  const bool aligned = (cols & 3) == 0, ragged = cols % V != 0;
-  int col[NV], dup[NV];
+  const bool aligned = (cols & 3) == 0, ragged = cols % V != 0, has_gate = a.gate, post = a.post != ADVOC_NORM_NONE;
+  const void* gate_base = has_gate ? a.gate : a.h;
+  const int64_t gate_pitch = has_gate ? a.gate_pitch : a.h_pitch;
+  const uint32_t gate_group = has_gate ? (uint32_t)a.gate_group : 1u;
+  int chunk[NV], col[NV], dup[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, cols, col[j], dup[j]);
+  for (int j = 0; j < NV; ++j) advoc::chunk_place<V, L>(j, lane, cols, chunk[j], col[j], dup[j]);
 
+  const advoc::Chunks<V> chunks(cols);
+  const int floats = chunks.floats();
   advoc::Raw<T, V, NV> h, gate;
   advoc::Raw<R, V, NV> x;
   auto load = [&](int64_t row) {
     if (row >= a.rows) row = a.rows - 1;        // (the lanes of a wave leave the loop together)
     x.load(a.x, row * a.x_pitch, col);
-    if (a.h) h.load(a.h, row * a.h_pitch, col);
-    if (a.gate) gate.load(a.gate, (int64_t)((uint32_t)row / (uint32_t)a.gate_group) * a.gate_pitch, col);
+    if constexpr (H) {
+      h.load(a.h, row * a.h_pitch, col);
+      gate.load(gate_base, (int64_t)((uint32_t)row / gate_group) * gate_pitch, col);
+    }
   };
   const int64_t step = (int64_t)gridDim.x * Row::kRows;
   const float kept = a.alpha * a.key.scale;
   int64_t row = (int64_t)blockIdx.x * Row::kRows + Row::slot();
-  load(row);
-  advoc::stage_vector<WG>(vec, a.scale, 1.f, cols);
-  advoc::stage_vector<WG>(vec + cols, a.w_post, 1.f, cols);
-  advoc::stage_vector<WG>(vec + 2 * cols, a.b_post, 0.f, cols);
-  advoc::stage_vector<WG>(vec + 3 * cols, a.w_pre, 1.f, cols);
-  if constexpr (kFive) advoc::stage_vector<WG>(vec + 4 * cols, a.b_pre, 0.f, cols);
+  if constexpr (kAhead) load(row);
+  if constexpr (kFive)
+    advoc::stage_vectors<WG, V, 5>(vec, {a.scale, a.w_post, a.b_post, a.w_pre, a.b_pre}, {1.f, 1.f, 0.f, 1.f, 0.f}, cols);
+  else
+    advoc::stage_vectors<WG, V, 4>(vec, {a.scale, a.w_post, a.b_post, a.w_pre}, {1.f, 1.f, 0.f, 1.f}, cols);
   Row::meet();
   for (; row < a.rows; row += step) {
     advoc::forget_lds();
+    if constexpr (!kAhead) load(row);
     f32x8 r[NV], u[NV], g[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       r[j] = x[j];
-      u[j] = h[j];
-      g[j] = gate[j];
+      if constexpr (H) {
+        u[j] = h[j];
+        g[j] = gate[j];
+      }
     }
     if constexpr (L > 64) Row::meet();          // outputs may be the inputs' own buffers, and a column may have two holders
-    load(row + step);
+    if constexpr (kAhead) load(row + step);
     float mean0 = 0.f, rstd0 = 0.f, mean1 = 0.f, rstd1 = 0.f;
-    if (a.h) {
-      if (a.post != ADVOC_NORM_NONE) row_stats<V, L, NV, WG>(u, dup, ragged, a.post, a.inv_cols, a.eps, red, turn, mean0, rstd0);
+    if constexpr (H) {
+      if (post) row_stats<V, L, NV, WG>(u, dup, ragged, a.post, a.inv_cols, a.eps, red, turn, mean0, rstd0);
+      const float by = post ? rstd0 : 1.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (a.post != ADVOC_NORM_NONE)
-          u[j] = (u[j] - mean0) * rstd0 * advoc::cols_chunk<V>(vec + cols + col[j]) + advoc::cols_chunk<V>(vec + 2 * cols + col[j]);
+        u[j] = (u[j] - mean0) * by * chunks.get(vec + floats, chunk[j]) + chunks.get(vec + 2 * floats, chunk[j]);
         uint32_t words[8];
         advoc::draw_chunk<V>(words, a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
-        f32x8 s = advoc::cols_chunk<V>(vec + col[j]) * kept;
-        if (a.gate) {
-          advoc::activate<V>(g[j], a.act);
-          s *= g[j];
-        }
+        f32x8 s = chunks.get(vec, chunk[j]) * kept;
+        advoc::activate<V>(g[j], a.act);
 #pragma unroll
-        for (int k = 0; k < V; ++k) r[j][k] += s[k] * (words[k] >= a.key.thresh ? u[j][k] : 0.f);
+        for (int k = 0; k < V; ++k) {
+          s[k] *= has_gate ? g[j][k] : 1.f;
+          r[j][k] += s[k] * (words[k] >= a.key.thresh ? u[j][k] : 0.f);
+        }
         advoc::store_chunk<V>(advoc::row_at<R>(a.r, row * a.r_pitch, col[j]), r[j]);
       }
     }
-    if (a.pre != ADVOC_NORM_NONE) {
+    if constexpr (PRE) {
       row_stats<V, L, NV, WG>(r, dup, ragged, a.pre, a.inv_cols, a.eps, red, turn, mean1, rstd1);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        f32x8 z = (r[j] - mean1) * rstd1 * advoc::cols_chunk<V>(vec + 3 * cols + col[j]);
-        if constexpr (kFive) z += advoc::cols_chunk<V>(vec + 4 * cols + col[j]);
-        else if (a.b_pre) z += advoc::cols_chunk<V>(a.b_pre + col[j]);
+        f32x8 z = (r[j] - mean1) * rstd1 * chunks.get(vec + 3 * floats, chunk[j]);
+        if constexpr (kFive) z += chunks.get(vec + 4 * floats, chunk[j]);
+        else if (a.b_pre) z += advoc::floats_at<V>(a.b_pre + col[j]);
         advoc::store_chunk<V>(advoc::row_at<T>(a.z, row * a.z_pitch, col[j]), z);
       }
     }
@@ -122,8 +135,11 @@ struct Launch {
     int64_t blocks = advoc::ceil_div(a.rows, Team<L, WG>::kRows);
     const int64_t most = 256 * (1024 / WG);      // the workgroups that are resident together, then rows in turn
     if (blocks > most) blocks = most;
-    hipLaunchKernelGGL((norm_forward_kernel<T, R, V, L, NV, WG>), dim3((unsigned)blocks), dim3(WG),
-                       (kFiveVectors<V, L, NV> ? 20 : 16) * a.cols, stream, a);
+    const dim3 grid((unsigned)blocks), block(WG);
+    const unsigned lds = (kFiveVectors<V, L, NV> ? 20u : 16u) * advoc::Chunks<V>(a.cols).floats();
+    if (!a.h) hipLaunchKernelGGL((norm_forward_kernel<T, R, V, L, NV, WG, false, true>), grid, block, lds, stream, a);
+    else if (a.pre == ADVOC_NORM_NONE) hipLaunchKernelGGL((norm_forward_kernel<T, R, V, L, NV, WG, true, false>), grid, block, lds, stream, a);
+    else hipLaunchKernelGGL((norm_forward_kernel<T, R, V, L, NV, WG, true, true>), grid, block, lds, stream, a);
   }
 };
 
