@@ -145,7 +145,7 @@ class ResidualNorm(object):
       raise _lib.AdvocHipError('cols must be 1 ... {}, got {}'.format(MAX_COLS, cols))
     if not eps > 0 or not 0 < keep_prob <= 1:
       raise _lib.AdvocHipError('eps must be positive and keep_prob in (0, 1]')
-    self.cols = cols
+    self.cols, self._shape = cols, torch.Size((cols,))
     self.post, self.pre = _choice(NORMS, post, 'norm'), _choice(NORMS, pre, 'norm')
     self.gate_act = _choice(GATE_ACTS, gate_act, 'gate activation')
     self.alpha, self.eps, self.keep_prob = alpha, eps, keep_prob
@@ -156,8 +156,8 @@ class ResidualNorm(object):
   def _vector(self, t, name, index):
     if t is None:
       return None
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != index or t.dtype != torch.float32 or (
-        t.dim() != 1 or t.shape[0] != self.cols or not t.is_contiguous()):
+    if not isinstance(t, torch.Tensor) or t.get_device() != index or t.dtype != torch.float32 or t.shape != self._shape or (
+        not t.is_contiguous()):
       raise _lib.AdvocHipError('{} must be a contiguous float32 tensor of {} on device {}'.format(name, self.cols, index))
     return t.data_ptr()
 
@@ -277,23 +277,26 @@ class ResidualNorm(object):
     if gate is not None:
       g['dgate'] = torch.empty_like(gate, memory_format=torch.contiguous_format)
       d.dgate.p, d.dgate.pitch = g['dgate'].data_ptr(), self.cols
-    into = into or {}
-    for name in ('w_post', 'b_post', 'scale', 'w_pre', 'b_pre'):
-      if getattr(self, name) is None or h is None and name in ('w_post', 'b_post', 'scale'):
-        if 'd' + name in into:
-          raise _lib.AdvocHipError('d{} has nothing to be the gradient of'.format(name))
-        continue
-      t = into.get('d' + name)
-      if t is None:
-        if accumulate:
-          raise _lib.AdvocHipError('accumulate needs a buffer for d{}'.format(name))
-        t = torch.empty(self.cols, dtype=torch.float32, device=r.device)
-      g['d' + name] = t
-      setattr(d, 'd' + name, self._vector(t, 'd' + name, index))
+    wanted = [('dw_pre', self.w_pre), ('db_pre', self.b_pre)]
+    if h is not None:
+      wanted += [('dw_post', self.w_post), ('db_post', self.b_post), ('dscale', self.scale)]
+    wanted = [name for name, p in wanted if p is not None]
     if into:
-      unknown = set(into) - {'dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre'}
+      unknown = set(into) - set(wanted)
       if unknown:
-        raise _lib.AdvocHipError('no such parameter gradients: {}'.format(sorted(unknown)))
+        raise _lib.AdvocHipError('no such parameter gradients here: {}'.format(sorted(unknown)))
+    new = [name for name in wanted if not into or into.get(name) is None]
+    if new:
+      if accumulate:
+        raise _lib.AdvocHipError('accumulate needs a buffer for {}'.format(new))
+      for name, t in zip(new, torch.empty(len(new), self.cols, dtype=torch.float32, device=r.device)):
+        g[name] = t
+        setattr(d, name, t.data_ptr())
+    if into:
+      for name in wanted:
+        if g[name] is None:
+          g[name] = into[name]
+          setattr(d, name, self._vector(into[name], name, index))
     d.accumulate = int(bool(accumulate))
     lib = _lib.load()
     nbytes = lib.advoc_residual_norm_workspace_bytes(ctypes.byref(d))

@@ -8,8 +8,8 @@
 
 namespace advoc {
 
-// Both halves of a 32 x 32-bit product in one instruction; the compiler issues two, each at a quarter of the vector rate, and they
-// are what the generator's time goes to.
+// Both halves of a 32 x 32-bit product in one instruction where the compiler issues two (with the first round's product that is
+// known to be zero left out and the words compared directly, 65536 x 1024 bf16 elements: 60 -> 54 us).
 __device__ __forceinline__ void mul64(uint64_t& p, uint32_t a, uint32_t b) {
   uint64_t carry;
   asm("v_mad_u64_u32 %0, %1, %2, %3, 0" : "=v"(p), "=s"(carry) : "s"(a), "v"(b));
@@ -70,10 +70,12 @@ __device__ __forceinline__ void drop_words8(uint32_t (&words)[8], uint64_t i, bo
     const uint4 c = philox4x32(q + 2, key);
     const uint32_t w[11] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z};
     uint32_t v[10];
+    // by masks: a choice between neighbours of an array becomes a load at a chosen address, from memory of the lane's own
+    const uint32_t one = 0u - (uint32_t)(i & 1), two = 0u - (uint32_t)(i >> 1 & 1);
 #pragma unroll
-    for (int k = 0; k < 10; ++k) v[k] = (i & 1) ? w[k + 1] : w[k];
+    for (int k = 0; k < 10; ++k) v[k] = (w[k + 1] & one) | (w[k] & ~one);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) words[k] = (i & 2) ? v[k + 2] : v[k];
+    for (int k = 0; k < 8; ++k) words[k] = (v[k + 2] & two) | (v[k] & ~two);
   }
 }
 

@@ -285,6 +285,25 @@ def test_norm_of_zeros_constants_and_bad_rows(blocks):
   assert bool((z == 0).all())
 
 
+def test_norm_sigmoid_of_extreme_gates(blocks):
+  """Shut at minus infinity, open at infinity, a NaN passed on; in between within 6 units in the last place."""
+  norm = blocks.ResidualNorm(512, post='none', pre='none', gate_act='sigmoid', scale=torch.ones(512, device='cuda'))
+  inf = float('inf')
+  edge = torch.tensor([-inf, inf, -1e30, 1e30, -89.0, 89.0, 0.0, -0.0], device='cuda')
+  gate = torch.cat([edge, torch.linspace(-87, 87, 504, device='cuda')]).reshape(1, 512)
+  h, x = torch.ones(1, 512, device='cuda'), torch.zeros(1, 512, device='cuda')
+  r = norm.forward(h, x, gate=gate)[0].cpu().double().flatten()
+  assert r[:8].tolist() == [0, 1, 0, 1, 0, 1, 0.5, 0.5]
+  want = torch.sigmoid(gate.cpu().double().flatten())[8:]
+  assert bool(((r[8:] - want).abs() <= 12 * U * want).all())
+  gate[0, 100] = float('nan')
+  r = norm.forward(h, x, gate=gate)[0]
+  assert bool(torch.isnan(r[0, 100])) and int(torch.isnan(r).sum()) == 1
+  st = torch.zeros(1, 4, device='cuda')
+  g = norm.backward(None, torch.ones_like(x), h, r, st, gate=gate)
+  assert bool((g.dgate[0, :6] == 0).all()) and bool((g.dgate[0, 6:8] == 0.25).all()) and int(torch.isnan(g.dgate).sum()) == 1
+
+
 def test_norm_empty(blocks):
   norm = blocks.ResidualNorm(16, w_pre=torch.ones(16, device='cuda'))
   e = torch.zeros(0, 16, device='cuda')
