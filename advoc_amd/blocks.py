@@ -18,6 +18,7 @@ stream of the tensors' device and can be captured into a graph.
 """
 import collections
 import ctypes
+import functools
 
 import torch
 
@@ -364,6 +365,11 @@ def quantize_f8_both(x, fmt='e4m3'):
   return _quantize(x, fmt, True, True)
 
 
+@functools.lru_cache(maxsize=4096)
+def _product_workspace(m, n, k, code):
+  return _lib.load().advoc_matmul_nt_f8_workspace_bytes(m, n, k, code)
+
+
 def matmul_nt_f8(a, b, out_dtype=torch.float32, out=None, accumulate=False):
   """a b^T of two F8Matrix operands with the same k -> [a.rows, b.rows] (``advoc_matmul_nt_f8``); a float32 result is
   accumulated in fp32 throughout.  accumulate: add to `out` (float32), e.g. a gradient arena's slice."""
@@ -378,7 +384,7 @@ def matmul_nt_f8(a, b, out_dtype=torch.float32, out=None, accumulate=False):
     raise _lib.AdvocHipError('out must be a contiguous [{}, {}] tensor on {}'.format(m, n, device))
   code = _dtype(out, 'out')
   lib = _lib.load()
-  nbytes = lib.advoc_matmul_nt_f8_workspace_bytes(m, n, a.k, code) if m > 64 else 0
+  nbytes = _product_workspace(m, n, a.k, code)
   work = torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
   _call(lib.advoc_matmul_nt_f8, 'advoc_matmul_nt_f8', device.index, a.data_ptr, a.scale_ptr, a.format, b.data_ptr, b.scale_ptr,
         b.format, out.data_ptr(), code, int(bool(accumulate)), m, n, a.k,

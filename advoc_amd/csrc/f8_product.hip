@@ -95,53 +95,39 @@ __device__ __forceinline__ void store_part(const Args& g, int64_t row, int64_t c
     if (col + k < g.n) p[k] = (O)((g.accumulate ? (float)p[k] : 0.f) + v[k]);
 }
 
-// ---- few rows (m <= 64): the weights are read once, by whoever multiplies them ----
-// A workgroup is 16 rows of b; its waves take the blocks of the contraction in turn, straight from memory to registers (a lane's 32
-// bytes; 16 lanes x 4 groups cover 16 lines), and meet in LDS in wave order.
-template <typename O, bool EXACT, int FA, int FB, int MF>
+// ---- few rows (m <= 16): the weights are read once, by whoever multiplies them ----
+// A workgroup is 16 rows of b; its waves take the blocks of the contraction in turn, straight from memory to registers (lane
+// group g the 16-byte pieces g and g + 4 of 16 rows, so that a load covers half lines whole), and meet in LDS in wave order.
+template <typename O, bool EXACT, int FA, int FB>
 __global__ __launch_bounds__(1024) void f8_thin_kernel(Args g) {
   extern __shared__ f32x4 red[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
-  const int64_t nrow = n0 + (lane & 15) < g.n ? n0 + (lane & 15) : g.n - 1;
-  const uint8_t* bp = g.b + nrow * g.kp + (lane >> 4) * 32;
-  const uint8_t* bs = g.b_scale + nrow * g.sp;
-  const uint8_t *ap[MF], *as[MF];
-#pragma unroll
-  for (int i = 0; i < MF; ++i) {
-    const int64_t r = i * 16 + (lane & 15) < g.m ? i * 16 + (lane & 15) : g.m - 1;
-    ap[i] = g.a + r * g.kp + (lane >> 4) * 32;
-    as[i] = g.a_scale + r * g.sp;
-  }
-  f32x4 acc[MF];
-#pragma unroll
-  for (int i = 0; i < MF; ++i) acc[i] = (f32x4)(0.f);
+  const int64_t nrow = n0 + (lane & 15) < g.n ? n0 + (lane & 15) : g.n - 1, mrow = (lane & 15) < g.m ? (lane & 15) : g.m - 1;
+  const uint8_t *bp = g.b + nrow * g.kp + (lane >> 4) * 16, *ap = g.a + mrow * g.kp + (lane >> 4) * 16;
+  const uint8_t *bs = g.b_scale + nrow * g.sp, *as = g.a_scale + mrow * g.sp;
+  f32x4 acc = (f32x4)(0.f);
 #pragma unroll 2
   for (int kb = wave; kb < g.blocks; kb += waves) {
-    const int4* p = reinterpret_cast<const int4*>(bp + (int64_t)kb * kBlock);
-    const Frag<FB, EXACT> b(join(p[0], p[1]), bs[kb]);
-#pragma unroll
-    for (int i = 0; i < MF; ++i) {
-      const int4* q = reinterpret_cast<const int4*>(ap[i] + (int64_t)kb * kBlock);
-      acc[i] = mfma<FA, FB>(b, Frag<FA, EXACT>(join(q[0], q[1]), as[i][kb]), acc[i]);
-    }
+    const int4 *p = reinterpret_cast<const int4*>(bp + (int64_t)kb * kBlock), *q = reinterpret_cast<const int4*>(ap + (int64_t)kb * kBlock);
+    acc = mfma<FA, FB>(Frag<FB, EXACT>(join(p[0], p[4]), bs[kb]), Frag<FA, EXACT>(join(q[0], q[4]), as[kb]), acc);
   }
-#pragma unroll
-  for (int i = 0; i < MF; ++i) red[(wave * MF + i) * 64 + lane] = acc[i];
+  red[wave * 64 + lane] = acc;
   __syncthreads();
-  for (int e = threadIdx.x; e < MF * 64; e += blockDim.x) {
-    f32x4 v = red[e];
-    for (int w = 1; w < waves; ++w) v += red[w * MF * 64 + e];
-    const int l = e & 63;
+  if (wave == 0) {
+    f32x4 v = red[lane];
+    for (int w = 1; w < waves; ++w) v += red[w * 64 + lane];
     float o[4] = {v[0], v[1], v[2], v[3]};
-    store_part<O, 4>(g, (e >> 6) * 16 + (l & 15), n0 + (l >> 4) * 4, o);
+    store_part<O, 4>(g, lane & 15, n0 + (lane >> 4) * 4, o);
   }
 }
 
 // ---- tiles ----
-// BM x BN outputs per workgroup, WM x WN per wave.  A block of the contraction of both operands, with the dword that holds its
-// exponent byte for every row, is one of S stages in LDS, fetched by LDS-DMA while those before are multiplied.  (Loads that the compiler counts must not follow a DMA in the loop: memory counters retire in order, and waiting for
-// such a load waits for the next stage too.  That alone held the first form of this kernel at 0.8 PFLOP/s.)
+// BM x BN outputs per workgroup, WM x WN per wave.  A block of the contraction of both operands is one of S stages in LDS, fetched by
+// LDS-DMA while those before are multiplied.  (Loads that the compiler counts must not follow a DMA in the loop: memory counters
+// retire in order, and waiting for such a load waits for the next stage too.  That alone held the first form of this kernel at 0.8
+// PFLOP/s.)  The exponents of four blocks are a dword of every row, fetched with the first of them, into one of two places: a row's
+// dword is a cache line of its own in a long contraction, as much to ask for as the row's 128 bytes.
 // A row's eight 16-byte pieces lie at piece ^ key(row), and lane group g reads pieces g and g + 4: measured without bank conflicts, 4
 // cycles for a wave's 16 bytes a lane.  (Pieces 2 g and 2 g + 1 take 8.)
 template <typename O, int BM, int BN, int WM, int WN, int S>
@@ -149,9 +135,8 @@ struct Tile {
   static constexpr int kWaves = BM / WM * (BN / WN), kFm = WM / 16, kFn = WN / 16;
   static constexpr int kRun = sizeof(O) == 4 ? 1 : 2;            // fragments of b that give a lane 16 consecutive bytes of output
   static constexpr int kRows = BM + BN, kStage = kRows * kBlock, kExp = kRows * 4;
-  static constexpr int kLds = S * (kStage + kExp);
+  static constexpr int kLds = S * kStage + 2 * kExp;
   static constexpr int kDma = kRows / 8 / kWaves;                // a DMA instruction fetches 8 rows, or the exponents of 64
-  static constexpr int kInFlight = kDma + 1;                     // DMA instructions of a wave per stage
   static_assert(kFn % kRun == 0, "whole runs");
   static_assert(kDma * 8 * kWaves == kRows && BM % (8 * kWaves) == 0, "whole DMA instructions per wave and operand");
   static_assert(8 * kWaves % 32 == 0, "the keys of the rows that a lane fetches repeat");
@@ -196,17 +181,18 @@ struct Tile {
     piece1 = piece0 ^ 64;
   }
 
-  // block kb of the contraction into stage `slot`
-  __device__ __forceinline__ void fetch(int kb, int slot) const {
+  // block kb of the contraction, which is part of one that starts at kb0, into stage `slot`
+  __device__ __forceinline__ void fetch(int kb, int kb0, int slot) const {
 #pragma unroll
     for (int t = 0; t < kDma; ++t) {
       const unsigned to = base + slot * kStage + (t * kWaves + wave) * 1024;
       if (t * 8 * kWaves < BM) advoc::dma16(ra, to, voff_a + t * 8 * kWaves * kp, kb * kBlock);
       else advoc::dma16(rb, to, voff_b + (t * 8 * kWaves - BM) * kp, kb * kBlock);
     }
+    if ((kb & 3) && kb != kb0) return;
     const int first = wave % (kRows / 64) * 64;                  // (waves beyond the rows fetch the same dwords again)
     const bool is_a = first < BM;
-    advoc::dma4(is_a ? rea : reb, base + S * kStage + slot * kExp + first * 4, (first + lane - (is_a ? 0 : BM)) * spitch, kb & ~3);
+    advoc::dma4(is_a ? rea : reb, base + S * kStage + (kb >> 2 & 1) * kExp + first * 4, (first + lane - (is_a ? 0 : BM)) * spitch, kb & ~3);
   }
 
   __device__ __forceinline__ i32x8 bytes(int row) const {      // slot * kRows + row of the stage
@@ -215,12 +201,12 @@ struct Tile {
   }
   __device__ __forceinline__ i32x8 bytes_a(int slot, int i) const { return bytes(slot * kRows + off_a + i * 16); }
   __device__ __forceinline__ i32x8 bytes_b(int slot, int j) const { return bytes(slot * kRows + off_b + place_b(j, 0)); }
-  __device__ __forceinline__ int exponent_a(int slot, int kb, int i) const { return exponent(slot * kRows + off_a + i * 16, kb); }
-  __device__ __forceinline__ int exponent_b(int slot, int kb, int j) const { return exponent(slot * kRows + off_b + place_b(j, 0), kb); }
-  __device__ __forceinline__ int exponent(int row, int kb) const { return lds[S * kStage + row * 4 + (kb & 3)]; }
+  __device__ __forceinline__ int exponent_a(int kb, int i) const { return exponent(off_a + i * 16, kb); }
+  __device__ __forceinline__ int exponent_b(int kb, int j) const { return exponent(off_b + place_b(j, 0), kb); }
+  __device__ __forceinline__ int exponent(int row, int kb) const { return lds[S * kStage + (kb >> 2 & 1) * kExp + row * 4 + (kb & 3)]; }
 
   // Four lane groups store 64 consecutive bytes of a row together.  Tiles inside the matrix have a loop of their own: next to the
-  // element-wise form the compiler cut their 16-byte stores in two (34 -> 46 us for a 16 MB output).
+  // element-wise form the compiler cut their 16-byte stores in two (with that, 16384 x 1024 x 1024 took 28 us instead of 22).
   __device__ __forceinline__ void store(const Args& g, int64_t m0, int64_t n0, const f32x4 (&acc)[kFm][kFn]) const {
     constexpr int C = 4 * kRun;
     typedef O run __attribute__((ext_vector_type(C)));
@@ -291,21 +277,22 @@ __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void f8_tile_kernel(Args 
   int ea[T::kFm], eb[T::kFn];
   auto read = [&](int slot, int kb) {
 #pragma unroll
-    for (int j = 0; j < T::kFn; ++j) qb[j] = t.bytes_b(slot, j), eb[j] = t.exponent_b(slot, kb, j);
+    for (int j = 0; j < T::kFn; ++j) qb[j] = t.bytes_b(slot, j), eb[j] = t.exponent_b(kb, j);
 #pragma unroll
-    for (int i = 0; i < T::kFm; ++i) qa[i] = t.bytes_a(slot, i), ea[i] = t.exponent_a(slot, kb, i);
+    for (int i = 0; i < T::kFm; ++i) qa[i] = t.bytes_a(slot, i), ea[i] = t.exponent_a(kb, i);
   };
-  for (int kb = kb0; kb < kb0 + S && kb < kb1; ++kb) t.fetch(kb, kb - kb0);
-  if (kb0 + S - 1 < kb1) advoc::dma_ring_barrier<(S - 1) * T::kInFlight>();
+  for (int kb = kb0; kb < kb0 + S && kb < kb1; ++kb) t.fetch(kb, kb0, kb - kb0);
+  if (kb0 + S - 1 < kb1) advoc::dma_ring_barrier<(S - 1) * T::kDma>();
   else advoc::dma_ring_barrier<0>();
   read(0, kb0);
   int slot = 0;
 #pragma unroll 2
   for (int kb = kb0; kb < kb1; ++kb) {
-    // everyone holds block kb, block kb + 1 has landed; S - 2 younger stages may be in flight, the last ones are waited for
-    if (kb + S - 1 < kb1) advoc::dma_ring_barrier<(S - 2) * T::kInFlight>();
+    // everyone holds block kb, block kb + 1 has landed; S - 2 younger stages may be in flight (but for a fetch of exponents, which is
+    // not counted), the last ones are waited for
+    if (kb + S - 1 < kb1) advoc::dma_ring_barrier<(S - 2) * T::kDma>();
     else advoc::dma_ring_barrier<0>();
-    if (kb + S < kb1) t.fetch(kb + S, slot);
+    if (kb + S < kb1) t.fetch(kb + S, kb0, slot);
     slot = slot == S - 1 ? 0 : slot + 1;
     auto multiply = [&](const auto&... b) {
       const Frag<FA, EXACT> fa[] = {{qa[0], ea[0]}, {qa[1], ea[1]}, {qa[T::kFm - 2], ea[T::kFm - 2]}, {qa[T::kFm - 1], ea[T::kFm - 1]}};
@@ -378,10 +365,10 @@ __global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
     for (int i = 0; i < T::kFm; ++i) a[i] = t.bytes_a(slot, i);
 #pragma unroll
     for (int i = 0; i < T::kFm; i += 4)
-      ea[i / 4] = t.exponent_a(slot, kb, i) | t.exponent_a(slot, kb, i + 1) << 8 | t.exponent_a(slot, kb, i + 2) << 16 | t.exponent_a(slot, kb, i + 3) << 24;
+      ea[i / 4] = t.exponent_a(kb, i) | t.exponent_a(kb, i + 1) << 8 | t.exponent_a(kb, i + 2) << 16 | t.exponent_a(kb, i + 3) << 24;
 #pragma unroll
     for (int j = 0; j < T::kFn; j += 4)
-      eb[j / 4] = t.exponent_b(slot, kb, j) | t.exponent_b(slot, kb, j + 1) << 8 | t.exponent_b(slot, kb, j + 2) << 16 | t.exponent_b(slot, kb, j + 3) << 24;
+      eb[j / 4] = t.exponent_b(kb, j) | t.exponent_b(kb, j + 1) << 8 | t.exponent_b(kb, j + 2) << 16 | t.exponent_b(kb, j + 3) << 24;
   };
   auto multiply = [&]() {
     __builtin_amdgcn_s_setprio(1);
@@ -390,7 +377,7 @@ __global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
   };
   auto fetch = [&](int kb) {
     if (kb >= g.blocks) return;
-    t.fetch(kb, kb & 1);
+    t.fetch(kb, 0, kb & 1);
   };
   auto meet = [&](bool landed) {      // my reads have arrived and, with `landed`, what I fetched lies in LDS
     __builtin_amdgcn_sched_barrier(0);
@@ -443,17 +430,29 @@ struct Plan {
   int form, splits, per_split;
 };
 
+// The cheapest estimate.  A CU takes 0.75 us for a block of 128 x 128 outputs (1.2 EXACT), 0.4 (0.35) times that for one of
+// 64 x 64 and twice for one of 256 x 256, whichever its neighbours do; the CUs take tiles in rounds of 256.  A contraction split in s
+// has s times the tiles with 1 / s of the blocks, and 3 us and a write and a read of its partial results more.
+// The thin kernel takes 0.08 us and 4.2 ns a row for a block of 16 columns, 256 of them together.
+// Measured, in us (64 | 128 | 256, 16-bit outputs):  1024 x 1024 x 1024: 5.5 | 8.1;  2048 x 1024 x 4096: 19 | 25 | 48;  2048 x 2048 x
+// 4096: 33 | 24 | 48;  4096 x 2048 x 4096: 63 | 47 | 50;  4096 x 2560 x 4096: 128: 68, 256: 52;  16384 x 1024 x 1024: 39 | 31 | 21.
+// fp32 outputs in 1 | 2 | 4 | 8 parts:  1024 x 1024 x 16384: 112 | 65 | 43 | 50 (128), 57 | 47 | 49 (64);  512 x 512 x 2048: 9.1 |
+// 9.1 | 8.6 | 11.6 (64).
+// Thin | 64 in parts:  1 x 512 x 8192: 8.4 | 8.4;  16 x 512 x 8192: 12.7 | 9.3;  16 x 4096 x 4096: 8.0 | 9.3;  16 x 1000 x 1000: 3.7 |
+// 5.2;  with 17 to 64 rows the thin form lost nearly everywhere (64 x 512 x 8192: 28.8 | 9.8).
 Plan make_plan(int64_t m, int64_t n, int blocks, bool exact) {
   Plan p = {kThin, 1, blocks};
-  if (m <= 64) return p;
-  const int64_t t256 = ceil_div(m, 256) * ceil_div(n, 256), t128 = ceil_div(m, 128) * ceil_div(n, 128);
-  p.form = t256 >= 192 && !exact ? kTile256 : t128 >= 64 ? kTile128 : kTile64;
-  const int64_t tiles = p.form == kTile256 ? t256 : p.form == kTile128 ? t128 : ceil_div(m, 64) * ceil_div(n, 64);
-  int64_t splits = (p.form == kTile64 ? 512 : 256) / tiles;
-  if (splits > blocks / 8) splits = blocks / 8;
-  if (splits > 1 && p.form != kTile256) {
-    p.per_split = (int)ceil_div(blocks, splits);
-    p.splits = (int)ceil_div(blocks, p.per_split);
+  const double block_us = exact ? 1.2 : 0.75, fold_us = 8.0 * m * n / 5e6;
+  double best = m <= 16 ? (0.08 + 0.0042 * m) * blocks * ceil_div(n, 16 * 256) : 1e30;
+  for (int form = kTile64; form <= (exact ? kTile128 : kTile256); ++form) {
+    const int64_t side = form == kTile64 ? 64 : form == kTile128 ? 128 : 256;
+    const int64_t tiles = ceil_div(m, side) * ceil_div(n, side);
+    const double cost = block_us * (form == kTile64 ? exact ? 0.35 : 0.4 : form == kTile128 ? 1.0 : 2.0);
+    for (int s = 1; s == 1 || (form != kTile256 && s <= 16 && s <= blocks / 8); s *= 2) {
+      const int per = (int)ceil_div(blocks, s), parts = (int)ceil_div(blocks, per);
+      const double us = cost * ceil_div(tiles * parts, 256) * per + (parts > 1 ? 3.0 + fold_us * parts : 0.0);
+      if (us < best) best = us, p = {form, parts, per};
+    }
   }
   return p;
 }
@@ -472,12 +471,7 @@ int run(const Args& g, const Plan& p, hipStream_t stream) {
   ADVOC_CLEAR_LAUNCH_ERROR();
   if (p.form == kThin) {
     const unsigned waves = g.blocks >= 16 ? 16 : g.blocks >= 8 ? 8 : g.blocks >= 4 ? 4 : 2;
-    const int mf = g.m <= 16 ? 1 : g.m <= 32 ? 2 : 4;
-    const dim3 grid((unsigned)ceil_div(g.n, 16)), block(64 * waves);
-    const unsigned lds = waves * mf * 1024;
-    if (mf == 1) hipLaunchKernelGGL((f8_thin_kernel<O, EXACT, FA, FB, 1>), grid, block, lds, stream, g);
-    else if (mf == 2) hipLaunchKernelGGL((f8_thin_kernel<O, EXACT, FA, FB, 2>), grid, block, lds, stream, g);
-    else hipLaunchKernelGGL((f8_thin_kernel<O, EXACT, FA, FB, 4>), grid, block, lds, stream, g);
+    hipLaunchKernelGGL((f8_thin_kernel<O, EXACT, FA, FB>), dim3((unsigned)ceil_div(g.n, 16)), dim3(64 * waves), waves * 1024, stream, g);
     ADVOC_RETURN_IF_LAUNCH_FAILED();
     return ADVOC_OK;
   }

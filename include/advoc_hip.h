@@ -649,8 +649,8 @@ int advoc_f8_quantize(const void* x, int64_t x_pitch, int64_t rows, int64_t cols
  * advoc_matmul_nt_f32.  ADVOC_F32 outputs are accumulated in fp32 throughout.  16-bit outputs take the 8-bit matrix instruction at
  * twice the rate: it adds up in fp32 but for products below 2^-13 of the largest of eight neighbours, which it drops (1.5e-5 of
  * the result in norm; their own rounding is 1.7e-3 or 2e-4).  out [m, n] dense; accumulate != 0 (out_dtype ADVOC_F32) adds to it.
- * workspace: advoc_matmul_nt_f8_workspace_bytes(m, n, k, out_dtype) bytes, 4-byte aligned (0, as for m <= 64: may be NULL); with too
- * little the product runs unsplit.  The order of every sum is fixed by the shapes: two calls give the same bits. */
+ * workspace: advoc_matmul_nt_f8_workspace_bytes(m, n, k, out_dtype) bytes, 4-byte aligned (0: may be NULL); with too little the
+ * product runs unsplit.  The order of every sum is fixed by the shapes: two calls give the same bits. */
 int64_t advoc_matmul_nt_f8_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t out_dtype);
 int advoc_matmul_nt_f8(const uint8_t* a, const uint8_t* a_scale, int32_t a_format, const uint8_t* b, const uint8_t* b_scale,
                        int32_t b_format, void* out, int32_t out_dtype, int32_t accumulate, int64_t m, int64_t n, int64_t k,
