@@ -129,6 +129,9 @@ ResidualNormGrads = collections.namedtuple('ResidualNormGrads',
                                            ['dh', 'dx', 'dgate', 'dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre'])
 
 
+_PARAMETER_GRADS = ResidualNormGrads._fields[3:]
+
+
 class ResidualNorm(object):
   """The glue between two residual blocks (``advoc_residual_norm_forward / _backward``), per row of `cols` channels:
 
@@ -269,47 +272,52 @@ class ResidualNorm(object):
           stats.dtype != torch.float32 or stats.shape != (rows, 4) or not stats.is_contiguous()):
         raise _lib.AdvocHipError('stats must be the contiguous float32 [rows, 4] tensor of forward(..., save=True)')
       d.stats = stats.data_ptr()
-    g = dict.fromkeys(ResidualNormGrads._fields)
-    g['dx'] = torch.empty_like(r, memory_format=torch.contiguous_format)
-    d.dx.p, d.dx.pitch = g['dx'].data_ptr(), self.cols
+    contiguous = torch.contiguous_format
+    dx = torch.empty_like(r, memory_format=contiguous)
+    d.dx.p, d.dx.pitch = dx.data_ptr(), self.cols
+    dh = dgate = None
     if h is not None:
-      g['dh'] = torch.empty_like(r, dtype=h.dtype, memory_format=torch.contiguous_format)
-      d.dh.p, d.dh.pitch = g['dh'].data_ptr(), self.cols
+      dh = torch.empty_like(r, dtype=h.dtype, memory_format=contiguous)
+      d.dh.p, d.dh.pitch = dh.data_ptr(), self.cols
     if gate is not None:
-      g['dgate'] = torch.empty_like(gate, memory_format=torch.contiguous_format)
-      d.dgate.p, d.dgate.pitch = g['dgate'].data_ptr(), self.cols
-    wanted = [('dw_pre', self.w_pre), ('db_pre', self.b_pre)]
-    if h is not None:
-      wanted += [('dw_post', self.w_post), ('db_post', self.b_post), ('dscale', self.scale)]
-    wanted = [name for name, p in wanted if p is not None]
+      dgate = torch.empty_like(gate, memory_format=contiguous)
+      d.dgate.p, d.dgate.pitch = dgate.data_ptr(), self.cols
+    wanted = [] if h is None else [name for name, p in (('dw_post', self.w_post), ('db_post', self.b_post), ('dscale', self.scale))
+                                   if p is not None]
+    if self.w_pre is not None:
+      wanted.append('dw_pre')
+    if self.b_pre is not None:
+      wanted.append('db_pre')
+    g = dict.fromkeys(_PARAMETER_GRADS)
     if into:
       unknown = set(into) - set(wanted)
       if unknown:
         raise _lib.AdvocHipError('no such parameter gradients here: {}'.format(sorted(unknown)))
-    new = [name for name in wanted if not into or into.get(name) is None]
+      for name in wanted:
+        t = into.get(name)
+        if t is not None:
+          setattr(d, name, self._vector(t, name, index))
+          g[name] = t
+    new = [name for name in wanted if g[name] is None]
     if new:
       if accumulate:
         raise _lib.AdvocHipError('accumulate needs a buffer for {}'.format(new))
       for name, t in zip(new, torch.empty(len(new), self.cols, dtype=torch.float32, device=r.device)):
         g[name] = t
         setattr(d, name, t.data_ptr())
-    if into:
-      for name in wanted:
-        if g[name] is None:
-          g[name] = into[name]
-          setattr(d, name, self._vector(into[name], name, index))
     d.accumulate = int(bool(accumulate))
     lib = _lib.load()
-    nbytes = lib.advoc_residual_norm_workspace_bytes(ctypes.byref(d))
+    ref = ctypes.byref(d)
+    nbytes = lib.advoc_residual_norm_workspace_bytes(ref)
     if nbytes:
       work = torch.empty(nbytes // 4, dtype=torch.float32, device=r.device)
       d.workspace, d.workspace_bytes = work.data_ptr(), nbytes
     if rows == 0 and not accumulate:
-      for name in ('dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre'):
-        if g[name] is not None:
-          g[name].zero_()
-    _call(lib.advoc_residual_norm_backward, 'advoc_residual_norm_backward', index, ctypes.byref(d))
-    return ResidualNormGrads(**g)
+      for t in g.values():
+        if t is not None:
+          t.zero_()
+    _call(lib.advoc_residual_norm_backward, 'advoc_residual_norm_backward', index, ref)
+    return ResidualNormGrads(dh, dx, dgate, *g.values())
 
 
 class F8Matrix(object):

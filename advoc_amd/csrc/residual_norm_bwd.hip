@@ -26,16 +26,14 @@ struct Sums {
   int slot[kSums];              // place in NormArgs.part, -1: not wanted
 };
 
-// Lanes of a workgroup and waves per SIMD.  Rows of 16 columns a lane: 256 registers, a third of them sums, and 512 lanes to a
-// workgroup (half the partial column sums of 256); rows of 8: three waves to a SIMD (8192 x 2048: 90.5 us, two 92.4).  A row of
-// 4096 columns is 512 lanes of 8, one workgroup to a CU: 4096 rows take 88 us, with registers for three waves 115 (they spill),
-// 256 lanes of 16 97.
+// Two waves to a SIMD, 256 registers to a lane: rows of 16 columns a lane need them all, a third for the sums, and have 512 lanes to a
+// workgroup (half the partial column sums of 256); rows of 8 columns a lane use the rest to fetch a row ahead, which is worth more
+// than a third wave (16384 x 256: 24 -> 20 us, 8192 x 2048: 80 -> 74, 4096 x 4096 fp16: 60 -> 51).
+constexpr int kWavesPerSimd = 2;
 template <int L, int NV>
 constexpr int kLanes = L > 64 ? L : NV > 1 ? 512 : 256;
-template <int L, int NV>
-constexpr int kWavesPerSimd = NV > 1 || L > 256 ? 2 : 3;
 
-// Column sums that go through LDS together at the end of a workgroup: 40 KB with three workgroups to a CU, 128 KB with one.
+// Column sums that go through LDS together at the end of a workgroup: 40 KB with two workgroups to a CU, 128 KB with one.
 template <int NV>
 constexpr int kSumsTogether = NV > 1 ? 4 : 5;
 
@@ -56,8 +54,11 @@ __device__ __forceinline__ void norm_back(f32x8 (&t)[NV], const f32x8 (&hat)[NV]
 // absent is not a branch (register allocation around those cost more than the work they save): an absent dr or gate is read from
 // where r or h lies and replaced by its neutral value, absent vectors are staged as theirs.
 template <typename T, typename R, int V, int L, int NV, int WG, bool H, bool PRE>
-__global__ __launch_bounds__(WG, (kWavesPerSimd<L, NV>)) void norm_backward_kernel(NormArgs a, Sums sums) {
+__global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormArgs a, Sums sums) {
   using Row = Team<L, WG>;
+  // a row's loads go out as soon as those of the row before have been used, ahead of that one's second half (with 16 columns a lane
+  // that spills: 16384 x 1024 69 -> 116 us)
+  constexpr bool kAhead = NV == 1;
   __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
   extern __shared__ __align__(16) float vec[];                // w_pre, w_post, b_post, scale; afterwards the column sums of the workgroup's rows
   int turn = 0;
@@ -115,9 +116,10 @@ __global__ __launch_bounds__(WG, (kWavesPerSimd<L, NV>)) void norm_backward_kern
         raw_gate.load(gate_base, (shared_gate ? group : row) * gate_pitch, col);
       }
     };
+    if constexpr (kAhead) load(end - group_rows + first);
     for (int64_t row = end - group_rows + first; row < end; row += a.splits) {
       advoc::forget_lds();
-      load(row);
+      if constexpr (!kAhead) load(row);
       f32x8 hat[NV], t[NV], g[NV], gate[NV];
       const float4 st = PRE || post ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -147,6 +149,7 @@ __global__ __launch_bounds__(WG, (kWavesPerSimd<L, NV>)) void norm_backward_kern
         }
       }
       if constexpr (L > 64) Row::meet();        // outputs may be the inputs' own buffers, and a column may have two holders
+      if constexpr (kAhead) load(row + a.splits < end ? row + a.splits : row);
       if (a.dx)
 #pragma unroll
         for (int j = 0; j < NV; ++j) advoc::store_chunk<V>(advoc::row_at<R>(a.dx, row * a.dx_pitch, col[j]), g[j]);
@@ -315,7 +318,7 @@ struct MakePlan {
   template <int V, int L, int NV>
   void run() const {
     constexpr int kRows = Team<L, kLanes<L, NV>>::kRows;
-    const int64_t most = 256 * 4 * 64 * kWavesPerSimd<L, NV> / kLanes<L, NV>;      // what is resident together
+    const int64_t most = 256 * 4 * 64 * kWavesPerSimd / kLanes<L, NV>;      // what is resident together
     const bool shared_gate = a.gate && a.gate_group > 1;
     const int64_t rows = shared_gate ? a.gate_group : a.rows, groups = a.rows / rows;
     int64_t splits = most * kRows / groups;
