@@ -22,6 +22,7 @@ __device__ __forceinline__ uint32_t largest_finite(F&& get) {
   for (int i = 0; i < N; ++i) m = larger(m, magnitude(get(i)));
   if (m >= kInfinity) {
     m = 0;
+#pragma unroll
     for (int i = 0; i < N; ++i) {
       const uint32_t b = magnitude(get(i));
       if (b < kInfinity) m = larger(m, b);

@@ -153,6 +153,19 @@ struct Raw {
     for (int k = 0; k < 8; ++k) f[k] = k < V ? (float)v[j][k] : 0.f;
     return f;
   }
+  // The loads have returned behind this.  (A wave may use what it has loaded behind a rendezvous; without this the wait for it would
+  // lie there too, and another wave could store to the place first.)
+  __device__ __forceinline__ void arrived() {
+    constexpr int kWords = (V * sizeof(T) + 3) / 4;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      int w[sizeof(v[j]) / 4];
+      __builtin_memcpy(w, &v[j], sizeof(w));
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+      __builtin_memcpy(&v[j], w, sizeof(w));
+    }
+  }
 };
 template <int V, typename T>
 __device__ __forceinline__ void store_chunk(T* p, const f32x8& v) {

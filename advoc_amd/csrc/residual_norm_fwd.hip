@@ -37,12 +37,16 @@ constexpr bool kFiveVectors = V * L * NV <= 4096;
 
 // H: there is a block output; PRE: there is a pre norm.  Nothing else that may be absent is a branch around memory: an absent gate is
 // read from where h lies and replaced by ones.
-// The next row's loads are in flight while a row is computed.  A wave waits for its loads and stores in the order of their issue, so
-// that holds only while the number of stores behind the loads is known where the loads are waited for.
+// Four waves to a SIMD, 128 registers to a lane.  With 8 columns a lane the next row's loads are in flight while a row is computed
+// (8192 x 2048: 50 us, without 55; 4096 x 4096: 50, without 62); with 16 they would spill (16384 x 1024: 38 us, with them 65).  A wave waits for its loads and stores in the order of their issue, so that the number of stores behind the
+// loads is to be known where the loads are waited for: hence the templates.
+// 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (202 MB): 38 us, 5.3 TB/s, a copy's rate.  Rows of a whole
+// workgroup meet four times on their way: 4096 x 4096 50 us, 4.0 TB/s.  16384 x 513: 32 us, 3.1 TB/s, bound by arithmetic (a second
+// chunk for one column, rows at odd offsets, three Philox blocks for eight words).  One row: 6 us, latency.
 template <typename T, typename R, int V, int L, int NV, int WG, bool H, bool PRE>
 __global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
   using Row = Team<L, WG>;
-  extern __shared__ __align__(16) float vec[];                // scale, w_post, b_post, w_pre and, where five fit into LDS, b_pre
+  extern __shared__ __align__(16) float vec[];  // scale, w_post, b_post, w_pre and, where five fit into LDS, b_pre
   constexpr bool kAhead = NV == 1;
   constexpr bool kFive = kFiveVectors<V, L, NV>;
   __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
@@ -81,6 +85,11 @@ __global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
   for (; row < a.rows; row += step) {
     advoc::forget_lds();
     if constexpr (!kAhead) load(row);
+    if constexpr (L > 64) {                     // outputs may be the inputs' own buffers, and a column may have two holders
+      x.arrived();
+      if constexpr (H) h.arrived(), gate.arrived();
+      Row::meet();
+    }
     f32x8 r[NV], u[NV], g[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -90,7 +99,6 @@ __global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
         g[j] = gate[j];
       }
     }
-    if constexpr (L > 64) Row::meet();          // outputs may be the inputs' own buffers, and a column may have two holders
     if constexpr (kAhead) load(row + step);
     float mean0 = 0.f, rstd0 = 0.f, mean1 = 0.f, rstd1 = 0.f;
     if constexpr (H) {
@@ -133,7 +141,7 @@ struct Launch {
   void run() const {
     constexpr int WG = L > 64 ? L : 256;
     int64_t blocks = advoc::ceil_div(a.rows, Team<L, WG>::kRows);
-    const int64_t most = 256 * (1024 / WG);      // the workgroups that are resident together, then rows in turn
+    const int64_t most = 256 * (1024 / WG);      // the workgroups that are resident together (four waves to a SIMD), then rows in turn
     if (blocks > most) blocks = most;
     const dim3 grid((unsigned)blocks), block(WG);
     const unsigned lds = (kFiveVectors<V, L, NV> ? 20u : 16u) * advoc::Chunks<V>(a.cols).floats();

@@ -198,7 +198,7 @@ def test_norm_rows_and_clips(blocks, lead):
   check_norm(blocks, 1, lead, 72, 'f16', 'f32', *KINDS[1])
 
 
-@pytest.mark.parametrize('lead,cols', [((13000, 2), 16), ((2500, 2), 1000), ((900, 3), 1100), ((300, 2), 2500), ((130, 2), 4100)])
+@pytest.mark.parametrize('lead,cols', [((13000, 2), 16), ((2500, 2), 1000), ((900, 3), 1100), ((300, 2), 2500), ((300, 2), 4100)])
 def test_norm_more_clips_than_workers(blocks, lead, cols):
   """A worker that passes through several gate rows carries the sums of those before, at every width that holds rows its own way."""
   check_norm(blocks, 3, lead, cols, 'bf16', 'bf16', *KINDS[1])
@@ -245,6 +245,29 @@ def test_norm_backward_in_place(blocks, cols):
   assert _lib.load().advoc_residual_norm_workspace_bytes(ctypes.byref(q)) == 0
   _lib.check(_lib.load().advoc_residual_norm_backward(ctypes.byref(q), _lib.stream()))
   assert torch.equal(dr, g.dx) and torch.equal(h, g.dh)
+
+
+@pytest.mark.parametrize('lead,cols', [((600, 2), 1032), ((300, 3), 2056), ((9, 40), 1544), ((2200, 1), 700), ((3, 70), 80)])
+def test_norm_every_output_over_an_input(blocks, lead, cols):
+  """dx over dr, dh over h and dgate over a gate per clip: whole clips to a worker and clips cut up, waves that hold the same columns."""
+  import ctypes
+  from advoc_amd import _lib
+  norm, d, call, g, (r, z, stats) = check_norm(blocks, 8, lead, cols, 'f32', 'f32', 'rms', 'layer', 'clip', 'sigmoid', 0.9)
+  h, dr, gate = d['h'].clone(), d['dr'].clone(), d['gate'].clone()
+  q, rows, _ = norm._descriptor(r, 'r', torch.float32, gate, call['seed'], call['offset'], None, True)
+  for name, t in (('dz', d['dz']), ('dr', dr), ('dx', dr), ('h', h), ('dh', h), ('dgate', gate)):
+    getattr(q, name).p, getattr(q, name).pitch = t.data_ptr(), cols
+  sums = {k: torch.full((cols,), float('nan'), device='cuda') for k in ('dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre')}
+  for k, t in sums.items():
+    setattr(q, k, t.data_ptr())
+  q.stats = stats.data_ptr()
+  n = _lib.load().advoc_residual_norm_workspace_bytes(ctypes.byref(q))
+  work = torch.empty(n // 4, device='cuda')
+  q.workspace, q.workspace_bytes = work.data_ptr(), n
+  _lib.check(_lib.load().advoc_residual_norm_backward(ctypes.byref(q), _lib.stream()))
+  assert torch.equal(dr, g.dx) and torch.equal(h, g.dh) and torch.equal(gate, g.dgate)
+  for k, t in sums.items():
+    assert torch.equal(t, getattr(g, k)), k
 
 
 def test_norm_before_the_first_block(blocks):
