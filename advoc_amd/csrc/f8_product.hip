@@ -529,6 +529,7 @@ extern "C" int advoc_matmul_nt_f8(const uint8_t* a, const uint8_t* a_scale, int3
     return ADVOC_ERR_UNSUPPORTED;
   if (!advoc::dtype_ok(out_dtype) || (accumulate && out_dtype != ADVOC_F32)) return ADVOC_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) return ADVOC_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(a_scale) | reinterpret_cast<uintptr_t>(b_scale)) & 3) return ADVOC_ERR_UNSUPPORTED;
   // 256 rows of an operand lie behind one 32-bit descriptor; tiles are numbered in 31 bits
   if (k > 8000000 || m > (1LL << 31) || n > (1LL << 31) || ceil_div(m, 64) * ceil_div(n, 64) > 0x3fffffff) return ADVOC_ERR_UNSUPPORTED;
   Args g = {a, a_scale, b, b_scale, out, static_cast<float*>(workspace), m, n};

@@ -24,6 +24,7 @@ int check(const advoc_residual_norm& d) {
   if (d.cols > ADVOC_NORM_MAX_COLS || d.rows > 0x7fffffffLL || (d.offset & 3)) return ADVOC_ERR_UNSUPPORTED;
   if (d.gate.p && (d.gate_group < 1 || d.rows % d.gate_group)) return ADVOC_ERR_BAD_SHAPE;
   if (d.rows > 0 && !d.h.p && (d.norm_post != ADVOC_NORM_NONE || d.gate.p || d.scale)) return ADVOC_ERR_BAD_SHAPE;
+  if (d.rows > 0 && !d.h.p && d.norm_pre == ADVOC_NORM_NONE) return ADVOC_ERR_BAD_SHAPE;      // nothing to compute
   if (d.gate.p && d.rows > d.gate_group && d.gate.pitch < d.cols) return ADVOC_ERR_BAD_SHAPE;
   if (!pitch_ok(d.h, d) || !pitch_ok(d.x, d) || !pitch_ok(d.r, d) || !pitch_ok(d.z, d)) return ADVOC_ERR_BAD_SHAPE;
   return ADVOC_OK;
@@ -37,11 +38,12 @@ advoc::NormArgs device_args(const advoc_residual_norm& d) {
   a.pre = d.norm_pre;
   a.act = d.gate_act;
   a.gate_group = d.gate.p ? d.gate_group : 1;
-  a.w_post = d.w_post;
-  a.b_post = d.b_post;
+  const bool post = d.norm_post != ADVOC_NORM_NONE, pre = d.norm_pre != ADVOC_NORM_NONE;
+  a.w_post = post ? d.w_post : nullptr;      // the identity has neither weight nor bias
+  a.b_post = post ? d.b_post : nullptr;
   a.scale = d.scale;
-  a.w_pre = d.w_pre;
-  a.b_pre = d.b_pre;
+  a.w_pre = pre ? d.w_pre : nullptr;
+  a.b_pre = pre ? d.b_pre : nullptr;
   a.alpha = d.alpha;
   a.eps = d.eps;
   a.inv_cols = (float)(1.0 / d.cols);

@@ -134,7 +134,8 @@ def _norm_desc(**kw):
     (dict(keep_prob=1.1), -1), (dict(norm_post=3), -2), (dict(norm_pre=-1), -2), (dict(gate_act=2), -2), (dict(dtype=3), -2),
     (dict(dtype=1, res_dtype=2), -2), (dict(cols=8193), -2), (dict(rows=2 ** 31), -2), (dict(offset=1), -2),
     (dict(gate=(64, 8), gate_group=3), -1), (dict(gate=(64, 8), gate_group=0), -1), (dict(gate=(64, 7)), -1), (dict(h=(64, 7)), -1),
-    (dict(x=(64, 7)), -1), (dict(z=(64, 7)), -1), (dict(r=(64, 7)), -1), (dict(h=(None, 0)), -1), (dict(stats=68), -2)])
+    (dict(x=(64, 7)), -1), (dict(z=(64, 7)), -1), (dict(r=(64, 7)), -1), (dict(h=(None, 0)), -1), (dict(stats=68), -2),
+    (dict(h=(None, 0), norm_post=0, norm_pre=0), -1)])
 def test_norm_entries_refuse(lib, bad, code):
   assert lib.advoc_residual_norm_forward(_norm_desc(**bad), None) == code
   if 'x' not in bad:                                       # the backward pass reads r
@@ -173,7 +174,7 @@ def test_f8_entries_refuse(lib):
   for k in ('a', 'sa', 'b', 'sb', 'out'):
     assert mul(**{k: None}) == -4
   assert mul(m=-1) == -1 and mul(k=0) == -1 and mul(fa=2) == -2 and mul(fb=-1) == -2 and mul(dtype=5) == -2
-  assert mul(acc=1, dtype=1) == -2 and mul(a=72) == -2 and mul(k=2 ** 24) == -2 and mul(n=2 ** 32) == -2 and mul(m=2 ** 24, n=2 ** 24) == -2
+  assert mul(acc=1, dtype=1) == -2 and mul(a=72) == -2 and mul(sa=66) == -2 and mul(sb=65) == -2 and mul(k=2 ** 24) == -2 and mul(n=2 ** 32) == -2 and mul(m=2 ** 24, n=2 ** 24) == -2
   assert mul(m=0) == 0 and mul(n=0, out=None) == 0
   assert lib.advoc_matmul_nt_f8_workspace_bytes(0, 4, 4, 0) == 0 and lib.advoc_matmul_nt_f8_workspace_bytes(1, 4, 4, 0) == 0
 

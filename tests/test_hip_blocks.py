@@ -308,6 +308,24 @@ def test_norm_of_zeros_constants_and_bad_rows(blocks):
   assert bool((z == 0).all())
 
 
+def test_norm_of_kind_none_takes_no_weight_or_bias(blocks):
+  """What a C caller leaves in a descriptor's w_post, b_post (w_pre, b_pre) is ignored without the norm they belong to."""
+  import ctypes
+  from advoc_amd import _lib
+  norm, d, call, g, (r, z, stats) = check_norm(blocks, 9, (2, 7), 72, 'f32', 'f32', 'none', 'none', 'row', 'none', 0.9)
+  q, rows, _ = norm._descriptor(d['x'], 'x', torch.float32, d['gate'], call['seed'], call['offset'], None, True)
+  wrong = torch.full((72,), 7.0, device='cuda')
+  q.w_post = q.b_post = q.w_pre = q.b_pre = wrong.data_ptr()
+  out = {k: torch.empty_like(r) for k in ('r', 'dh', 'dx', 'dgate')}
+  for name, t in (('h', d['h']), ('r', out['r']), ('dr', d['dr']), ('dh', out['dh']), ('dx', out['dx']), ('dgate', out['dgate'])):
+    getattr(q, name).p, getattr(q, name).pitch = t.data_ptr(), 72
+  _lib.check(_lib.load().advoc_residual_norm_forward(ctypes.byref(q), _lib.stream()))
+  _lib.check(_lib.load().advoc_residual_norm_backward(ctypes.byref(q), _lib.stream()))
+  assert torch.equal(out['r'], r)
+  for k in ('dh', 'dx', 'dgate'):
+    assert torch.equal(out[k], getattr(g, k)), k
+
+
 def test_norm_sigmoid_of_extreme_gates(blocks):
   """Shut at minus infinity, open at infinity, a NaN passed on; in between within 6 units in the last place."""
   norm = blocks.ResidualNorm(512, post='none', pre='none', gate_act='sigmoid', scale=torch.ones(512, device='cuda'))
