@@ -13,8 +13,9 @@
 // four of them 64 consecutive ones, without a turn through LDS.
 #include <utility>
 
-#include "rows.h"
+#include "lanes.h"
 #include "lds_dma.h"
+#include "rows.h"
 
 namespace {
 
@@ -95,10 +96,82 @@ __device__ __forceinline__ void store_part(const Args& g, int64_t row, int64_t c
     if (col + k < g.n) p[k] = (O)((g.accumulate ? (float)p[k] : 0.f) + v[k]);
 }
 
-// ---- few rows (m <= 16): the weights are read once, by whoever multiplies them ----
+// ---- one or two rows: dot products ----
+// A wave is one row of b and reads it in pieces of 1024 bytes, 16 a lane, all of up to 8192 in flight together; a lane's products are
+// summed in fp32 and take their two exponents once per piece.  Bound by the weights' latency: 1 x 512 x 8192 3.9 us a call and 1 x
+// 4096 x 4096 4.2 (the thin kernel: 8.4 and 6.4; the host's share of a call alone is 3.9); from three rows on its arithmetic costs
+// more (3 x 4096 x 4096: 8.1, thin 6.5).
+template <int F>
+__device__ __forceinline__ void widen(int word, float (&v)[4]) {
+  if constexpr (F == ADVOC_E4M3) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
+    v[0] = lo[0], v[1] = lo[1], v[2] = hi[0], v[3] = hi[1];
+  } else {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_bf8(word, false), hi = __builtin_amdgcn_cvt_pk_f32_bf8(word, true);
+    v[0] = lo[0], v[1] = lo[1], v[2] = hi[0], v[3] = hi[1];
+  }
+}
+
+template <typename O, int FA, int FB, int M>
+__global__ __launch_bounds__(256) void f8_dot_kernel(Args g) {
+  constexpr int kPieces = 8, kPiece = 1024;
+  const int lane = threadIdx.x & 63, kp = (int)g.kp;
+  const int64_t n = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (n >= g.n) return;
+  const uint8_t *b = g.b + n * g.kp, *bs = g.b_scale + n * g.sp;
+  float acc[M];
+#pragma unroll
+  for (int i = 0; i < M; ++i) acc[i] = 0.f;
+  for (int k0 = 0; k0 < kp; k0 += kPieces * kPiece) {
+    int4 qb[kPieces];
+    int eb[kPieces];
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      if (k0 + p * kPiece >= kp) continue;
+      const int k = k0 + p * kPiece + lane * 16, at = k < kp ? k : 0;      // (lanes behind the row's end: some piece, times nothing)
+      qb[p] = *reinterpret_cast<const int4*>(b + at);
+      eb[p] = bs[at / kBlock];
+    }
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) {
+      if (k0 + p * kPiece >= kp) continue;
+      const int k = k0 + p * kPiece + lane * 16, at = k < kp ? k : 0;
+      const int words[4] = {qb[p].x, qb[p].y, qb[p].z, qb[p].w};
+      float w[16];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) widen<FB>(words[i], *reinterpret_cast<float(*)[4]>(w + 4 * i));
+#pragma unroll
+      for (int i = 0; i < M; ++i) {
+        const int4 qa = *reinterpret_cast<const int4*>(g.a + i * g.kp + at);
+        const int ea = g.a_scale[i * g.sp + at / kBlock], word[4] = {qa.x, qa.y, qa.z, qa.w};
+        float dot = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+          widen<FA>(word[q], v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dot = fmaf(v[e], w[4 * q + e], dot);
+        }
+        const float term = ldexpf(dot, ea + eb[p] - 254);
+        acc[i] += k < kp ? term : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    const float v = advoc::lanes_sum<64>(acc[i]);
+    if (lane == 0) {
+      O* p = (O*)g.out + i * g.n + n;
+      *p = (O)((g.accumulate ? (float)*p : 0.f) + v);
+    }
+  }
+}
+
+// ---- three to 16 rows: the weights are read once, by whoever multiplies them ----
 // A workgroup is 16 rows of b; its waves take the blocks of the contraction in turn, straight from memory to registers (lane
 // group g the 16-byte pieces g and g + 4 of 16 rows, so that a load covers half lines whole), and meet in LDS in wave order.
-// Bound by the weights' latency: 1 x 4096 x 4096 6.4 us (2.6 TB/s), 1 x 512 x 8192 8.4 (32 workgroups, four blocks a wave).
+// Bound by the weights' latency and, with few columns, by the lines a CU asks for: 4 x 4096 x 4096 6.6 us (2.5 TB/s), 4 x 512 x 8192
+// 9.4 (32 workgroups).
 template <typename O, bool EXACT, int FA, int FB>
 __global__ __launch_bounds__(1024) void f8_thin_kernel(Args g) {
   extern __shared__ f32x4 red[];
@@ -430,13 +503,14 @@ __global__ __launch_bounds__(256) void f8_fold_kernel(const float* __restrict__ 
   }
 }
 
-enum { kThin, kTile64, kTile128, kTile256 };
+enum { kDot, kThin, kTile64, kTile128, kTile256 };
 
 struct Plan {
   int form, splits, per_split;
 };
 
-// The cheapest estimate.  A CU takes 0.75 us for a block of 128 x 128 outputs (1.2 EXACT), 0.4 (0.35) times that for one of
+// One or two rows: dot products (2 x 4096 x 4096: 5.7 us, thin 6.5; 2 x 16384 x 4096: 17.7, thin 17.0).  Otherwise the cheapest
+// estimate.  A CU takes 0.75 us for a block of 128 x 128 outputs (1.2 EXACT), 0.4 (0.35) times that for one of
 // 64 x 64 and twice for one of 256 x 256, whichever its neighbours do; the CUs take tiles in rounds of 256.  A contraction split in s
 // has s times the tiles with 1 / s of the blocks, and 3 us and a write and a read of its partial results more.
 // The thin kernel takes 0.08 us and 4.2 ns a row for a block of 16 columns, 256 of them together.
@@ -444,10 +518,11 @@ struct Plan {
 // 4096: 33 | 24 | 48;  4096 x 2048 x 4096: 63 | 47 | 50;  4096 x 2560 x 4096: 128: 68, 256: 52;  16384 x 1024 x 1024: 39 | 31 | 21.
 // fp32 outputs in 1 | 2 | 4 | 8 parts:  1024 x 1024 x 16384: 112 | 65 | 43 | 50 (128), 57 | 47 | 49 (64);  512 x 512 x 2048: 9.1 |
 // 9.1 | 8.6 | 11.6 (64).
-// Thin | 64 in parts:  1 x 512 x 8192: 8.4 | 8.4;  16 x 512 x 8192: 12.7 | 9.3;  16 x 4096 x 4096: 8.0 | 9.3;  16 x 1000 x 1000: 3.7 |
+// Thin | 64 in parts:  16 x 512 x 8192: 12.7 | 9.3;  16 x 4096 x 4096: 8.0 | 9.3;  16 x 1000 x 1000: 3.7 |
 // 5.2;  with 17 to 64 rows the thin form lost nearly everywhere (64 x 512 x 8192: 28.8 | 9.8).
 Plan make_plan(int64_t m, int64_t n, int blocks, bool exact) {
-  Plan p = {kThin, 1, blocks};
+  Plan p = {m <= 2 ? kDot : kThin, 1, blocks};
+  if (m <= 2) return p;
   const double block_us = exact ? 1.2 : 0.75, fold_us = 8.0 * m * n / 5e6;
   double best = m <= 16 ? (0.08 + 0.0042 * m) * blocks * ceil_div(n, 16 * 256) : 1e30;
   for (int form = kTile64; form <= (exact ? kTile128 : kTile256); ++form) {
@@ -478,6 +553,13 @@ int run(const Args& g, const Plan& p, hipStream_t stream) {
   if (p.form == kThin) {
     const unsigned waves = g.blocks >= 16 ? 16 : g.blocks >= 8 ? 8 : g.blocks >= 4 ? 4 : 2;
     hipLaunchKernelGGL((f8_thin_kernel<O, EXACT, FA, FB>), dim3((unsigned)ceil_div(g.n, 16)), dim3(64 * waves), waves * 1024, stream, g);
+    ADVOC_RETURN_IF_LAUNCH_FAILED();
+    return ADVOC_OK;
+  }
+  if (p.form == kDot) {
+    const dim3 grid((unsigned)ceil_div(g.n, 4));
+    if (g.m == 1) hipLaunchKernelGGL((f8_dot_kernel<O, FA, FB, 1>), grid, dim3(256), 0, stream, g);
+    else hipLaunchKernelGGL((f8_dot_kernel<O, FA, FB, 2>), grid, dim3(256), 0, stream, g);
     ADVOC_RETURN_IF_LAUNCH_FAILED();
     return ADVOC_OK;
   }
