@@ -31,7 +31,7 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(Args a) {
   const int64_t i = base + threadIdx.x * kPer;
   if (i >= a.n) return;
   uint32_t words[kPer] = {};
-  if (thresh) advoc::drop_words8(words, a.key.offset + (uint64_t)i, true, key);
+  if (thresh) advoc::drop_words<kPer>(words, a.key.offset + (uint64_t)i, true, key);
   const T* x = (const T*)a.x;
   T* y = (T*)a.y;
   uint32_t col = 0;

@@ -58,24 +58,26 @@ __device__ __forceinline__ uint2 drop_key_words(const DropKey& k) {
   return make_uint2((uint32_t)s, (uint32_t)(s >> 32));
 }
 
-// The words of elements i ... i + 7 of the stream: element k is kept when words[k] >= thresh.  i = offset + index, of any
-// alignment: a third block is drawn only where i is no multiple of 4, which `aligned` -- uniform over the launch -- rules out.
-__device__ __forceinline__ void drop_words8(uint32_t (&words)[8], uint64_t i, bool aligned, uint2 key) {
+// The words of elements i ... i + N - 1 of the stream, N = 8 or 9: element k is kept when words[k] >= thresh.  i = offset + index, of
+// any alignment: a third block is drawn only where i is no multiple of 4, which `aligned` -- uniform over the launch -- rules out, or
+// for a ninth word.
+template <int N>
+__device__ __forceinline__ void drop_words(uint32_t (&words)[N], uint64_t i, bool aligned, uint2 key) {
   const uint64_t q = i >> 2;
   const uint4 a = philox4x32(q, key), b = philox4x32(q + 1, key);
-  if (aligned) {
+  if (N == 8 && aligned) {
     words[0] = a.x, words[1] = a.y, words[2] = a.z, words[3] = a.w;
     words[4] = b.x, words[5] = b.y, words[6] = b.z, words[7] = b.w;
   } else {
     const uint4 c = philox4x32(q + 2, key);
-    const uint32_t w[11] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z};
-    uint32_t v[10];
+    const uint32_t w[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
+    uint32_t v[11];
     // by masks: a choice between neighbours of an array becomes a load at a chosen address, from memory of the lane's own
     const uint32_t one = 0u - (uint32_t)(i & 1), two = 0u - (uint32_t)(i >> 1 & 1);
 #pragma unroll
-    for (int k = 0; k < 10; ++k) v[k] = (w[k + 1] & one) | (w[k] & ~one);
+    for (int k = 0; k < 11; ++k) v[k] = (w[k + 1] & one) | (w[k] & ~one);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) words[k] = (v[k + 2] & two) | (v[k] & ~two);
+    for (int k = 0; k < N; ++k) words[k] = (v[k + 2] & two) | (v[k] & ~two);
   }
 }
 

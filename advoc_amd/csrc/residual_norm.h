@@ -80,13 +80,15 @@ struct Team {
 };
 
 // The instance for a number of columns: L lanes, NV chunks of V.  Rows of up to 512 columns have one chunk of 8 a lane.
-// (V = 1 only below 8 columns, where a chunk of 8 does not fit.)
+// (V = 1 only below 8 columns, where a chunk of 8 does not fit.  V = 9 for what is a little more than a power of two, as the 2^n + 1
+// bins of a transform are: 16384 x 513 forward 25 us, with two chunks of 8 32; 3999 x 513 fp32 backward 21, 25.)
 template <typename F>
 static inline bool norm_dispatch(int cols, F&& f) {
   if (cols < 8) f.template run<1, 8, 1>();
   else if (cols <= 128) f.template run<8, 16, 1>();
   else if (cols <= 256) f.template run<8, 32, 1>();
   else if (cols <= 512) f.template run<8, 64, 1>();
+  else if (cols <= 576) f.template run<9, 64, 1>();
   else if (cols <= 1024) f.template run<8, 64, 2>();
   else if (cols <= 2048) f.template run<8, 256, 1>();
   else if (cols <= 4096) f.template run<8, 512, 1>();
@@ -118,71 +120,86 @@ __device__ __forceinline__ const T* row_at(const void* base, int64_t at, int col
 template <typename T, int V, int NV>
 struct Raw {
   typename vec8<T>::type v[NV];
+  T one[NV];                    // V = 1: the value, V = 9: the last one
   __device__ __forceinline__ void load(const void* base, int64_t at, const int (&col)[NV]) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const T* p = row_at<T>(base, at, col[j]);
-      if constexpr (V == 8) __builtin_memcpy(&v[j], p, sizeof(v[j]));
-      else v[j][0] = *p;
+      if constexpr (V >= 8) __builtin_memcpy(&v[j], p, sizeof(v[j]));
+      if constexpr (V % 8 == 1) one[j] = p[V - 1];
     }
   }
-  __device__ __forceinline__ f32x8 operator[](int j) const {
-    f32x8 f;
+  __device__ __forceinline__ Vals<V> operator[](int j) const {
+    Vals<V> f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = k < V ? (float)v[j][k] : 0.f;
+    for (int k = 0; k < V; ++k) f[k] = V % 8 == 1 && k == V - 1 ? (float)one[j] : (float)v[j][k & 7];
     return f;
   }
   // The loads have returned behind this.  (A wave may use what it has loaded behind a rendezvous; without this the wait for it would
   // lie there too, and another wave could store to the place first.)
   __device__ __forceinline__ void arrived() {
-    constexpr int kWords = (V * sizeof(T) + 3) / 4;
+    static_assert(V == 8, "wide rows");
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       int w[sizeof(v[j]) / 4];
       __builtin_memcpy(w, &v[j], sizeof(w));
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) asm volatile("" : "+v"(w[i]));
+      for (int i = 0; i < (int)(sizeof(w) / 4); ++i) asm volatile("" : "+v"(w[i]));
       __builtin_memcpy(&v[j], w, sizeof(w));
     }
   }
 };
 template <int V, typename T>
-__device__ __forceinline__ void store_chunk(T* p, const f32x8& v) {
-  if constexpr (V == 8) store8(p, v);
-  else *p = (T)v[0];
+__device__ __forceinline__ void store_chunk(T* p, const Vals<V>& v) {
+  if constexpr (V >= 8) {
+    f32x8 eight;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) eight[k] = v[k];
+    store8(p, eight);
+  }
+  if constexpr (V % 8 == 1) p[V - 1] = (T)v[V - 1];
 }
 
 // Column vectors in LDS: the lanes' chunks side by side, so that 64 lanes read or write theirs without a bank twice.  The first four
-// values of every chunk lie together, then the last four (V = 1: value by value).  The moved-back chunk at the row's end is the last
-// one.  A lane reads its columns of the call's vectors for every row (kept in registers they cost the waves that hide the loads'
-// latency; from the caches, a round trip per vector and row); an absent vector is staged as its neutral value.
+// values of every chunk lie together, then the next four, then the ninth (V = 9) or only (V = 1).  The moved-back chunk at the row's
+// end is the last one.  A lane reads its columns of the call's vectors for every row (kept in registers they cost the waves that hide
+// the loads' latency; from the caches, a round trip per vector and row); an absent vector is staged as its neutral value.
 template <int V>
 struct Chunks {
-  int count;                    // V = 8: of chunks;  V = 1: of columns
-  __host__ __device__ __forceinline__ explicit Chunks(int cols) : count(V == 8 ? (cols + 7) / 8 : cols) {}
-  __host__ __device__ __forceinline__ int floats() const { return count * V; }
-  __device__ __forceinline__ f32x8 get(const float* vec, int chunk) const {
-    f32x8 f(0.f);
-    if constexpr (V == 8) {
-      const float4 a = reinterpret_cast<const float4*>(vec)[chunk], b = reinterpret_cast<const float4*>(vec)[count + chunk];
-      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    } else f[0] = vec[chunk];
+  static constexpr int kFours = V / 4, kOnes = V % 4;
+  int cols, count;
+  __host__ __device__ __forceinline__ explicit Chunks(int cols_) : cols(cols_), count((cols_ + V - 1) / V) {}
+  __host__ __device__ __forceinline__ int floats() const { return (count * V + 3) / 4 * 4; }
+  __device__ __forceinline__ Vals<V> get(const float* vec, int chunk) const {
+    Vals<V> f;
+#pragma unroll
+    for (int h = 0; h < kFours; ++h) {
+      const float4 a = reinterpret_cast<const float4*>(vec)[h * count + chunk];
+      f[4 * h] = a.x, f[4 * h + 1] = a.y, f[4 * h + 2] = a.z, f[4 * h + 3] = a.w;
+    }
+    if constexpr (kOnes) f[V - 1] = vec[4 * kFours * count + chunk];
     return f;
   }
-  __device__ __forceinline__ void put(float* vec, int chunk, const f32x8& f) const {
-    if constexpr (V == 8) {
-      reinterpret_cast<float4*>(vec)[chunk] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(vec)[count + chunk] = make_float4(f[4], f[5], f[6], f[7]);
-    } else vec[chunk] = f[0];
+  __device__ __forceinline__ void put(float* vec, int chunk, const Vals<V>& f) const {
+#pragma unroll
+    for (int h = 0; h < kFours; ++h)
+      reinterpret_cast<float4*>(vec)[h * count + chunk] = make_float4(f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]);
+    if constexpr (kOnes) vec[4 * kFours * count + chunk] = f[V - 1];
   }
-  // the columns that four values (V = 1: one) at `at` of such a vector stand for
-  static constexpr int kPiece = V == 8 ? 4 : 1;
-  __device__ __forceinline__ int pieces() const { return V == 8 ? 2 * count : count; }
-  __device__ __forceinline__ int piece_col(int piece, int cols) const {
-    if constexpr (V == 1) return piece;
-    const int half = piece >= count, at = 8 * (piece - half * count);
-    return (at <= cols - 8 ? at : cols - 8) + 4 * half;
+  // For a workgroup that walks over a vector: f(place in the vector, first column, how many) for this thread's pieces of four values
+  // and of one
+  template <int WG, typename F>
+  __device__ __forceinline__ void walk(F&& f) const {
+    for (int q = threadIdx.x; q < kFours * count; q += WG) {
+      const int h = kFours > 1 && q >= count;
+      f(4 * q, start(q - h * count) + 4 * h, Four());
+    }
+    if constexpr (kOnes)
+      for (int q = threadIdx.x; q < count; q += WG) f(4 * kFours * count + q, start(q) + V - 1, One());
   }
+  struct Four { static constexpr int value = 4; };
+  struct One { static constexpr int value = 1; };
+  __device__ __forceinline__ int start(int chunk) const { return chunk * V <= cols - V ? chunk * V : cols - V; }
 };
 
 // (the compiler would carry what it has read of LDS from row to row in registers, and spill)
@@ -192,9 +209,8 @@ __device__ __forceinline__ void forget_lds() { asm volatile("" ::: "memory"); }
 template <int WG, int V, int N>
 __device__ __forceinline__ void stage_vectors(float* lds, const float* const (&p)[N], const float (&otherwise)[N], int cols) {
   const Chunks<V> chunks(cols);
-  constexpr int kPiece = Chunks<V>::kPiece;
-  for (int q = threadIdx.x; q < chunks.pieces(); q += WG) {
-    const int col = chunks.piece_col(q, cols);
+  chunks.template walk<WG>([&](int at, int col, auto n) {
+    constexpr int kPiece = decltype(n)::value;
     float v[N][kPiece];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -203,26 +219,25 @@ __device__ __forceinline__ void stage_vectors(float* lds, const float* const (&p
       if (p[i]) __builtin_memcpy(v[i], p[i] + col, sizeof(v[i]));
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) __builtin_memcpy(__builtin_assume_aligned(lds + i * chunks.floats() + q * kPiece, 4 * kPiece), v[i], sizeof(v[i]));
-  }
+    for (int i = 0; i < N; ++i) __builtin_memcpy(__builtin_assume_aligned(lds + i * chunks.floats() + at, 4 * kPiece), v[i], sizeof(v[i]));
+  });
 }
 
 // V consecutive floats in global memory
 template <int V>
-__device__ __forceinline__ f32x8 floats_at(const float* p) {
-  f32x8 f(0.f);
-  if constexpr (V == 8) __builtin_memcpy(f.v, p, sizeof(f.v));
-  else f[0] = *p;
+__device__ __forceinline__ Vals<V> floats_at(const float* p) {
+  Vals<V> f;
+  __builtin_memcpy(f.v, p, sizeof(f.v));
   return f;
 }
 
 // what a chunk's elements draw (all kept where nothing is drawn: thresh 0)
 template <int V>
-__device__ __forceinline__ void draw_chunk(uint32_t (&words)[8], uint64_t i, bool aligned, uint2 key, uint32_t thresh) {
+__device__ __forceinline__ void draw_chunk(uint32_t (&words)[V], uint64_t i, bool aligned, uint2 key, uint32_t thresh) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) words[k] = 0;
+  for (int k = 0; k < V; ++k) words[k] = 0;
   if (!thresh) return;
-  if constexpr (V == 8) drop_words8(words, i, aligned, key);
+  if constexpr (V >= 8) drop_words<V>(words, i, aligned, key);
   else words[0] = drop_word(i, key);
 }
 
@@ -239,7 +254,7 @@ __device__ __forceinline__ float sigmoid(float x) {
 
 // act(gate) in place
 template <int V>
-__device__ __forceinline__ void activate(f32x8& g, int act) {
+__device__ __forceinline__ void activate(Vals<V>& g, int act) {
   if (act == ADVOC_GATE_SIGMOID)
 #pragma unroll
     for (int k = 0; k < V; ++k) g[k] = sigmoid(g[k]);

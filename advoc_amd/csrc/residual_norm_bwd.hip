@@ -16,14 +16,14 @@
 // Measured (kernel + the second launch): 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (302 MB): 69 + 6 us, 4.4
 // TB/s; each further row comes at 5.0 TB/s, a copy's rate, and 12 us are the way of the first row (arguments and vectors 4, loads 2,
 // arithmetic 4, the workgroup's column sums 3).  4096 x 4096 fp16 (201 MB, and 25 MB of column sums): 51 + 5.  3999 x 513 fp32 (66
-// MB): 24 + 4, two rows a worker: the same start, and the arithmetic of a second chunk for one column.
+// MB): 21 + 4, two rows a worker: the same start, and the arithmetic.
 #include "residual_norm.h"
 
 namespace {
 
-using advoc::f32x8;
 using advoc::NormArgs;
 using advoc::Team;
+using advoc::Vals;
 
 enum { kDwPost, kDbPost, kDscale, kDwPre, kDbPre, kSums };
 
@@ -44,7 +44,7 @@ constexpr int kSumsTogether = NV > 1 ? 4 : 5;
 
 // t <- the gradient of a row given that of its normed values (times the weight): rstd (t - [mean t] - hat mean(t hat))
 template <int V, int L, int NV, int WG>
-__device__ __forceinline__ void norm_back(f32x8 (&t)[NV], const f32x8 (&hat)[NV], const int (&dup)[NV], bool ragged, int kind,
+__device__ __forceinline__ void norm_back(Vals<V> (&t)[NV], const Vals<V> (&hat)[NV], const int (&dup)[NV], bool ragged, int kind,
                                           float inv_cols, float rstd, float* red, int& turn) {
   float s0 = advoc::own_sum<V>(dup, ragged, [&](int j, int k) { return t[j][k]; });
   float s1 = advoc::own_sum<V>(dup, ragged, [&](int j, int k) { return t[j][k] * hat[j][k]; });
@@ -91,9 +91,9 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
   Row::meet();
 
   // sums over rows.  g0, g1 are E0, E1 but for the gate where rows share one
-  f32x8 dw_pre[NV], db_pre[NV], g0[NV], g1[NV];
+  Vals<V> dw_pre[NV], db_pre[NV], g0[NV], g1[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) dw_pre[j] = db_pre[j] = g0[j] = g1[j] = f32x8(0.f);
+  for (int j = 0; j < NV; ++j) dw_pre[j] = db_pre[j] = g0[j] = g1[j] = Vals<V>(0.f);
   // a worker with several clips carries E0, E1 of those before in memory of its own
   constexpr int kOwn = NV * L * V;
   float* const carry = a.carry ? a.carry + ((int64_t)blockIdx.x * Row::kRows + Row::slot()) * 2 * kOwn + lane * V : nullptr;
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
     const int64_t end = (int64_t)(group + 1) * group_rows;
     if (H && carry)
 #pragma unroll
-      for (int j = 0; j < NV; ++j) g0[j] = g1[j] = f32x8(0.f);
+      for (int j = 0; j < NV; ++j) g0[j] = g1[j] = Vals<V>(0.f);
     advoc::Raw<T, V, NV> raw_gate, raw_dz, raw_h;
     advoc::Raw<R, V, NV> raw_r, raw_dr;
     auto load = [&](int64_t row) {
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
     for (int64_t row = end - group_rows + first; row < end; row += a.splits) {
       advoc::forget_lds();
       if constexpr (!kAhead) load(row);
-      f32x8 hat[NV], t[NV], g[NV], gate[NV];
+      Vals<V> hat[NV], t[NV], g[NV], gate[NV];
       const float4 st = PRE || post ? a.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
@@ -166,22 +166,22 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
       advoc::forget_lds();
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        uint32_t words[8];
+        uint32_t words[V];
         advoc::draw_chunk<V>(words, a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
         advoc::activate<V>(gate[j], a.act);
-        const f32x8 s = scale(j);
+        const Vals<V> s = scale(j);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
           gate[j][k] = has_gate ? gate[j][k] : 1.f;
           t[j][k] = words[k] >= a.key.thresh ? g[j][k] * kept : 0.f;
         }
         if (row_gate && a.dgate) {
-          f32x8 dg = t[j] * s * (hat[j] * w_post(j) + b_post(j));
-          if (a.act == ADVOC_GATE_SIGMOID) dg *= gate[j] * (f32x8(1.f) - gate[j]);
+          Vals<V> dg = t[j] * s * (hat[j] * w_post(j) + b_post(j));
+          if (a.act == ADVOC_GATE_SIGMOID) dg *= gate[j] * (Vals<V>(1.f) - gate[j]);
           advoc::store_chunk<V>(advoc::row_at<T>(a.dgate, row * a.dgate_pitch, col[j]), dg);
         }
-        const f32x8 e = t[j] * gate[j];
-        f32x8 sum = shared_gate ? t[j] : e;
+        const Vals<V> e = t[j] * gate[j];
+        Vals<V> sum = shared_gate ? t[j] : e;
         g0[j] += sum;
         g1[j] += sum * hat[j];
         t[j] = e * s * w_post(j);               // (w_post is staged as ones without a post norm)
@@ -199,11 +199,11 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        f32x8 gate = raw_gate[j];
+        Vals<V> gate = raw_gate[j];
         advoc::activate<V>(gate, a.act);
         if (a.dgate) {
-          f32x8 dg = scale(j) * (w_post(j) * g1[j] + b_post(j) * g0[j]);
-          if (a.act == ADVOC_GATE_SIGMOID) dg *= gate * (f32x8(1.f) - gate);
+          Vals<V> dg = scale(j) * (w_post(j) * g1[j] + b_post(j) * g0[j]);
+          if (a.act == ADVOC_GATE_SIGMOID) dg *= gate * (Vals<V>(1.f) - gate);
           if (a.gate_part) advoc::store_chunk<V>(a.gate_part + (int64_t)seg * cols + col[j], dg);
           else advoc::store_chunk<V>(advoc::row_at<T>(a.dgate, group * a.dgate_pitch, col[j]), dg);
         }
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
   }
 
   // the workgroup's column sums: values of a column with two holders are equal, so either may store them
-  f32x8 out[kSums][NV];
+  Vals<V> out[kSums][NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     out[kDwPost][j] = scale(j) * g1[j];
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
           advoc::store_chunk<V>(a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * cols + col[j], out[s][j]);
   } else {
     // kTogether sums at a time: [sum][row of the workgroup] in LDS
-    constexpr int kTogether = kSumsTogether<NV>, kPiece = advoc::Chunks<V>::kPiece;
+    constexpr int kTogether = kSumsTogether<NV>;
 #pragma unroll
     for (int first = 0; first < kSums; first += kTogether) {
       __syncthreads();
@@ -252,12 +252,12 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
 #pragma unroll
           for (int j = 0; j < NV; ++j) chunks.put(vec + ((s - first) * Row::kRows + Row::slot()) * floats, chunk[j], out[s][j]);
       __syncthreads();
-      for (int q = threadIdx.x; q < chunks.pieces(); q += WG) {
-        const int c = chunks.piece_col(q, cols);
+      chunks.template walk<WG>([&](int at, int c, auto n) {
+        constexpr int kPiece = decltype(n)::value;
 #pragma unroll
         for (int s = first; s < kSums && s < first + kTogether; ++s) {
           if (sums.slot[s] < 0) continue;
-          const float* from = vec + (s - first) * Row::kRows * floats + q * kPiece;
+          const float* from = vec + (s - first) * Row::kRows * floats + at;
           float v[kPiece];
 #pragma unroll
           for (int k = 0; k < kPiece; ++k) v[k] = 0.f;
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
           }
           __builtin_memcpy(a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * cols + c, v, sizeof(v));
         }
-      }
+      });
     }
   }
 }

@@ -9,13 +9,13 @@
 
 namespace {
 
-using advoc::f32x8;
 using advoc::NormArgs;
 using advoc::Team;
+using advoc::Vals;
 
 // mean and 1 / sqrt(var + eps) of a row
 template <int V, int L, int NV, int WG>
-__device__ __forceinline__ void row_stats(const f32x8 (&a)[NV], const int (&dup)[NV], bool ragged, int kind, float inv_cols, float eps,
+__device__ __forceinline__ void row_stats(const Vals<V> (&a)[NV], const int (&dup)[NV], bool ragged, int kind, float inv_cols, float eps,
                                           float* red, int& turn, float& mean, float& rstd) {
   mean = 0.f;
   float none = 0.f;
@@ -41,8 +41,8 @@ constexpr bool kFiveVectors = V * L * NV <= 4096;
 // (8192 x 2048: 50 us, without 55; 4096 x 4096: 50, without 62); with 16 they would spill (16384 x 1024: 38 us, with them 65).  A wave waits for its loads and stores in the order of their issue, so that the number of stores behind the
 // loads is to be known where the loads are waited for: hence the templates.
 // 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (202 MB): 38 us, 5.3 TB/s, a copy's rate.  Rows of a whole
-// workgroup meet four times on their way: 4096 x 4096 50 us, 4.0 TB/s.  16384 x 513: 32 us, 3.1 TB/s, bound by arithmetic (a second
-// chunk for one column, rows at odd offsets, three Philox blocks for eight words).  One row: 6 us, latency.
+// workgroup meet four times on their way: 4096 x 4096 50 us, 4.0 TB/s.  16384 x 513: 25 us, 4.0 TB/s, bound by arithmetic (rows at
+// odd offsets, three Philox blocks for nine words).  One row: 6 us, latency.
 template <typename T, typename R, int V, int L, int NV, int WG, bool H, bool PRE>
 __global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
   using Row = Team<L, WG>;
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
       if constexpr (H) h.arrived(), gate.arrived();
       Row::meet();
     }
-    f32x8 r[NV], u[NV], g[NV];
+    Vals<V> r[NV], u[NV], g[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       r[j] = x[j];
@@ -107,9 +107,9 @@ __global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         u[j] = (u[j] - mean0) * by * chunks.get(vec + floats, chunk[j]) + chunks.get(vec + 2 * floats, chunk[j]);
-        uint32_t words[8];
+        uint32_t words[V];
         advoc::draw_chunk<V>(words, a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
-        f32x8 s = chunks.get(vec, chunk[j]) * kept;
+        Vals<V> s = chunks.get(vec, chunk[j]) * kept;
         advoc::activate<V>(g[j], a.act);
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
       row_stats<V, L, NV, WG>(r, dup, ragged, a.pre, a.inv_cols, a.eps, red, turn, mean1, rstd1);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        f32x8 z = (r[j] - mean1) * rstd1 * chunks.get(vec + 3 * floats, chunk[j]);
+        Vals<V> z = (r[j] - mean1) * rstd1 * chunks.get(vec + 3 * floats, chunk[j]);
         if constexpr (kFive) z += chunks.get(vec + 4 * floats, chunk[j]);
         else if (a.b_pre) z += advoc::floats_at<V>(a.b_pre + col[j]);
         advoc::store_chunk<V>(advoc::row_at<T>(a.z, row * a.z_pitch, col[j]), z);

@@ -6,38 +6,44 @@
 
 namespace advoc {
 
-// eight fp32 values in eight registers of their own (a 256-bit vector type would tie them together)
-struct f32x8 {
-  float v[8];
-  f32x8() = default;
-  __device__ __forceinline__ explicit f32x8(float x) {
+// N fp32 values in N registers of their own (a 256-bit vector type would tie them together)
+template <int N>
+struct Vals {
+  float v[N];
+  Vals() = default;
+  __device__ __forceinline__ explicit Vals(float x) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = x;
+    for (int k = 0; k < N; ++k) v[k] = x;
   }
   __device__ __forceinline__ float& operator[](int k) { return v[k]; }
   __device__ __forceinline__ float operator[](int k) const { return v[k]; }
 };
-#define ADVOC_F32X8_OP(OP)                                                     \
-  __device__ __forceinline__ f32x8 operator OP(f32x8 a, const f32x8& b) {      \
-    _Pragma("unroll") for (int k = 0; k < 8; ++k) a.v[k] = a.v[k] OP b.v[k];   \
-    return a;                                                                  \
-  }                                                                            \
-  __device__ __forceinline__ f32x8 operator OP(f32x8 a, float b) {             \
-    _Pragma("unroll") for (int k = 0; k < 8; ++k) a.v[k] = a.v[k] OP b;        \
-    return a;                                                                  \
-  }                                                                            \
-  __device__ __forceinline__ f32x8& operator OP##=(f32x8& a, const f32x8& b) { \
-    _Pragma("unroll") for (int k = 0; k < 8; ++k) a.v[k] = a.v[k] OP b.v[k];   \
-    return a;                                                                  \
-  }                                                                            \
-  __device__ __forceinline__ f32x8& operator OP##=(f32x8& a, float b) {        \
-    _Pragma("unroll") for (int k = 0; k < 8; ++k) a.v[k] = a.v[k] OP b;        \
-    return a;                                                                  \
+#define ADVOC_VALS_OP(OP)                                                                  \
+  template <int N>                                                                         \
+  __device__ __forceinline__ Vals<N> operator OP(Vals<N> a, const Vals<N>& b) {            \
+    _Pragma("unroll") for (int k = 0; k < N; ++k) a.v[k] = a.v[k] OP b.v[k];               \
+    return a;                                                                              \
+  }                                                                                        \
+  template <int N>                                                                         \
+  __device__ __forceinline__ Vals<N> operator OP(Vals<N> a, float b) {                     \
+    _Pragma("unroll") for (int k = 0; k < N; ++k) a.v[k] = a.v[k] OP b;                    \
+    return a;                                                                              \
+  }                                                                                        \
+  template <int N>                                                                         \
+  __device__ __forceinline__ Vals<N>& operator OP##=(Vals<N>& a, const Vals<N>& b) {       \
+    _Pragma("unroll") for (int k = 0; k < N; ++k) a.v[k] = a.v[k] OP b.v[k];               \
+    return a;                                                                              \
+  }                                                                                        \
+  template <int N>                                                                         \
+  __device__ __forceinline__ Vals<N>& operator OP##=(Vals<N>& a, float b) {                \
+    _Pragma("unroll") for (int k = 0; k < N; ++k) a.v[k] = a.v[k] OP b;                    \
+    return a;                                                                              \
   }
-ADVOC_F32X8_OP(+)
-ADVOC_F32X8_OP(-)
-ADVOC_F32X8_OP(*)
-#undef ADVOC_F32X8_OP
+ADVOC_VALS_OP(+)
+ADVOC_VALS_OP(-)
+ADVOC_VALS_OP(*)
+#undef ADVOC_VALS_OP
+typedef Vals<8> f32x8;
 
 template <typename T>
 struct vec8 {

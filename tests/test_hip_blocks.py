@@ -186,7 +186,7 @@ def test_norm_types_and_options(blocks, dt, res, kind):
   check_norm(blocks, kind, (3, 37), 200, dt, res, *KINDS[kind])
 
 
-@pytest.mark.parametrize('cols', [1, 2, 7, 8, 9, 16, 80, 127, 128, 129, 256, 257, 512, 513, 1000, 1024, 1025, 2048, 2049, 4096, 4099, 8191, 8192])
+@pytest.mark.parametrize('cols', [1, 2, 7, 8, 9, 16, 80, 127, 128, 129, 256, 257, 512, 513, 514, 575, 576, 577, 1000, 1024, 1025, 2048, 2049, 4096, 4099, 8191, 8192])
 def test_norm_widths(blocks, cols):
   """Every instance of the kernels, at its edges, whole chunks and ragged ones."""
   check_norm(blocks, cols, (2, 5), cols, 'bf16', 'f32', *KINDS[1 + cols % 2])
