@@ -1,7 +1,8 @@
 // Dropout whose mask is never stored (gfx950): y_i = x_i / keep where word i of the Philox stream (philox.h) is kept, exactly 0
 // elsewhere whatever x_i holds; the gradient is the same call on dy.  Reads and writes each element once: no byte of mask in
-// HBM, and the backward pass draws the same words again.  HBM-bound: 65536 x 1024 bf16 (268 MB) in 46 us, 5.8 TB/s, a copy's rate;
-// one frame takes the 6.6 us of a call.
+// HBM, and the backward pass draws the same words again.  HBM-bound: 65536 x 1024 bf16 (268 MB) in 43 us, 6.2 TB/s, a copy's rate
+// (45 with the loads behind the drawing); 8192 x 513 fp16 in padded rows 8.4, one round of workgroups; one frame takes the 6.6 us of a
+// call.
 #include "philox.h"
 #include "rows.h"
 
@@ -30,8 +31,6 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(Args a) {
   const int64_t base = (int64_t)blockIdx.x * (kThreads * kPer);      // a multiple of 4, as the offset is
   const int64_t i = base + threadIdx.x * kPer;
   if (i >= a.n) return;
-  uint32_t words[kPer] = {};
-  if (thresh) advoc::drop_words<kPer>(words, a.key.offset + (uint64_t)i, true, key);
   const T* x = (const T*)a.x;
   T* y = (T*)a.y;
   uint32_t col = 0;
@@ -46,17 +45,19 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(Args a) {
     x += i;
     y += i;
   }
-  if (i + kPer <= a.n && (!PITCHED || col + kPer <= a.cols)) {
-    const f32x8 v = advoc::load8(x);
-    f32x8 o;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) o[k] = words[k] >= thresh ? v[k] * scale : 0.f;
-    advoc::store8(y, o);
+  // A chunk in which a row or the tensor ends (one in a wave for rows of 513) goes by elements.  Loads first, all of them in flight
+  // while the words are drawn.
+  const bool whole = i + kPer <= a.n && (!PITCHED || col + kPer <= a.cols);
+  typename advoc::vec8<T>::type v;
+  T* to[kPer];
+  if (whole) {
+    __builtin_memcpy(&v, x, sizeof(v));
   } else {
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
-      if (i + k >= a.n) break;
-      *y = (T)(words[k] >= thresh ? (float)*x * scale : 0.f);
+      to[k] = y;
+      v[k] = *x;
+      if (i + k + 1 >= a.n) continue;           // (behind the last element: that one again, not stored)
       ++x, ++y;
       if (PITCHED && ++col == a.cols) {
         col = 0;
@@ -64,6 +65,18 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(Args a) {
         y += a.y_pitch - a.cols;
       }
     }
+  }
+  uint32_t words[kPer] = {};
+  if (thresh) advoc::drop_words<kPer>(words, a.key.offset + (uint64_t)i, true, key);
+  f32x8 o;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) o[k] = words[k] >= thresh ? (float)v[k] * scale : 0.f;
+  if (whole) {
+    advoc::store8(y, o);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      if (i + k < a.n) *to[k] = (T)o[k];
   }
 }
 
