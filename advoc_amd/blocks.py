@@ -17,8 +17,8 @@ stream of the tensors' device and can be captured into a graph.
   dw = blocks.matmul_nt_f8(dyt, z8t)                                             # z8t = blocks.quantize_f8_transposed(z)
 """
 import collections
-import ctypes
 import functools
+import struct
 
 import torch
 
@@ -76,7 +76,7 @@ def _rows(t, name, index=None):
 
 def _seed_word(seed_dev, index):
   if seed_dev is None:
-    return None
+    return 0
   if not isinstance(seed_dev, torch.Tensor) or not seed_dev.is_cuda or seed_dev.get_device() != index or (
       seed_dev.numel() != 1) or seed_dev.dtype not in (torch.int64, torch.uint64):
     raise _lib.AdvocHipError('seed_dev must be one int64 or uint64 on device {}'.format(index))
@@ -131,6 +131,15 @@ ResidualNormGrads = collections.namedtuple('ResidualNormGrads',
 
 _PARAMETER_GRADS = ResidualNormGrads._fields[3:]
 
+# struct advoc_residual_norm packed in one go (a ctypes structure costs 4 us a call to fill): up to the parameter gradients, and the
+# workspace behind them
+_DESCRIPTOR_HEAD = struct.Struct('@q6iq5P3fi2QP' + 'Pq' * 5 + 'P' + 'Pq' * 5 + '5P')
+_DESCRIPTOR_TAIL = struct.Struct('@Pq')
+_DESCRIPTOR = struct.Struct(_DESCRIPTOR_HEAD.format + _DESCRIPTOR_TAIL.format[1:])
+_ABSENT = (0, 0)
+_NO_BACKWARD = (0,) * 17
+_NO_WORKSPACE = _DESCRIPTOR_TAIL.pack(0, 0)
+
 
 class ResidualNorm(object):
   """The glue between two residual blocks (``advoc_residual_norm_forward / _backward``), per row of `cols` channels:
@@ -159,21 +168,25 @@ class ResidualNorm(object):
 
   def _vector(self, t, name, index):
     if t is None:
-      return None
+      return 0
     if not isinstance(t, torch.Tensor) or t.get_device() != index or t.dtype != torch.float32 or t.shape != self._shape or (
         not t.is_contiguous()):
       raise _lib.AdvocHipError('{} must be a contiguous float32 tensor of {} on device {}'.format(name, self.cols, index))
     return t.data_ptr()
 
-  def _bind(self, field, name, t, rows, index, dtype=None):
-    field.p, n, cols, field.pitch = _rows(t, name, index)
+  def _tensor(self, name, t, rows, index, dtype=None):
+    """(address, pitch) of `rows` rows of self.cols; dtype: the one it has to have."""
+    p, n, cols, pitch = _rows(t, name, index)
     if n != rows or cols != self.cols:
       raise _lib.AdvocHipError('{} has shape {}: {} rows of {} wanted'.format(name, tuple(t.shape), rows, self.cols))
     if dtype is not None and t.dtype != dtype:
       raise _lib.AdvocHipError('{} is {}, {} wanted'.format(name, t.dtype, dtype))
+    return p, pitch
 
-  def _descriptor(self, x, name, dtype, gate, seed, offset, seed_dev, has_h):
-    """What both directions share; x (r in the backward pass) sets rows, device and residual dtype."""
+  def _head(self, x, name, dtype, gate, seed, offset, seed_dev, has_h):
+    """What both directions share; x (r in the backward pass) sets rows, device and residual dtype.  -> (device index, rows, x's
+    address and pitch, the gate's, the descriptor's fields up to the gate group, those from the weights to keep_prob, seed to
+    seed_dev)"""
     px, rows, cols, pitch = _rows(x, name)
     if cols != self.cols:
       raise _lib.AdvocHipError('{} has {} columns, {} wanted'.format(name, cols, self.cols))
@@ -181,29 +194,24 @@ class ResidualNorm(object):
     code, res_code = _DTYPES.get(dtype, -1), _dtype(x, name)
     if code < 0 or res_code not in (code, 0):
       raise _lib.AdvocHipError('{} is {}: it must be float32 or the dtype of the block ({})'.format(name, x.dtype, dtype))
+    w_pre, b_pre = self._vector(self.w_pre, 'w_pre', index), self._vector(self.b_pre, 'b_pre', index)
     if not has_h:
       if gate is not None:
         raise _lib.AdvocHipError('a gate needs a block output h')
-      d = _lib.ResidualNorm(rows, cols, code, res_code, 0, self.pre, 0, 1, None, None, None,
-                            self._vector(self.w_pre, 'w_pre', index), self._vector(self.b_pre, 'b_pre', index), self.alpha,
-                            self.eps, self.keep_prob)
-    else:
-      d = _lib.ResidualNorm(rows, cols, code, res_code, self.post, self.pre, self.gate_act, 1,
-                            self._vector(self.w_post, 'w_post', index), self._vector(self.b_post, 'b_post', index),
-                            self._vector(self.scale, 'scale', index), self._vector(self.w_pre, 'w_pre', index),
-                            self._vector(self.b_pre, 'b_pre', index), self.alpha, self.eps, self.keep_prob, 0, seed & _MASK64,
-                            offset & _MASK64, _seed_word(seed_dev, index))
-      if gate is not None:
-        field = d.gate
-        field.p, n, cols, field.pitch = _rows(gate, 'gate', index)
-        if cols != self.cols or gate.dtype != dtype or (rows % n if n else rows):
-          raise _lib.AdvocHipError('gate {} {} does not divide {} rows of {} {}'.format(
-              gate.dtype, tuple(gate.shape), rows, self.cols, dtype))
-        self._check_gate_shape(gate, x)
-        d.gate_group = rows // n if n else 1
-    field = getattr(d, name)
-    field.p, field.pitch = px, pitch
-    return d, rows, index
+      return (index, rows, px, pitch, _ABSENT, (rows, cols, code, res_code, 0, self.pre, 0, 1),
+              (0, 0, 0, w_pre, b_pre, self.alpha, self.eps, self.keep_prob), (0, 0, 0))
+    pg, group = _ABSENT, 1
+    if gate is not None:
+      p, n, gate_cols, gate_pitch = _rows(gate, 'gate', index)
+      if gate_cols != cols or gate.dtype != dtype or (rows % n if n else rows):
+        raise _lib.AdvocHipError('gate {} {} does not divide {} rows of {} {}'.format(
+            gate.dtype, tuple(gate.shape), rows, cols, dtype))
+      self._check_gate_shape(gate, x)
+      pg, group = (p, gate_pitch), rows // n if n else 1
+    return (index, rows, px, pitch, pg, (rows, cols, code, res_code, self.post, self.pre, self.gate_act, group),
+            (self._vector(self.w_post, 'w_post', index), self._vector(self.b_post, 'b_post', index),
+             self._vector(self.scale, 'scale', index), w_pre, b_pre, self.alpha, self.eps, self.keep_prob),
+            (seed & _MASK64, offset & _MASK64, _seed_word(seed_dev, index)))
 
   def _check_gate_shape(self, gate, x):
     """A gate has x's shape, with ones for trailing row dimensions that share it: [clips, 1, cols] for [clips, frames, cols]."""
@@ -225,30 +233,30 @@ class ResidualNorm(object):
     if not isinstance(like, torch.Tensor):
       raise _lib.AdvocHipError('h and x must be torch tensors')
     dtype = like.dtype
-    d, rows, index = self._descriptor(x, 'x', dtype, gate, seed, offset, seed_dev, h is not None)
+    index, rows, px, pitch, pg, shape, weights, draw = self._head(x, 'x', dtype, gate, seed, offset, seed_dev, h is not None)
+    ph = pr = pz = _ABSENT
     if h is None:
       if not self.pre:
         raise _lib.AdvocHipError('neither h nor a pre norm: nothing to compute')
       r = x
     else:
-      self._bind(d.h, 'h', h, rows, index)
+      ph = self._tensor('h', h, rows, index)
       if r is None:
         r = torch.empty_like(x, memory_format=torch.contiguous_format)
-        d.r.p, d.r.pitch = r.data_ptr(), self.cols
+        pr = r.data_ptr(), self.cols
       else:
-        self._bind(d.r, 'r', r, rows, index, x.dtype)
+        pr = self._tensor('r', r, rows, index, x.dtype)
     if not self.pre:
       z = None
     elif z is None:
       z = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
-      d.z.p, d.z.pitch = z.data_ptr(), self.cols
+      pz = z.data_ptr(), self.cols
     else:
-      self._bind(d.z, 'z', z, rows, index, dtype)
-    stats = None
-    if save:
-      stats = torch.empty(rows, 4, dtype=torch.float32, device=x.device)
-      d.stats = stats.data_ptr()
-    _call(_lib.load().advoc_residual_norm_forward, 'advoc_residual_norm_forward', index, ctypes.byref(d))
+      pz = self._tensor('z', z, rows, index, dtype)
+    stats = torch.empty(rows, 4, dtype=torch.float32, device=x.device) if save else None
+    d = _DESCRIPTOR.pack(*shape, *weights, 0, *draw, *ph, px, pitch, *pg, *pr, *pz, stats.data_ptr() if save else 0,
+                         *_NO_BACKWARD)
+    _call(_lib.load().advoc_residual_norm_forward, 'advoc_residual_norm_forward', index, d)
     return r, z, stats
 
   def backward(self, dz, dr, h, r, stats, gate=None, seed=0, offset=0, seed_dev=None, into=None, accumulate=False):
@@ -258,66 +266,59 @@ class ResidualNorm(object):
     like = h if h is not None else dz
     if not isinstance(like, torch.Tensor):
       raise _lib.AdvocHipError('h or dz is needed')
-    d, rows, index = self._descriptor(r, 'r', like.dtype, gate, seed, offset, seed_dev, h is not None)
+    index, rows, p, pitch, pg, shape, weights, draw = self._head(r, 'r', like.dtype, gate, seed, offset, seed_dev, h is not None)
     if (dz is None) != (not self.pre) or (dz is None and dr is None):
       raise _lib.AdvocHipError('dz goes with a pre norm, and dz or dr must be given')
-    if dz is not None:
-      self._bind(d.dz, 'dz', dz, rows, index, like.dtype)
-    if dr is not None:
-      self._bind(d.dr, 'dr', dr, rows, index, r.dtype)
-    if h is not None:
-      self._bind(d.h, 'h', h, rows, index)
+    pdz = _ABSENT if dz is None else self._tensor('dz', dz, rows, index, like.dtype)
+    pdr = _ABSENT if dr is None else self._tensor('dr', dr, rows, index, r.dtype)
+    ph = _ABSENT if h is None else self._tensor('h', h, rows, index)
+    pstats = 0
     if self.pre or h is not None and self.post:
-      if not isinstance(stats, torch.Tensor) or not stats.is_cuda or stats.get_device() != index or (
-          stats.dtype != torch.float32 or stats.shape != (rows, 4) or not stats.is_contiguous()):
+      if not isinstance(stats, torch.Tensor) or stats.get_device() != index or stats.dtype != torch.float32 or (
+          stats.shape != (rows, 4) or not stats.is_contiguous()):
         raise _lib.AdvocHipError('stats must be the contiguous float32 [rows, 4] tensor of forward(..., save=True)')
-      d.stats = stats.data_ptr()
-    contiguous = torch.contiguous_format
+      pstats = stats.data_ptr()
+    contiguous, cols = torch.contiguous_format, self.cols
     dx = torch.empty_like(r, memory_format=contiguous)
-    d.dx.p, d.dx.pitch = dx.data_ptr(), self.cols
     dh = dgate = None
+    pdh = pdgate = _ABSENT
     if h is not None:
       dh = torch.empty_like(r, dtype=h.dtype, memory_format=contiguous)
-      d.dh.p, d.dh.pitch = dh.data_ptr(), self.cols
+      pdh = dh.data_ptr(), cols
     if gate is not None:
       dgate = torch.empty_like(gate, memory_format=contiguous)
-      d.dgate.p, d.dgate.pitch = dgate.data_ptr(), self.cols
-    wanted = [] if h is None else [name for name, p in (('dw_post', self.w_post), ('db_post', self.b_post), ('dscale', self.scale))
-                                   if p is not None]
-    if self.w_pre is not None:
-      wanted.append('dw_pre')
-    if self.b_pre is not None:
-      wanted.append('db_pre')
-    g = dict.fromkeys(_PARAMETER_GRADS)
+      pdgate = dgate.data_ptr(), cols
+    # dw_post, db_post, dscale, dw_pre, db_pre
+    wanted = [w is not None for w in (self.w_post, self.b_post, self.scale, self.w_pre, self.b_pre)]
+    if h is None:
+      wanted[:3] = (False, False, False)
+    g = [None] * 5
     if into:
-      unknown = set(into) - set(wanted)
+      unknown = set(into) - {name for name, want in zip(_PARAMETER_GRADS, wanted) if want}
       if unknown:
         raise _lib.AdvocHipError('no such parameter gradients here: {}'.format(sorted(unknown)))
-      for name in wanted:
-        t = into.get(name)
-        if t is not None:
-          setattr(d, name, self._vector(t, name, index))
-          g[name] = t
-    new = [name for name in wanted if g[name] is None]
+      for i, name in enumerate(_PARAMETER_GRADS):
+        g[i] = into.get(name)
+        self._vector(g[i], name, index)
+    new = [i for i in range(5) if wanted[i] and g[i] is None]
     if new:
       if accumulate:
-        raise _lib.AdvocHipError('accumulate needs a buffer for {}'.format(new))
-      for name, t in zip(new, torch.empty(len(new), self.cols, dtype=torch.float32, device=r.device)):
-        g[name] = t
-        setattr(d, name, t.data_ptr())
-    d.accumulate = int(bool(accumulate))
+        raise _lib.AdvocHipError('accumulate needs a buffer for {}'.format([_PARAMETER_GRADS[i] for i in new]))
+      for i, t in zip(new, torch.empty(len(new), cols, dtype=torch.float32, device=r.device).unbind()):
+        g[i] = t
+    pgrads = [0 if t is None else t.data_ptr() for t in g]
+    head = _DESCRIPTOR_HEAD.pack(*shape, *weights, 1 if accumulate else 0, *draw, *ph, *_ABSENT, *pg, p, pitch, *_ABSENT, pstats,
+                                 *pdz, *pdr, *pdh, dx.data_ptr(), cols, *pdgate, *pgrads)
     lib = _lib.load()
-    ref = ctypes.byref(d)
-    nbytes = lib.advoc_residual_norm_workspace_bytes(ref)
-    if nbytes:
-      work = torch.empty(nbytes // 4, dtype=torch.float32, device=r.device)
-      d.workspace, d.workspace_bytes = work.data_ptr(), nbytes
+    nbytes = lib.advoc_residual_norm_workspace_bytes(head + _NO_WORKSPACE)
+    work = torch.empty(nbytes // 4, dtype=torch.float32, device=r.device) if nbytes else None
     if rows == 0 and not accumulate:
-      for t in g.values():
+      for t in g:
         if t is not None:
           t.zero_()
-    _call(lib.advoc_residual_norm_backward, 'advoc_residual_norm_backward', index, ref)
-    return ResidualNormGrads(dh, dx, dgate, *g.values())
+    _call(lib.advoc_residual_norm_backward, 'advoc_residual_norm_backward', index,
+          head + _DESCRIPTOR_TAIL.pack(work.data_ptr(), nbytes) if nbytes else head + _NO_WORKSPACE)
+    return ResidualNormGrads(dh, dx, dgate, *g)
 
 
 class F8Matrix(object):

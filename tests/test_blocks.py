@@ -99,6 +99,17 @@ def test_struct_layout_matches_the_header(tmp_path):
     assert int(out[f]) == getattr(_lib.ResidualNorm, f).offset, f
 
 
+def test_packed_descriptor_is_the_struct():
+  n = len(blocks._DESCRIPTOR.unpack(bytes(blocks._DESCRIPTOR.size)))
+  assert blocks._DESCRIPTOR.size == ctypes.sizeof(_lib.ResidualNorm) == blocks._DESCRIPTOR_HEAD.size + blocks._DESCRIPTOR_TAIL.size
+  d = _lib.ResidualNorm.from_buffer_copy(blocks._DESCRIPTOR.pack(*range(1, n + 1)))
+  flat = []
+  for name, _ in _lib.ResidualNorm._fields_:
+    v = getattr(d, name)
+    flat += [v.p, v.pitch] if isinstance(v, _lib.Rows) else [v]
+  assert flat == list(range(1, n + 1))
+
+
 def test_dropout_entry_refuses(lib):
   ok = dict(x=16, xp=8, y=16, yp=8, rows=2, cols=8, dtype=0, keep=0.5, seed=0, offset=0, dev=None)
 

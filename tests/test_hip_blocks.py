@@ -231,13 +231,25 @@ def test_norm_repeats_bit_for_bit_and_takes_buffers(blocks):
   assert r2 is x and torch.equal(x, r) and torch.equal(z2, z) and bool((wide[..., 513:] == 3).all())
 
 
+def descriptor(norm, r, gate, call):
+  """The C entries' struct for float32 rows, with everything but the tensors that a test binds itself."""
+  from advoc_amd import _lib
+  rows, ptr = r.numel() // norm.cols, lambda t: None if t is None else t.data_ptr()      # noqa: E731
+  q = _lib.ResidualNorm(rows, norm.cols, 0, 0, norm.post, norm.pre, norm.gate_act, 1 if gate is None else rows // (gate.numel() // norm.cols),
+                        ptr(norm.w_post), ptr(norm.b_post), ptr(norm.scale), ptr(norm.w_pre), ptr(norm.b_pre), norm.alpha, norm.eps,
+                        norm.keep_prob, 0, call['seed'], call['offset'])
+  for name, t in (('r', r), ('gate', gate)):
+    getattr(q, name).p, getattr(q, name).pitch = ptr(t), norm.cols
+  return q
+
+
 @pytest.mark.parametrize('cols', [40, 513, 2500])
 def test_norm_backward_in_place(blocks, cols):
   """dx over dr and dh over h through the C entry, ragged rows included."""
   import ctypes
   from advoc_amd import _lib
   norm, d, call, g, (r, z, stats) = check_norm(blocks, 6, (2, 9), cols, 'f32', 'f32', *KINDS[0])
-  q, rows, _ = norm._descriptor(r, 'r', torch.float32, None, call['seed'], call['offset'], None, True)
+  q = descriptor(norm, r, None, call)
   h, dr = d['h'].clone(), d['dr'].clone()
   for name, t in (('dz', d['dz']), ('dr', dr), ('dx', dr), ('h', h), ('dh', h)):
     getattr(q, name).p, getattr(q, name).pitch = t.data_ptr(), cols
@@ -254,7 +266,7 @@ def test_norm_every_output_over_an_input(blocks, lead, cols):
   from advoc_amd import _lib
   norm, d, call, g, (r, z, stats) = check_norm(blocks, 8, lead, cols, 'f32', 'f32', 'rms', 'layer', 'clip', 'sigmoid', 0.9)
   h, dr, gate = d['h'].clone(), d['dr'].clone(), d['gate'].clone()
-  q, rows, _ = norm._descriptor(r, 'r', torch.float32, gate, call['seed'], call['offset'], None, True)
+  q = descriptor(norm, r, gate, call)
   for name, t in (('dz', d['dz']), ('dr', dr), ('dx', dr), ('h', h), ('dh', h), ('dgate', gate)):
     getattr(q, name).p, getattr(q, name).pitch = t.data_ptr(), cols
   sums = {k: torch.full((cols,), float('nan'), device='cuda') for k in ('dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre')}
@@ -313,7 +325,8 @@ def test_norm_of_kind_none_takes_no_weight_or_bias(blocks):
   import ctypes
   from advoc_amd import _lib
   norm, d, call, g, (r, z, stats) = check_norm(blocks, 9, (2, 7), 72, 'f32', 'f32', 'none', 'none', 'row', 'none', 0.9)
-  q, rows, _ = norm._descriptor(d['x'], 'x', torch.float32, d['gate'], call['seed'], call['offset'], None, True)
+  q = descriptor(norm, r, d['gate'], call)
+  q.x.p, q.x.pitch = d['x'].data_ptr(), 72
   wrong = torch.full((72,), 7.0, device='cuda')
   q.w_post = q.b_post = q.w_pre = q.b_pre = wrong.data_ptr()
   out = {k: torch.empty_like(r) for k in ('r', 'dh', 'dx', 'dgate')}
