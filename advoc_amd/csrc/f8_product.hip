@@ -91,6 +91,13 @@ template <typename O, int C>
 __device__ __forceinline__ void store_part(const Args& g, int64_t row, int64_t col, const float (&v)[C]) {
   if (row >= g.m) return;
   O* p = (O*)g.out + row * g.n + col;
+  if (!g.accumulate && col + C <= g.n) {
+    O o[C];
+#pragma unroll
+    for (int k = 0; k < C; ++k) o[k] = (O)v[k];
+    __builtin_memcpy(p, o, sizeof(o));
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < C; ++k)
     if (col + k < g.n) p[k] = (O)((g.accumulate ? (float)p[k] : 0.f) + v[k]);
@@ -214,7 +221,7 @@ struct Tile {
   static_assert(kFn % kRun == 0, "whole runs");
   static_assert(kDma * 8 * kWaves == kRows && BM % (8 * kWaves) == 0, "whole DMA instructions per wave and operand");
   static_assert(8 * kWaves % 32 == 0, "the keys of the rows that a lane fetches repeat");
-  static_assert(BM % 64 == 0 && BN % 64 == 0 && kWaves % (kRows / 64) == 0, "64 rows of one operand per wave's exponent fetch");
+  static_assert(BM % 64 == 0 && BN % 64 == 0 && kWaves >= kRows / 64, "64 rows of one operand per wave's exponent fetch");
 
   advoc::u32x4s ra, rb, rea, reb;
   const uint8_t* lds;
@@ -329,10 +336,10 @@ struct Place {
   }
 };
 
-// 128 x 128 EXACT, 1024 x 1024 x 16384 in four parts: 37 us and 5 for adding these up, 4096 x 4096 x 4096 137 us = 1.0 PFLOP/s (a
-// library product of bf16 matrices reaches 1.4).  A block takes a CU 1.1 us: with the matrix instructions and conversions left out 0.66
-// to 1.0 (DMA into LDS and fragments out of it), with only the conversions left out 1.0; conversions dealt between the matrix
-// instructions, and wave tiles of 64 x 64, measured the same.
+// EXACT, 4096 x 4096 x 4096: 127 us, 1.08 PFLOP/s in tiles of 256 x 128, 142 in tiles of 128 x 128 (a library product of bf16 matrices
+// of 8192 reaches 1.41); 1024 x 1024 x 16384: 40 us and 5 for adding up its parts.  A block of 128 x 128 takes a CU 1.1 us: with the
+// matrix instructions and conversions left out 0.66 to 1.0 (DMA into LDS and fragments out of it), with only the conversions left out
+// 1.0; conversions dealt between the matrix instructions, and wave tiles of 64 x 64 in the same tile, measured the same.
 template <typename O, bool EXACT, int FA, int FB, int BM, int BN, int WM, int WN, int S, bool SPLIT>
 __global__ __launch_bounds__(BM / WM * (BN / WN) * 64) void f8_tile_kernel(Args g) {
   using T = Tile<O, BM, BN, WM, WN, S>;
@@ -503,35 +510,38 @@ __global__ __launch_bounds__(256) void f8_fold_kernel(const float* __restrict__ 
   }
 }
 
-enum { kDot, kThin, kTile64, kTile128, kTile256 };
+enum { kDot, kThin, kTile64, kTile128, kTile256 };      // kTile256: 256 x 256, EXACT 256 x 128
 
 struct Plan {
   int form, splits, per_split;
 };
 
 // One or two rows: dot products (2 x 4096 x 4096: 5.7 us, thin 6.5; 2 x 16384 x 4096: 17.7, thin 17.0).  Otherwise the cheapest
-// estimate.  A CU takes 0.75 us for a block of 128 x 128 outputs (1.2 EXACT), 0.4 (0.35) times that for one of
-// 64 x 64 and twice for one of 256 x 256, whichever its neighbours do; the CUs take tiles in rounds of 256.  A contraction split in s
-// has s times the tiles with 1 / s of the blocks, and 3 us and a write and a read of its partial results more.
-// The thin kernel takes 0.08 us and 4.2 ns a row for a block of 16 columns, 256 of them together.
-// Measured, in us (64 | 128 | 256, 16-bit outputs):  1024 x 1024 x 1024: 5.5 | 8.1;  2048 x 1024 x 4096: 19 | 25 | 48;  2048 x 2048 x
+// estimate.  A CU takes 0.7 us for a block of 128 x 128 outputs (EXACT 1.06), 0.4 times that for one of 64 x 64 (EXACT 0.36), twice
+// for one of 256 x 256 (EXACT 1.56 times for one of 256 x 128), whichever its neighbours do, and four blocks' time to begin and end a
+// tile; the CUs take tiles in rounds of 256.  A contraction split in s has s times the tiles with 1 / s of the blocks, and 3 us and a write and a read of its partial results more.
+// The thin kernel (up to 16 rows) takes 0.08 us and 4.2 ns a row for a block of 16 columns, 256 of them together.
+// Measured, in us.  64 | 128 | 256, 16-bit outputs:  1024 x 1024 x 1024: 5.5 | 8.1;  2048 x 1024 x 4096: 19 | 25 | 48;  2048 x 2048 x
 // 4096: 33 | 24 | 48;  4096 x 2048 x 4096: 63 | 47 | 50;  4096 x 2560 x 4096: 128: 68, 256: 52;  16384 x 1024 x 1024: 39 | 31 | 21.
+// 128 x 128 | 256 x 128, fp32 outputs:  4096 x 4096 x 4096: 142 | 127;  16384 x 4096 x 4096: 550 | 458;  2048 x 2048 x 4096: 36 | 48;
+// 1024 x 1024 x 16384 in 4 | 8 parts: 48 | 46.
 // fp32 outputs in 1 | 2 | 4 | 8 parts:  1024 x 1024 x 16384: 112 | 65 | 43 | 50 (128), 57 | 47 | 49 (64);  512 x 512 x 2048: 9.1 |
 // 9.1 | 8.6 | 11.6 (64).
-// Thin | 64 in parts:  16 x 512 x 8192: 12.7 | 9.3;  16 x 4096 x 4096: 8.0 | 9.3;  16 x 1000 x 1000: 3.7 |
-// 5.2;  with 17 to 64 rows the thin form lost nearly everywhere (64 x 512 x 8192: 28.8 | 9.8).
+// Thin | 64 in parts:  16 x 512 x 8192: 12.7 | 9.3;  16 x 4096 x 4096: 8.0 | 9.3;  16 x 1000 x 1000: 3.7 | 5.2;  with 17 to 64 rows
+// the thin form lost nearly everywhere (64 x 512 x 8192: 28.8 | 9.8).
 Plan make_plan(int64_t m, int64_t n, int blocks, bool exact) {
   Plan p = {m <= 2 ? kDot : kThin, 1, blocks};
   if (m <= 2) return p;
-  const double block_us = exact ? 1.2 : 0.75, fold_us = 8.0 * m * n / 5e6;
+  const double block_us = exact ? 1.06 : 0.7, fold_us = 8.0 * m * n / 5e6;
   double best = m <= 16 ? (0.08 + 0.0042 * m) * blocks * ceil_div(n, 16 * 256) : 1e30;
-  for (int form = kTile64; form <= (exact ? kTile128 : kTile256); ++form) {
-    const int64_t side = form == kTile64 ? 64 : form == kTile128 ? 128 : 256;
-    const int64_t tiles = ceil_div(m, side) * ceil_div(n, side);
-    const double cost = block_us * (form == kTile64 ? exact ? 0.35 : 0.4 : form == kTile128 ? 1.0 : 2.0);
-    for (int s = 1; s == 1 || (form != kTile256 && s <= 16 && s <= blocks / 8); s *= 2) {
+  const int64_t sides[] = {64, 128, 256}, wide = exact ? 128 : 256;      // the largest tile: 256 x wide
+  const double costs[] = {exact ? 0.36 : 0.4, 1.0, exact ? 1.56 : 2.0};
+  for (int form = kTile64; form <= kTile256; ++form) {
+    const int64_t side = sides[form - kTile64], tiles = ceil_div(m, side) * ceil_div(n, form == kTile256 ? wide : side);
+    const int most = form == kTile256 && !exact ? 1 : 16;
+    for (int s = 1; s == 1 || (s <= most && s <= blocks / 8); s *= 2) {
       const int per = (int)ceil_div(blocks, s), parts = (int)ceil_div(blocks, per);
-      const double us = cost * ceil_div(tiles * parts, 256) * per + (parts > 1 ? 3.0 + fold_us * parts : 0.0);
+      const double us = block_us * costs[form - kTile64] * ceil_div(tiles * parts, 256) * (per + 4) + (parts > 1 ? 3.0 + fold_us * parts : 0.0);
       if (us < best) best = us, p = {form, parts, per};
     }
   }
@@ -545,6 +555,14 @@ int run_tile(const Args& g, int splits, hipStream_t stream) {
   hipLaunchKernelGGL((f8_tile_kernel<O, EXACT, FA, FB, BM, BN, WM, WN, S, SPLIT>), grid, dim3(kThreads), 0, stream, g);
   ADVOC_RETURN_IF_LAUNCH_FAILED();
   return ADVOC_OK;
+}
+
+template <typename O, bool EXACT, int FA, int FB, bool SPLIT>
+int run_form(const Args& g, const Plan& p, hipStream_t stream) {
+  if constexpr (EXACT)
+    if (p.form == kTile256) return run_tile<O, EXACT, FA, FB, 256, 128, 64, 64, 3, SPLIT>(g, p.splits, stream);
+  return p.form == kTile128 ? run_tile<O, EXACT, FA, FB, 128, 128, 64, 32, 4, SPLIT>(g, p.splits, stream)
+                            : run_tile<O, EXACT, FA, FB, 64, 64, 32, 32, 4, SPLIT>(g, p.splits, stream);
 }
 
 template <typename O, bool EXACT, int FA, int FB>
@@ -571,12 +589,8 @@ int run(const Args& g, const Plan& p, hipStream_t stream) {
       return ADVOC_OK;
     }
   }
-  if (p.splits == 1)
-    return p.form == kTile128 ? run_tile<O, EXACT, FA, FB, 128, 128, 64, 32, 4, false>(g, 1, stream)
-                              : run_tile<O, EXACT, FA, FB, 64, 64, 32, 32, 4, false>(g, 1, stream);
-  const int rc = p.form == kTile128 ? run_tile<float, EXACT, FA, FB, 128, 128, 64, 32, 4, true>(g, p.splits, stream)
-                                    : run_tile<float, EXACT, FA, FB, 64, 64, 32, 32, 4, true>(g, p.splits, stream);
-  if (rc != ADVOC_OK) return rc;
+  const int rc = p.splits == 1 ? run_form<O, EXACT, FA, FB, false>(g, p, stream) : run_form<float, EXACT, FA, FB, true>(g, p, stream);
+  if (rc != ADVOC_OK || p.splits == 1) return rc;
   const int64_t count = g.m * g.n, blocks = ceil_div(count, 256);
   ADVOC_CLEAR_LAUNCH_ERROR();
   hipLaunchKernelGGL(f8_fold_kernel<O>, dim3((unsigned)(blocks > 4096 ? 4096 : blocks)), dim3(256), 0, stream, g.part, (O*)g.out, count,

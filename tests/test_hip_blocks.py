@@ -449,7 +449,7 @@ def ints(rows, k, seed):
 
 SHAPES = [(1, 1, 1), (1, 512, 8192), (1, 17, 100), (2, 1, 9000), (2, 513, 1025), (3, 50, 1300), (16, 16, 128), (17, 15, 129), (33, 513, 1000), (64, 10240, 100), (64, 100, 2000),
           (65, 64, 128), (65, 1, 300), (100, 70, 513), (128, 128, 256), (129, 130, 1000), (300, 257, 1100), (1285, 513, 1000), (700, 600, 640),
-          (200, 300, 5000), (1100, 1200, 4096), (4100, 4099, 200), (70, 16000, 130)]
+          (200, 300, 5000), (1100, 1200, 4096), (4100, 4099, 200), (70, 16000, 130), (1000, 1100, 12000)]
 
 
 @pytest.mark.parametrize('m,n,k', SHAPES)
