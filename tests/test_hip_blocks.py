@@ -208,6 +208,21 @@ def test_norm_many_rows(blocks):
   check_norm(blocks, 2, (3, 5001), 16, 'bf16', 'bf16', *KINDS[3])
 
 
+def test_norm_past_32_bits(blocks):
+  """Elements past 2^32: the last rows of a call are those of a call of these rows at their offset, both ways."""
+  rows, cols, tail = 2 ** 20 + 5, 4200, 3
+  h, x = (torch.empty(rows, cols, dtype=torch.bfloat16, device='cuda').normal_() for _ in range(2))
+  vec = [torch.rand(cols, generator=gen(i)).cuda() for i in range(3)]
+  norm = blocks.ResidualNorm(cols, post='rms', pre='layer', w_post=vec[0], scale=vec[1], w_pre=vec[2], keep_prob=0.9)
+  r, z, stats = norm.forward(h, x, seed=3, save=True)
+  last = dict(seed=3, offset=(rows - tail) * cols)
+  r2, z2, stats2 = norm.forward(h[-tail:], x[-tail:], save=True, **last)
+  assert torch.equal(r[-tail:], r2) and torch.equal(z[-tail:], z2) and torch.equal(stats[-tail:], stats2)
+  g = norm.backward(z, x, h, r, stats, seed=3)
+  g2 = norm.backward(z2, x[-tail:], h[-tail:], r2, stats2, **last)
+  assert torch.equal(g.dh[-tail:], g2.dh) and torch.equal(g.dx[-tail:], g2.dx)
+
+
 def test_norm_repeats_bit_for_bit_and_takes_buffers(blocks):
   norm, d, call, g, (r, z, stats) = check_norm(blocks, 5, (4, 300), 513, 'bf16', 'f32', *KINDS[1])
   again = norm.backward(d['dz'], d['dr'], d['h'], r, stats, **call)
@@ -417,6 +432,17 @@ def test_quantize_is_exact(blocks, fmt, dt, rows, cols, pad):
     want, e = O.f8_blocks(ref, fmt)
     got, s = values(q, fmt)
     assert torch.equal(s, e) and torch.equal(got, want)
+
+
+def test_quantize_past_32_bits(blocks):
+  rows, cols, start = 2 ** 20 + 130, 4220, 2 ** 20
+  x = torch.empty(rows, cols, dtype=torch.bfloat16, device='cuda').normal_()
+  a, t = blocks.quantize_f8_both(x)
+  b, u = blocks.quantize_f8_both(x[start:])
+  assert torch.equal(a.data[start:], b.data) and torch.equal(a.scale[start:], b.scale)
+  assert torch.equal(t.data[:, start:], u.data) and torch.equal(t.scale[:, start // 128:start // 128 + 2], u.scale[:, :2])
+  only = blocks.quantize_f8(x)
+  assert torch.equal(only.data[start:], b.data) and torch.equal(only.scale[start:], b.scale)
 
 
 @pytest.mark.parametrize('fmt', ['e4m3', 'e5m2'])
