@@ -34,7 +34,8 @@ struct NormArgs {
   void *dh, *dx, *dgate;
   int64_t dh_pitch, dx_pitch, dgate_pitch;
   float* part;                  // [sum][workgroup][cols]
-  float* gate_part;             // [gate row][splits][cols], NULL: a gate row's sum is complete in one worker
+  float* gate_part;             // [gate row][entries][cols], NULL: a gate row's sum is complete in one worker
+  int gate_blocks;              // an entry is a workgroup's: its rows have one segment each, all of one gate row; 0: a segment's
   float* carry;                 // per worker, where workers see several gate rows: see residual_norm_bwd.hip
   int64_t segments;
   int splits;                   // segments of a gate row

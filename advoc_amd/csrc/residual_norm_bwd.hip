@@ -13,8 +13,8 @@
 // same way, a worker's rows never crossing a clip: G0 = sum e, G1 = sum e hhat over them give dgate = scale (w_post G1 + b_post G0)
 // act' and their part of E0, E1.
 //
-// Measured (kernel + the second launch): 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (302 MB): 69 + 6 us, 4.4
-// TB/s; each further row comes at 5.0 TB/s, a copy's rate, and 12 us are the way of the first row (arguments and vectors 4, loads 2,
+// Measured (kernel + the second launch): 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (302 MB): 67 + 5 us, 4.5
+// TB/s (69 + 6 when every worker of a clip left its part of the gate's gradient in memory, not every workgroup); each further row comes at 5.0 TB/s, a copy's rate, and 12 us are the way of the first row (arguments and vectors 4, loads 2,
 // arithmetic 4, the workgroup's column sums 3).  4096 x 4096 fp16 (201 MB, and 25 MB of column sums): 51 + 5.  3999 x 513 fp32 (66
 // MB): 21 + 4, two rows a worker: the same start, and the arithmetic.
 #include "residual_norm.h"
@@ -38,9 +38,9 @@ constexpr int kWavesPerSimd = 2;
 template <int L, int NV>
 constexpr int kLanes = L > 64 ? L : NV > 1 ? 512 : 256;
 
-// Column sums that go through LDS together at the end of a workgroup: 40 KB with two workgroups to a CU, 128 KB with one.
+// Sums that go through LDS together at the end of a workgroup: up to 55 KB with two workgroups to a CU, 128 KB with one.
 template <int NV>
-constexpr int kSumsTogether = NV > 1 ? 4 : 5;
+constexpr int kSumsTogether = NV > 1 ? 4 : 6;
 
 // t <- the gradient of a row given that of its normed values (times the weight): rstd (t - [mean t] - hat mean(t hat))
 template <int V, int L, int NV, int WG>
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
 #pragma unroll
         for (int j = 0; j < NV; ++j) advoc::store_chunk<V>(advoc::row_at<T>(a.dh, row * a.dh_pitch, col[j]), t[j]);
     }
-    if (H && shared_gate) {
+    if (H && shared_gate && !a.gate_blocks) {
       raw_gate.load(gate_base, group * gate_pitch, col);
       if constexpr (L > 64) {
         raw_gate.arrived();
@@ -224,7 +224,28 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
   }
 
   // the workgroup's column sums: values of a column with two holders are equal, so either may store them
-  Vals<V> out[kSums][NV];
+  constexpr int kGate = kSums, kAll = H && L <= 64 ? kSums + 1 : kSums;
+  Vals<V> out[kAll][NV];
+  if constexpr (kAll > kSums) {
+    if (a.gate_blocks) {
+      const int group = ((int)blockIdx.x * Row::kRows + Row::slot()) / a.splits;
+      advoc::Raw<T, V, NV> raw_gate;
+      raw_gate.load(gate_base, group * gate_pitch, col);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        Vals<V> gate = raw_gate[j];
+        advoc::activate<V>(gate, a.act);
+        out[kGate][j] = scale(j) * (w_post(j) * g1[j] + b_post(j) * g0[j]);
+        if (a.act == ADVOC_GATE_SIGMOID) out[kGate][j] *= gate * (Vals<V>(1.f) - gate);
+        g0[j] *= gate;
+        g1[j] *= gate;
+      }
+    }
+  }
+  auto wanted = [&](int s) { return s < kSums ? sums.slot[s] >= 0 : a.gate_blocks != 0; };
+  auto entry = [&](int s) {
+    return (s < kSums ? a.part + (int64_t)sums.slot[s] * gridDim.x * cols : a.gate_part) + (int64_t)blockIdx.x * cols;
+  };
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     out[kDwPost][j] = scale(j) * g1[j];
@@ -236,27 +257,26 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
   if constexpr (L > 64) {
 #pragma unroll
     for (int s = 0; s < kSums; ++s)
-      if (sums.slot[s] >= 0)
+      if (wanted(s))
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-          advoc::store_chunk<V>(a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * cols + col[j], out[s][j]);
+        for (int j = 0; j < NV; ++j) advoc::store_chunk<V>(entry(s) + col[j], out[s][j]);
   } else {
     // kTogether sums at a time: [sum][row of the workgroup] in LDS
     constexpr int kTogether = kSumsTogether<NV>;
 #pragma unroll
-    for (int first = 0; first < kSums; first += kTogether) {
+    for (int first = 0; first < kAll; first += kTogether) {
       __syncthreads();
 #pragma unroll
-      for (int s = first; s < kSums && s < first + kTogether; ++s)
-        if (sums.slot[s] >= 0)
+      for (int s = first; s < kAll && s < first + kTogether; ++s)
+        if (wanted(s))
 #pragma unroll
           for (int j = 0; j < NV; ++j) chunks.put(vec + ((s - first) * Row::kRows + Row::slot()) * floats, chunk[j], out[s][j]);
       __syncthreads();
       chunks.template walk<WG>([&](int at, int c, auto n) {
         constexpr int kPiece = decltype(n)::value;
 #pragma unroll
-        for (int s = first; s < kSums && s < first + kTogether; ++s) {
-          if (sums.slot[s] < 0) continue;
+        for (int s = first; s < kAll && s < first + kTogether; ++s) {
+          if (!wanted(s)) continue;
           const float* from = vec + (s - first) * Row::kRows * floats + at;
           float v[kPiece];
 #pragma unroll
@@ -267,7 +287,7 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
 #pragma unroll
             for (int k = 0; k < kPiece; ++k) v[k] += x[k];
           }
-          __builtin_memcpy(a.part + ((int64_t)sums.slot[s] * gridDim.x + blockIdx.x) * cols + c, v, sizeof(v));
+          __builtin_memcpy(entry(s) + c, v, sizeof(v));
         }
       });
     }
@@ -319,8 +339,8 @@ __global__ __launch_bounds__(1024) void norm_fold_kernel(FoldArgs a) {
 // How the rows are cut: workgroups, and for a shared gate how many workers share a gate row.
 struct Plan {
   int64_t blocks = 0, segments = 0;
-  int splits = 0, sums = 0;
-  bool gate_fold = false;
+  int splits = 0, sums = 0, gate_entries = 0;
+  bool gate_fold = false, gate_blocks = false;
   int64_t part_floats = 0, gate_floats = 0, carry_floats = 0;
 };
 
@@ -337,6 +357,9 @@ struct MakePlan {
     int64_t splits = most * kRows / groups;
     if (splits > rows) splits = rows;
     if (splits < 1) splits = 1;
+    // whole workgroups to a gate row, where that makes no worker's share longer: its gradient then meets in LDS first
+    const int64_t whole = L <= 64 ? splits - splits % kRows : 0;
+    if (shared_gate && whole > 0 && advoc::ceil_div(rows, whole) == advoc::ceil_div(rows, splits)) splits = whole;
     p.splits = (int)splits;
     p.segments = groups * p.splits;
     p.blocks = advoc::ceil_div(p.segments, kRows);
@@ -344,7 +367,9 @@ struct MakePlan {
     for (int s = 0; s < kSums; ++s) p.sums += sums.slot[s] >= 0;
     p.gate_fold = shared_gate && a.dgate && p.splits > 1;
     p.part_floats = p.sums * p.blocks * a.cols;
-    p.gate_floats = p.gate_fold ? p.segments * a.cols : 0;
+    p.gate_blocks = p.gate_fold && L <= 64 && p.splits % kRows == 0;
+    p.gate_entries = p.gate_blocks ? p.splits / kRows : p.splits;
+    p.gate_floats = p.gate_fold ? groups * p.gate_entries * a.cols : 0;
     if (shared_gate && p.segments > p.blocks * kRows) p.carry_floats = p.blocks * kRows * 2 * NV * L * V;
   }
 };
@@ -399,6 +424,7 @@ int launch_norm_backward(NormArgs a, int dtype, int res_dtype, float* const (&ou
   a.part = (float*)workspace;
   a.gate_part = p.gate_fold ? (float*)workspace + p.part_floats : nullptr;
   a.carry = p.carry_floats ? (float*)workspace + p.part_floats + p.gate_floats : nullptr;
+  a.gate_blocks = p.gate_blocks;
   a.segments = p.segments;
   a.splits = p.splits;
   ADVOC_CLEAR_LAUNCH_ERROR();
@@ -422,7 +448,7 @@ int launch_norm_backward(NormArgs a, int dtype, int res_dtype, float* const (&ou
   f.col_blocks = (int)ceil_div(a.cols, 64);
   f.sums = p.sums;
   f.entries = (int)p.blocks;
-  f.splits = p.splits;
+  f.splits = p.gate_entries;
   f.accumulate = accumulate;
   const int64_t items = p.sums + (p.gate_fold ? a.rows / a.gate_group : 0);
   const dim3 grid((unsigned)(items * f.col_blocks));

@@ -204,6 +204,14 @@ def test_norm_more_clips_than_workers(blocks, lead, cols):
   check_norm(blocks, 3, lead, cols, 'bf16', 'bf16', *KINDS[1])
 
 
+@pytest.mark.parametrize('kind', [1, 3])
+@pytest.mark.parametrize('lead,cols', [((3, 64), 7), ((3, 64), 100), ((3, 64), 200), ((3, 64), 300), ((3, 64), 520), ((3, 64), 1000), ((64, 40), 1000),
+                                       ((3, 65), 520)])
+def test_norm_clips_cut_into_whole_workgroups(blocks, lead, cols, kind):
+  """A gate row's gradient that meets in a workgroup before it leaves, and (65 frames) one that cannot."""
+  check_norm(blocks, 4, lead, cols, 'bf16', 'f32', *KINDS[kind])
+
+
 def test_norm_many_rows(blocks):
   check_norm(blocks, 2, (3, 5001), 16, 'bf16', 'bf16', *KINDS[3])
 
@@ -274,7 +282,7 @@ def test_norm_backward_in_place(blocks, cols):
   assert torch.equal(dr, g.dx) and torch.equal(h, g.dh)
 
 
-@pytest.mark.parametrize('lead,cols', [((600, 2), 1032), ((300, 3), 2056), ((9, 40), 1544), ((2200, 1), 700), ((3, 70), 80)])
+@pytest.mark.parametrize('lead,cols', [((600, 2), 1032), ((300, 3), 2056), ((9, 40), 1544), ((2200, 1), 700), ((3, 70), 80), ((3, 64), 1000)])
 def test_norm_every_output_over_an_input(blocks, lead, cols):
   """dx over dr, dh over h and dgate over a gate per clip: whole clips to a worker and clips cut up, waves that hold the same columns."""
   import ctypes
