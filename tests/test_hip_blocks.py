@@ -4,8 +4,9 @@ Tolerances, from the arithmetic alone.  u = 2^-24 is half a step of fp32; half a
   * a row's sum is at most 16 terms in a lane, 6 exchanges and 8 waves: 30 roundings; two sums per norm, two norms, and under 100
     roundings of single operations around them (the sigmoid's exponential counts 4): a row output is within 256 u of the largest
     term of its row, before its own rounding;
-  * a column sum adds a worker's rows, the workers of a workgroup (at most 16) and a quarter of the workgroups (at most 128) in turn:
-    within (rows / workers + 160 + 256) u of the sum of the terms' magnitudes -- rows are few here, so `rows` itself is taken;
+  * a column sum adds a worker's rows, the workers of a workgroup (at most 32), a sixteenth of the workgroups (at most 32) and these
+    16 in turn, under 160 roundings: within (rows / workers + 160 + 256) u of the sum of the terms' magnitudes -- rows are few here,
+    so `rows` itself is taken;
   * an 8-bit product passes at most 128 additions inside an instruction, one per block of 128, and 16 + 64 where waves or splits
     meet: within (208 + k / 128) u of sum |a b|.  For 16-bit outputs the instruction also drops, of each of eight neighbouring
     products, what is below 2^-13 of the largest of them: under 8 2^-13 of that one, so 2^-10 of sum |a b| in all;
