@@ -170,20 +170,25 @@ __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_backward_kernel(NormAr
         advoc::draw_chunk<V>(words, a.key.offset + (uint64_t)(row * cols + col[j]), aligned, key, a.key.thresh);
         advoc::activate<V>(gate[j], a.act);
         const Vals<V> s = scale(j);
+        // What is dropped has no gradient and is no part of a sum, whatever its h and gate hold: 0 times an infinity or a NaN would be
+        // one, so both are replaced (norm_back below takes hat as it is: there a NaN is its row's).
+        Vals<V> hat_kept;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          gate[j][k] = has_gate ? gate[j][k] : 1.f;
-          t[j][k] = words[k] >= a.key.thresh ? g[j][k] * kept : 0.f;
+          const bool stays = words[k] >= a.key.thresh;
+          gate[j][k] = has_gate && stays ? gate[j][k] : 1.f;
+          hat_kept[k] = stays ? hat[j][k] : 0.f;
+          t[j][k] = stays ? g[j][k] * kept : 0.f;
         }
         if (row_gate && a.dgate) {
-          Vals<V> dg = t[j] * s * (hat[j] * w_post(j) + b_post(j));
+          Vals<V> dg = t[j] * s * (hat_kept * w_post(j) + b_post(j));
           if (a.act == ADVOC_GATE_SIGMOID) dg *= gate[j] * (Vals<V>(1.f) - gate[j]);
           advoc::store_chunk<V>(advoc::row_at<T>(a.dgate, row * a.dgate_pitch, col[j]), dg);
         }
         const Vals<V> e = t[j] * gate[j];
         Vals<V> sum = shared_gate ? t[j] : e;
         g0[j] += sum;
-        g1[j] += sum * hat[j];
+        g1[j] += sum * hat_kept;
         t[j] = e * s * w_post(j);               // (w_post is staged as ones without a post norm)
       }
       if (post) norm_back<V, L, NV, WG>(t, hat, dup, ragged, a.post, a.inv_cols, st.y, red, turn);

@@ -590,7 +590,8 @@ typedef struct advoc_rows {
  *        aligned): written by the forward pass when not NULL, read by the backward pass
  * z and the statistics are those of r BEFORE it is rounded to res_dtype.
  * An output may be the buffer of an input of the same type, rows and pitch (r over x, dx over dr, dh over h ...).
- * A row of zeros gives zeros (plus the bias).  A NaN or infinity stays in its row. */
+ * A row of zeros gives zeros (plus the bias).  A NaN or infinity stays in its row, and where it is dropped it adds nothing to r,
+ * to the gradient of its gate or to a column sum. */
 typedef struct advoc_residual_norm {
   int64_t rows;
   int32_t cols;

@@ -34,6 +34,11 @@ def norm_stats(a, kind, eps):
   return mean, 1 / torch.sqrt((a - mean).square().mean(-1, keepdim=True) + eps)
 
 
+def drop(v, mask, keep):
+  """What is dropped is 0 whatever it held."""
+  return v if mask is None else torch.where(mask, v / float(np.float32(keep)), torch.zeros((), dtype=v.dtype))
+
+
 def gate_act(gate, act):
   return torch.sigmoid(gate) if act == 'sigmoid' else gate
 
@@ -42,13 +47,12 @@ def residual_norm(h, x, gate=None, post='rms', pre='rms', act='none', alpha=1.0,
                   b_post=None, scale=None, w_pre=None, b_pre=None):
   """dict(r, z, stats) in the inputs' precision (float64).  mask: keep_mask of h's shape, or None."""
   one = torch.ones((), dtype=x.dtype)
-  factor = one if mask is None else mask.to(x.dtype) / float(np.float32(keep))
   r = x
   mean0 = rstd0 = torch.zeros_like(x[..., :1])
   if h is not None:
     mean0, rstd0 = norm_stats(h, post, eps)
     u = h if post == 'none' else (h - mean0) * rstd0 * (one if w_post is None else w_post) + (0 if b_post is None else b_post)
-    r = x + alpha * (one if scale is None else scale) * (one if gate is None else gate_act(gate, act)) * (u * factor)
+    r = x + alpha * (one if scale is None else scale) * (one if gate is None else gate_act(gate, act)) * drop(u, mask, keep)
   mean1, rstd1 = norm_stats(r, pre, eps)
   z = None if pre == 'none' else (r - mean1) * rstd1 * (one if w_pre is None else w_pre) + (0 if b_pre is None else b_pre)
   return dict(r=r, z=z, stats=torch.cat([mean0, rstd0, mean1, rstd1], -1).reshape(-1, 4))
@@ -86,11 +90,10 @@ def residual_norm_backward(dz, dr, h, r, stats, gate=None, post='rms', pre='rms'
   if h is None:
     return out, size
   gbig = size['dx']
-  factor = one if mask is None else mask.to(r.dtype) / float(np.float32(keep))
   hat = h if post == 'none' else (h - m0) * s0
-  v = factor * (h if post == 'none' else hat * (one if w_post is None else w_post) + (0 if b_post is None else b_post))
+  v = drop(h if post == 'none' else hat * (one if w_post is None else w_post) + (0 if b_post is None else b_post), mask, keep)
   hbig = (h.abs() + (0 if post == 'none' else m0.abs())) * (1 if post == 'none' else s0)
-  vbig = factor * (hbig * (one if w_post is None else w_post.abs()) + (0 if b_post is None else b_post.abs()))
+  vbig = drop(hbig * (one if w_post is None else w_post.abs()) + (0 if b_post is None else b_post.abs()), mask, keep)
   gt = one if gate is None else gate_act(gate, act)
   k = alpha * (one if scale is None else scale)
   colsum('dscale', alpha * g * gt * v)
@@ -103,10 +106,10 @@ def residual_norm_backward(dz, dr, h, r, stats, gate=None, post='rms', pre='rms'
       if gate.shape[d] == 1 and dg.shape[d] > 1:
         dg, dgb = dg.sum(d, keepdim=True), dgb.sum(d, keepdim=True)
     out['dgate'], size['dgate'] = dg, dgb
-  du = factor * k * gt * g
-  dub = factor * (k * gt).abs() * gbig
+  du = drop((k * gt * g).expand_as(h), mask, keep)
+  dub = drop(((k * gt).abs() * gbig).expand_as(h), mask, keep)
   if post != 'none':
-    colsum('dw_post', du * hat)
+    colsum('dw_post', du * (hat if mask is None else torch.where(mask, hat, torch.zeros((), dtype=hat.dtype))))
     colsum('db_post', du)
     size['dw_post'] = (dub * hbig).expand_as(du).reshape(-1, c).sum(0)
     size['db_post'] = dub.expand_as(du).reshape(-1, c).sum(0)

@@ -1,0 +1,89 @@
+"""GPU tests of advoc_amd.blocks where a call meets what it should not let through: values that are no numbers at places that are
+dropped, empty calls, outputs of other shapes and types, and the ends of the exponent range.  Expected values are exact (the same
+bits as a call without the bad value, or whole numbers and powers of two), but for where a tolerance is derived beside it."""
+import ctypes
+
+import pytest
+import torch
+
+from oracle import blocks_torch as O
+
+pytestmark = pytest.mark.gpu
+BAD = [float('inf'), -float('inf'), float('nan')]
+COLS = [5, 40, 96, 200, 513, 1000, 2048, 4100]      # every way a row lies on lanes
+
+
+@pytest.fixture(scope='module')
+def blocks():
+  from advoc_amd import _lib, blocks
+  assert torch.cuda.is_available(), 'gpu-marked test running without a HIP device'
+  _lib.load()
+  return blocks
+
+
+def gen(seed):
+  return torch.Generator().manual_seed(seed)
+
+
+# ---- values that are no numbers where an element is dropped ----
+@pytest.mark.parametrize('gates', ['none', 'row', 'clip'])
+@pytest.mark.parametrize('cols', COLS)
+def test_a_dropped_value_that_is_no_number_adds_nothing_to_gradients(blocks, cols, gates):
+  """Without a post norm an infinity or NaN of h at a dropped place leaves r and z as they were; every gradient has the bits it
+  has with a zero in that place."""
+  clips, frames, keep, seed = 3, 7, 0.5, 19
+  r = lambda *s: torch.randn(*s, generator=gen(cols + sum(s)))      # noqa: E731
+  h, x, dz, dr = (r(clips, frames, cols) + i for i in range(4))
+  gate = {'none': None, 'row': r(clips, frames, cols), 'clip': r(clips, 1, cols)}[gates]
+  gate = None if gate is None else gate.cuda()
+  dropped = ~O.keep_mask(h.shape, seed, 0, keep)
+  spots = dropped.flatten().nonzero().flatten()[::5]
+  for pre in ('layer', 'none'):
+    norm = blocks.ResidualNorm(cols, post='none', pre=pre, gate_act='sigmoid', alpha=0.7, keep_prob=keep, scale=r(cols).cuda(),
+                               w_pre=r(cols).cuda() if pre != 'none' else None)
+    call = dict(gate=gate, seed=seed)
+    res = []
+    for fill in (torch.zeros(len(spots)), torch.tensor(BAD).repeat(len(spots))[:len(spots)]):
+      hh = h.clone().flatten()
+      hh[spots] = fill
+      hh = hh.reshape(h.shape).cuda()
+      o, z, stats = norm.forward(hh, x.cuda(), save=True, **call)
+      g = norm.backward(dz.cuda() if pre != 'none' else None, dr.cuda(), hh, o, stats, **call)
+      res.append(dict(r=o, z=z, stats=stats, **g._asdict()))
+    for name, want in res[0].items():
+      if want is not None:
+        assert torch.isfinite(want).all() and torch.equal(res[1][name], want), (pre, name)
+
+
+@pytest.mark.parametrize('cols', COLS)
+def test_a_bad_row_adds_nothing_where_it_is_dropped(blocks, cols):
+  """With a post norm a NaN makes its row one: the column sums of elements that are dropped in that row stay what they are without
+  it, and so does a gate's gradient there."""
+  rows, keep, seed = 9, 0.5, 23
+  r = lambda *s: torch.randn(*s, generator=gen(cols + sum(s)))      # noqa: E731
+  h, x, dr, gate = (r(rows, cols) + i for i in range(4))
+  dropped = ~O.keep_mask(h.shape, seed, 0, keep)
+  norm = blocks.ResidualNorm(cols, post='rms', pre='none', keep_prob=keep, w_post=r(cols).cuda(), b_post=r(cols).cuda(), scale=r(cols).cuda())
+  res = []
+  for bad in (0.0, float('nan')):
+    h[4, 2] = bad
+    o, _, stats = norm.forward(h.cuda(), x.cuda(), gate=gate.cuda(), seed=seed, save=True)
+    res.append(norm.backward(None, dr.cuda(), h.cuda(), o, stats, gate=gate.cuda(), seed=seed))
+  at = dropped[4].cuda()
+  for name in ('dscale', 'dw_post', 'db_post'):
+    assert torch.equal(getattr(res[0], name)[at], getattr(res[1], name)[at]), name
+  assert torch.equal(res[0].dgate[4][at], res[1].dgate[4][at]) and torch.equal(res[0].dx, res[1].dx)
+  others = [i for i in range(rows) if i != 4]
+  assert torch.equal(res[0].dh[others], res[1].dh[others]) and torch.equal(res[0].dgate[others], res[1].dgate[others])
+
+
+def test_an_infinite_gate_leaves_a_dropped_gradient_zero(blocks):
+  """The gradient of what was dropped is 0 whatever its gate holds."""
+  cols, keep, seed = 200, 0.5, 3
+  x, gate = torch.ones(6, cols), torch.ones(6, cols)
+  dropped = ~O.keep_mask(x.shape, seed, 0, keep)
+  gate[dropped] = float('inf')
+  norm = blocks.ResidualNorm(cols, post='none', pre='none', keep_prob=keep)
+  g = norm.backward(None, x.cuda(), x.cuda(), x.cuda(), None, gate=gate.cuda(), seed=seed)
+  assert bool((g.dh.cpu()[dropped] == 0).all()) and bool((g.dgate.cpu()[dropped] == 0).all())
+  assert bool((g.dh.cpu()[~dropped] == 2).all())
