@@ -83,8 +83,8 @@ struct Team {
 // The instance for a number of columns: L lanes, NV chunks of V.  Rows of up to 512 columns have one chunk of 8 a lane.
 // (V = 1 only below 8 columns, where a chunk of 8 does not fit.  V = 9 for what is a little more than a power of two, as the 2^n + 1
 // bins of a transform are: 16384 x 513 forward 25 us, with two chunks of 8 32; 3999 x 513 fp32 backward 21, 25.)
-// Wider rows than 1024 are a workgroup's, 8 columns a lane as far as 512 lanes go: 8192 x 2048 forward 53 us, 16 columns a lane 62;
-// 4096 x 4096 51, 78, and backward 88, 97.
+// Wider rows than 1024 are a workgroup's, 8 columns a lane as far as 512 lanes go: 8192 x 2048 forward 53 us when that was
+// chosen, 16 columns a lane 62; 4096 x 4096 51, 78, and backward 88, 97.
 template <typename F>
 static inline bool norm_dispatch(int cols, F&& f) {
   if (cols < 8) f.template run<1, 8, 1>();

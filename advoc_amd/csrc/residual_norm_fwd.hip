@@ -32,23 +32,35 @@ __device__ __forceinline__ void row_stats(const Vals<V> (&a)[NV], const int (&du
   rstd = 1.f / sqrtf(sq * inv_cols + eps);
 }
 
-template <int V, int L, int NV>
-constexpr bool kFiveVectors = V * L * NV <= 4096;
+// Vectors in LDS: five, and four where a row is a workgroup's: five of 2048 or 4096 columns and the sums' place are more than a CU's
+// 160 KB over the workgroups that its waves allow, and one of those then waits for a round of its own (8192 x 2048 bf16: 50 us, four
+// vectors 45; 4096 x 4096 fp16: 39, 33; with five vectors and the launch cut to what fits 44 and 35).  There a lane holds its part of b_pre in registers; with 16 columns a lane it reads it for each row.
+template <int L>
+constexpr int kVectors = L > 64 ? 4 : 5;
+
+constexpr int kWavesPerSimd = 4, kCuLds = 160 * 1024;
+// LDS that a workgroup takes, in the 1280 bytes that a CU gives out
+template <int V, int L>
+constexpr int lds_taken(int cols) {
+  const int bytes = 4 * kVectors<L> * ((cols + V - 1) / V * V + 3) + 4 * (L > 64 ? 4 * (L / 64) : 1);
+  return (bytes + 1279) / 1280 * 1280;
+}
 
 // H: there is a block output; PRE: there is a pre norm.  Nothing else that may be absent is a branch around memory: an absent gate is
 // read from where h lies and replaced by ones.
 // Four waves to a SIMD, 128 registers to a lane.  With 8 columns a lane the next row's loads are in flight while a row is computed
-// (8192 x 2048: 50 us, without 55; 4096 x 4096: 50, without 62); with 16 they would spill (16384 x 1024: 38 us, with them 65).  A wave waits for its loads and stores in the order of their issue, so that the number of stores behind the
-// loads is to be known where the loads are waited for: hence the templates.
+// (measured with five vectors: 8192 x 2048 50 us, without 55; 4096 x 4096 50, without 62); with 16 they would spill (16384 x 1024: 38
+// us, with them 65).  A wave waits for its loads and stores in the order of their issue, so that the number of stores behind the loads
+// is to be known where the loads are waited for: hence the templates.
 // 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (202 MB): 38 us, 5.3 TB/s, a copy's rate.  Rows of a whole
-// workgroup meet four times on their way: 4096 x 4096 50 us, 4.0 TB/s.  16384 x 513: 25 us, 4.0 TB/s, bound by arithmetic (rows at
+// workgroup meet four times on their way: 4096 x 4096 in the same types 50 us, 4.0 TB/s, 8192 x 2048 48.  16384 x 513: 25 us, 4.0 TB/s, bound by arithmetic (rows at
 // odd offsets, three Philox blocks for nine words).  One row: 6 us, latency.
 template <typename T, typename R, int V, int L, int NV, int WG, bool H, bool PRE>
-__global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
+__global__ __launch_bounds__(WG, kWavesPerSimd) void norm_forward_kernel(NormArgs a) {
   using Row = Team<L, WG>;
-  extern __shared__ __align__(16) float vec[];  // scale, w_post, b_post, w_pre and, where five fit into LDS, b_pre
+  extern __shared__ __align__(16) float vec[];  // scale, w_post, b_post, w_pre and, where kFive, b_pre
   constexpr bool kAhead = NV == 1;
-  constexpr bool kFive = kFiveVectors<V, L, NV>;
+  constexpr bool kFive = kVectors<L> == 5, kHeld = !kFive && NV == 1;
   __shared__ float red[L > 64 ? 4 * (L / 64) : 1];
   int turn = 0;
   const int lane = Row::lane(), cols = a.cols;
@@ -82,6 +94,9 @@ __global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
   else
     advoc::stage_vectors<WG, V, 4>(vec, {a.scale, a.w_post, a.b_post, a.w_pre}, {1.f, 1.f, 0.f, 1.f}, cols);
   Row::meet();
+  Vals<V> b_pre(0.f);
+  if constexpr (kHeld && PRE)
+    if (a.b_pre) b_pre = advoc::floats_at<V>(a.b_pre + col[0]);
   for (; row < a.rows; row += step) {
     advoc::forget_lds();
     if constexpr (!kAhead) load(row);
@@ -125,6 +140,7 @@ __global__ __launch_bounds__(WG, 4) void norm_forward_kernel(NormArgs a) {
       for (int j = 0; j < NV; ++j) {
         Vals<V> z = (r[j] - mean1) * rstd1 * chunks.get(vec + 3 * floats, chunk[j]);
         if constexpr (kFive) z += chunks.get(vec + 4 * floats, chunk[j]);
+        else if constexpr (kHeld) z += b_pre;
         else if (a.b_pre) z += advoc::floats_at<V>(a.b_pre + col[j]);
         advoc::store_chunk<V>(advoc::row_at<T>(a.z, row * a.z_pitch, col[j]), z);
       }
@@ -141,10 +157,14 @@ struct Launch {
   void run() const {
     constexpr int WG = L > 64 ? L : 256;
     int64_t blocks = advoc::ceil_div(a.rows, Team<L, WG>::kRows);
-    const int64_t most = 256 * (1024 / WG);      // the workgroups that are resident together (four waves to a SIMD), then rows in turn
+    // the workgroups that are resident together, by waves and by LDS, then rows in turn
+    constexpr int kByWaves = 4 * 64 * kWavesPerSimd / WG;
+    static_assert(NV > 1 || kByWaves * lds_taken<V, L>(V * L * NV) <= kCuLds, "rows of this instance's width leave no wave without LDS");
+    const int by_lds = kCuLds / lds_taken<V, L>(a.cols);
+    const int64_t most = 256 * (by_lds < kByWaves ? by_lds : kByWaves);
     if (blocks > most) blocks = most;
     const dim3 grid((unsigned)blocks), block(WG);
-    const unsigned lds = (kFiveVectors<V, L, NV> ? 20u : 16u) * advoc::Chunks<V>(a.cols).floats();
+    const unsigned lds = 4u * kVectors<L> * advoc::Chunks<V>(a.cols).floats();
     if (!a.h) hipLaunchKernelGGL((norm_forward_kernel<T, R, V, L, NV, WG, false, true>), grid, block, lds, stream, a);
     else if (a.pre == ADVOC_NORM_NONE) hipLaunchKernelGGL((norm_forward_kernel<T, R, V, L, NV, WG, true, false>), grid, block, lds, stream, a);
     else hipLaunchKernelGGL((norm_forward_kernel<T, R, V, L, NV, WG, true, true>), grid, block, lds, stream, a);
