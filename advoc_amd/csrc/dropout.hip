@@ -99,7 +99,8 @@ extern "C" int advoc_dropout(const void* x, int64_t x_pitch, void* y, int64_t y_
   if (rows > 1 && (x_pitch < cols || y_pitch < cols)) return ADVOC_ERR_BAD_SHAPE;
   if (!advoc::dtype_ok(dtype) || (offset & 3)) return ADVOC_ERR_UNSUPPORTED;
   if (cols > 0x7fffffffLL - 2 * kThreads * kPer && rows > 1 && (x_pitch != cols || y_pitch != cols)) return ADVOC_ERR_UNSUPPORTED;
-  if (rows > (1LL << 40) / cols) return ADVOC_ERR_UNSUPPORTED;         // the grid ends at 2^31 workgroups of 2048 elements
+  // a launch ends at 2^32 - 1 work-items of 8 elements
+  if (rows > ((1LL << 35) - kThreads * kPer) / cols) return ADVOC_ERR_UNSUPPORTED;
   const bool pitched = rows > 1 && (x_pitch != cols || y_pitch != cols);
   Args a = {x, y, rows * cols, x_pitch, y_pitch, pitched ? (uint32_t)cols : 0u,
             advoc::make_drop_key(keep_prob, seed, offset, seed_dev)};

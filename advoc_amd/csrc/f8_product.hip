@@ -548,6 +548,21 @@ Plan make_plan(int64_t m, int64_t n, int blocks, bool exact) {
   return p;
 }
 
+unsigned thin_waves(int blocks) { return blocks >= 16 ? 16 : blocks >= 8 ? 8 : blocks >= 4 ? 4 : 2; }
+
+// A launch ends at 2^32 - 1 work-items.  (m and n are at most 2^31 each and less than 2^42 tiles of 64 x 64 together: no overflow.)
+bool launch_ok(const Plan& p, int64_t m, int64_t n, int blocks, bool exact) {
+  int64_t items = 0;
+  switch (p.form) {
+    case kDot: items = ceil_div(n, 4) * 256; break;
+    case kThin: items = ceil_div(n, 16) * 64 * thin_waves(blocks); break;
+    case kTile64: items = ceil_div(m, 64) * ceil_div(n, 64) * p.splits * 256; break;
+    case kTile128: items = ceil_div(m, 128) * ceil_div(n, 128) * p.splits * 512; break;
+    case kTile256: items = ceil_div(m, 256) * ceil_div(n, exact ? 128 : 256) * p.splits * 512; break;
+  }
+  return items <= 0xffffffffLL;
+}
+
 template <typename O, bool EXACT, int FA, int FB, int BM, int BN, int WM, int WN, int S, bool SPLIT>
 int run_tile(const Args& g, int splits, hipStream_t stream) {
   constexpr int kThreads = BM / WM * (BN / WN) * 64;
@@ -569,7 +584,7 @@ template <typename O, bool EXACT, int FA, int FB>
 int run(const Args& g, const Plan& p, hipStream_t stream) {
   ADVOC_CLEAR_LAUNCH_ERROR();
   if (p.form == kThin) {
-    const unsigned waves = g.blocks >= 16 ? 16 : g.blocks >= 8 ? 8 : g.blocks >= 4 ? 4 : 2;
+    const unsigned waves = thin_waves(g.blocks);
     hipLaunchKernelGGL((f8_thin_kernel<O, EXACT, FA, FB>), dim3((unsigned)ceil_div(g.n, 16)), dim3(64 * waves), waves * 1024, stream, g);
     ADVOC_RETURN_IF_LAUNCH_FAILED();
     return ADVOC_OK;
@@ -636,6 +651,7 @@ extern "C" int advoc_matmul_nt_f8(const uint8_t* a, const uint8_t* a_scale, int3
   Plan p = make_plan(m, n, g.blocks, out_dtype == ADVOC_F32);
   if (p.splits > 1 && (!workspace || workspace_bytes < 4 * p.splits * m * n)) p.splits = 1, p.per_split = g.blocks;
   if (p.splits > 1 && (reinterpret_cast<uintptr_t>(workspace) & 3)) return ADVOC_ERR_UNSUPPORTED;
+  if (!launch_ok(p, m, n, g.blocks, out_dtype == ADVOC_F32)) return ADVOC_ERR_UNSUPPORTED;
   g.per_split = p.per_split;
   if (out_dtype == ADVOC_F32) return run_formats<float>(g, p, a_format, b_format, advoc::as_stream(stream));
   if (out_dtype == ADVOC_BF16) return run_formats<__bf16>(g, p, a_format, b_format, advoc::as_stream(stream));

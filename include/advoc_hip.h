@@ -559,7 +559,8 @@ int advoc_dropout_mask_u8(uint8_t* mask, int64_t count, uint64_t seed, uint64_t 
  * dy.  A dropped element is 0 whatever x holds (NaN and infinities included); keep_prob 1 copies.
  *   seed_dev  NULL, or a device word that the kernel adds to `seed`: a captured graph whose program changes that word
  *             between replays draws another mask each time
- * y may be x (same pitch).  offset % 4 == 0. */
+ * y may be x (same pitch).  offset % 4 == 0.  Up to 2^35 - 2048 elements (a launch's 2^32 - 1 work-items of 8);
+ * ADVOC_ERR_UNSUPPORTED beyond. */
 int advoc_dropout(const void* x, int64_t x_pitch, void* y, int64_t y_pitch, int64_t rows, int64_t cols, int32_t dtype,
                   float keep_prob, uint64_t seed, uint64_t offset, const uint64_t* seed_dev, advoc_stream_t stream);
 
@@ -651,7 +652,9 @@ int advoc_f8_quantize(const void* x, int64_t x_pitch, int64_t rows, int64_t cols
  * twice the rate: it adds up in fp32 but for products below 2^-13 of the largest of eight neighbours, which it drops (1.5e-5 of
  * the result in norm; their own rounding is 1.7e-3 or 2e-4).  out [m, n] dense; accumulate != 0 (out_dtype ADVOC_F32) adds to it.
  * workspace: advoc_matmul_nt_f8_workspace_bytes(m, n, k, out_dtype) bytes, 4-byte aligned (0: may be NULL); with too little the
- * product runs unsplit.  The order of every sum is fixed by the shapes: two calls give the same bits. */
+ * product runs unsplit.  k <= 8 000 000, and the launch may take 2^32 - 1 work-items (up to 16 rows: n < 2^26 always does;
+ * otherwise fewer than 2^36 outputs, in whole tiles, do); ADVOC_ERR_UNSUPPORTED beyond.  The order of every sum is fixed by the shapes: two
+ * calls give the same bits. */
 int64_t advoc_matmul_nt_f8_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t out_dtype);
 int advoc_matmul_nt_f8(const uint8_t* a, const uint8_t* a_scale, int32_t a_format, const uint8_t* b, const uint8_t* b_scale,
                        int32_t b_format, void* out, int32_t out_dtype, int32_t accumulate, int64_t m, int64_t n, int64_t k,

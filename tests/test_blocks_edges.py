@@ -31,3 +31,17 @@ def test_the_oracle_selects_what_is_kept():
     assert torch.equal(r, res[0][0])
     for k, v in grads.items():
       assert torch.equal(v, res[0][1][k]), k
+
+
+def test_sizes_beyond_a_launch_are_refused(lib):
+  """A launch holds 2^32 - 1 work-items: what would need more is refused before it is made, whatever form a product takes."""
+  def drop(rows, cols, pad=0):
+    return lib.advoc_dropout(64, cols + pad, 64, cols + pad, rows, cols, 1, 0.5, 0, 0, None, None)
+  assert drop(2 ** 25, 1024) == -2 and drop(2 ** 25, 1024, 8) == -2 and drop(1, 2 ** 35) == -2
+
+  def mul(m, n, k, dtype):
+    return lib.advoc_matmul_nt_f8(64, 64, 0, 64, 64, 0, 64, dtype, 0, m, n, k, None, 0, None)
+  for dtype in (0, 1):
+    assert mul(1, 2 ** 26, 128, dtype) == -2 and mul(2, 2 ** 31, 128, dtype) == -2      # dot products: 64 work-items a column
+    assert mul(3, 2 ** 27, 1024, dtype) == -2                                           # thin: 32 of them
+    assert mul(2 ** 31, 1, 128, dtype) == -2 and mul(2 ** 22, 2 ** 18, 128, dtype) == -2      # tiles
