@@ -312,10 +312,6 @@ class ResidualNorm(object):
     lib = _lib.load()
     nbytes = lib.advoc_residual_norm_workspace_bytes(head + _NO_WORKSPACE)
     work = torch.empty(nbytes // 4, dtype=torch.float32, device=r.device) if nbytes else None
-    if rows == 0 and not accumulate:
-      for t in g:
-        if t is not None:
-          t.zero_()
     _call(lib.advoc_residual_norm_backward, 'advoc_residual_norm_backward', index,
           head + _DESCRIPTOR_TAIL.pack(work.data_ptr(), nbytes) if nbytes else head + _NO_WORKSPACE)
     return ResidualNormGrads(dh, dx, dgate, *g)

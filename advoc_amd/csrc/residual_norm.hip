@@ -4,6 +4,7 @@
 namespace advoc {
 bool launch_norm_forward(const NormArgs& a, int dtype, int res_dtype, hipStream_t stream);
 int64_t norm_backward_workspace(const NormArgs& a, float* const (&out)[5]);
+int clear_norm_sums(int cols, float* const (&out)[5], hipStream_t stream);
 int launch_norm_backward(NormArgs a, int dtype, int res_dtype, float* const (&out)[5], int accumulate, void* workspace,
                          int64_t workspace_bytes, hipStream_t stream);
 }  // namespace advoc
@@ -121,7 +122,10 @@ extern "C" int advoc_residual_norm_backward(const advoc_residual_norm* desc, adv
   float* out[5];
   const int rc = backward_args(d, a, out);
   if (rc != ADVOC_OK) return rc;
-  if (d.rows == 0) return ADVOC_OK;
+  if (d.rows == 0) {
+    out[2] = d.dscale;                         // (a tensor of no rows has no address: h may be there all the same)
+    return d.accumulate ? ADVOC_OK : advoc::clear_norm_sums(d.cols, out, advoc::as_stream(stream));
+  }
   const bool post = d.norm_post != ADVOC_NORM_NONE, pre = d.norm_pre != ADVOC_NORM_NONE;
   if ((pre && (!d.dz.p || !d.r.p)) || (!pre && !d.dr.p) || ((pre || post) && !d.stats)) return ADVOC_ERR_NULL;
   if (reinterpret_cast<uintptr_t>(d.stats) & 15) return ADVOC_ERR_UNSUPPORTED;

@@ -419,6 +419,20 @@ int64_t norm_backward_workspace(const NormArgs& a, float* const (&out)[5]) {
   return 4 * (p.part_floats + p.gate_floats + p.carry_floats);
 }
 
+// what a call without rows overwrites: the sums of no entries
+int clear_norm_sums(int cols, float* const (&out)[5], hipStream_t stream) {
+  FoldArgs f = {};
+  const Sums sums = wanted_sums(out, f.out);
+  for (int s = 0; s < kSums; ++s) f.sums += sums.slot[s] >= 0;
+  if (f.sums == 0) return ADVOC_OK;
+  f.cols = cols;
+  f.col_blocks = (int)ceil_div(cols, 64);
+  ADVOC_CLEAR_LAUNCH_ERROR();
+  hipLaunchKernelGGL(norm_fold_kernel<float>, dim3((unsigned)(f.sums * f.col_blocks)), dim3(1024), 0, stream, f);
+  ADVOC_RETURN_IF_LAUNCH_FAILED();
+  return ADVOC_OK;
+}
+
 int launch_norm_backward(NormArgs a, int dtype, int res_dtype, float* const (&out)[5], int accumulate, void* workspace,
                          int64_t workspace_bytes, hipStream_t stream) {
   FoldArgs f = {};

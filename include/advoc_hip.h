@@ -606,7 +606,7 @@ typedef struct advoc_residual_norm {
   const float* w_pre;
   const float* b_pre;
   float alpha, eps, keep_prob;
-  int32_t accumulate; /* backward: != 0 adds to the five parameter gradients, 0 overwrites them */
+  int32_t accumulate; /* backward: != 0 adds to the five parameter gradients, 0 overwrites them (with zeros if rows is 0) */
   uint64_t seed, offset;
   const uint64_t* seed_dev;
   advoc_rows h, x, gate;

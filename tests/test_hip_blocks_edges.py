@@ -87,3 +87,41 @@ def test_an_infinite_gate_leaves_a_dropped_gradient_zero(blocks):
   g = norm.backward(None, x.cuda(), x.cuda(), x.cuda(), None, gate=gate.cuda(), seed=seed)
   assert bool((g.dh.cpu()[dropped] == 0).all()) and bool((g.dgate.cpu()[dropped] == 0).all())
   assert bool((g.dh.cpu()[~dropped] == 2).all())
+
+
+# ---- empty calls, and outputs of other shapes and types ----
+@pytest.mark.parametrize('has_h', [True, False])
+def test_a_backward_call_without_rows_clears_what_it_overwrites(blocks, has_h):
+  """Sums over no rows are 0: written by the C entry, left alone where they are added to or not wanted."""
+  from advoc_amd import _lib
+  cols = 1030
+  arena = torch.full((6, cols), 3.0, device='cuda')
+  names = ['dw_post', 'db_post', 'dscale', 'dw_pre', 'db_pre']
+  q = _lib.ResidualNorm()
+  q.cols, q.gate_group, q.alpha, q.eps, q.keep_prob, q.norm_pre, q.norm_post = cols, 1, 1.0, 1e-5, 1.0, 1, 1 if has_h else 0
+  if has_h:
+    q.h.p, q.h.pitch = arena.data_ptr(), cols
+  for i, name in enumerate(names):
+    setattr(q, name, arena[i].data_ptr())
+  q.db_pre = None
+  lib = _lib.load()
+  q.accumulate = 1
+  _lib.check(lib.advoc_residual_norm_backward(ctypes.byref(q), _lib.stream()))
+  assert bool((arena == 3).all())
+  q.accumulate = 0
+  _lib.check(lib.advoc_residual_norm_backward(ctypes.byref(q), _lib.stream()))
+  cleared = ('dw_post', 'db_post', 'dscale', 'dw_pre') if has_h else ('dscale', 'dw_pre')
+  for i, name in enumerate(names):
+    assert bool((arena[i] == (0 if name in cleared else 3)).all()), name
+  assert bool((arena[5] == 3).all())
+
+
+def test_a_backward_call_without_rows_through_the_binding(blocks):
+  e = torch.zeros(0, 16, device='cuda')
+  norm = blocks.ResidualNorm(16, w_pre=torch.ones(16, device='cuda'), scale=torch.ones(16, device='cuda'))
+  into = {k: torch.full((16,), 5.0, device='cuda') for k in ('dw_pre', 'dscale')}
+  r, z, stats = norm.forward(e, e, save=True)
+  g = norm.backward(z, r, e, r, stats, into=into, accumulate=True)
+  assert bool((g.dw_pre == 5).all()) and bool((g.dscale == 5).all())
+  g = norm.backward(z, r, e, r, stats, into=into)
+  assert g.dw_pre is into['dw_pre'] and bool((g.dw_pre == 0).all()) and bool((g.dscale == 0).all())
