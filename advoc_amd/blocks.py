@@ -261,7 +261,8 @@ class ResidualNorm(object):
 
   def backward(self, dz, dr, h, r, stats, gate=None, seed=0, offset=0, seed_dev=None, into=None, accumulate=False):
     """Gradients of forward(h, x, gate, seed, offset) with its r and stats (h None: r is x).  dz: gradient of z (None without a
-    pre norm), dr: gradient of r from elsewhere (may be None with a pre norm).  Gradients of what was not given are None.
+    pre norm), dr: gradient of r from elsewhere (may be None with a pre norm).  Gradients of what was not given are None, the
+    others have the shapes of h, r, the gate and the parameters.
     into: {'dw_post': float32 [cols] buffer, ...} to write parameter gradients into, or with `accumulate` to add to."""
     like = h if h is not None else dz
     if not isinstance(like, torch.Tensor):
@@ -283,7 +284,7 @@ class ResidualNorm(object):
     dh = dgate = None
     pdh = pdgate = _ABSENT
     if h is not None:
-      dh = torch.empty_like(r, dtype=h.dtype, memory_format=contiguous)
+      dh = torch.empty_like(h, memory_format=contiguous)
       pdh = dh.data_ptr(), cols
     if gate is not None:
       dgate = torch.empty_like(gate, memory_format=contiguous)

@@ -125,3 +125,16 @@ def test_a_backward_call_without_rows_through_the_binding(blocks):
   assert bool((g.dw_pre == 5).all()) and bool((g.dscale == 5).all())
   g = norm.backward(z, r, e, r, stats, into=into)
   assert g.dw_pre is into['dw_pre'] and bool((g.dw_pre == 0).all()) and bool((g.dscale == 0).all())
+
+
+def test_gradients_have_their_tensors_shapes(blocks):
+  """h may lie in another leading shape than x, as a product leaves it: its gradient has h's."""
+  x = torch.randn(2, 6, 40, generator=gen(0)).cuda()
+  h = torch.randn(12, 40, generator=gen(1)).cuda().bfloat16()
+  norm = blocks.ResidualNorm(40, scale=torch.ones(40, device='cuda'))
+  r, z, stats = norm.forward(h, x, save=True)
+  assert r.shape == z.shape == x.shape
+  g = norm.backward(z, r, h, r, stats)
+  same = norm.backward(z, r, h.view(2, 6, 40), r, stats)
+  assert g.dh.shape == h.shape and g.dh.dtype == h.dtype and g.dx.shape == x.shape
+  assert same.dh.shape == x.shape and torch.equal(same.dh.view(12, 40), g.dh)
