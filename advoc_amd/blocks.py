@@ -376,18 +376,20 @@ def _product_workspace(m, n, k, code):
   return _lib.load().advoc_matmul_nt_f8_workspace_bytes(m, n, k, code)
 
 
-def matmul_nt_f8(a, b, out_dtype=torch.float32, out=None, accumulate=False):
+def matmul_nt_f8(a, b, out_dtype=None, out=None, accumulate=False):
   """a b^T of two F8Matrix operands with the same k -> [a.rows, b.rows] (``advoc_matmul_nt_f8``); a float32 result is
-  accumulated in fp32 throughout.  accumulate: add to `out` (float32), e.g. a gradient arena's slice."""
+  accumulated in fp32 throughout.  out_dtype: that of `out`, without one float32.  accumulate: add to `out` (float32), e.g. a gradient arena's slice."""
   if not isinstance(a, F8Matrix) or not isinstance(b, F8Matrix) or a.k != b.k or a.buffer.device != b.buffer.device:
     raise _lib.AdvocHipError('two F8Matrix operands with the same k on one device are needed')
   device, m, n = a.buffer.device, a.rows, b.rows
   if out is None:
     if accumulate:
       raise _lib.AdvocHipError('accumulate needs out')
-    out = torch.empty(m, n, dtype=out_dtype, device=device)
+    out = torch.empty(m, n, dtype=out_dtype or torch.float32, device=device)
   elif not isinstance(out, torch.Tensor) or out.device != device or out.shape != (m, n) or not out.is_contiguous():
     raise _lib.AdvocHipError('out must be a contiguous [{}, {}] tensor on {}'.format(m, n, device))
+  elif out_dtype is not None and out.dtype != out_dtype:
+    raise _lib.AdvocHipError('out is {}, out_dtype {}'.format(out.dtype, out_dtype))
   code = _dtype(out, 'out')
   lib = _lib.load()
   nbytes = _product_workspace(m, n, a.k, code)

@@ -138,3 +138,16 @@ def test_gradients_have_their_tensors_shapes(blocks):
   same = norm.backward(z, r, h.view(2, 6, 40), r, stats)
   assert g.dh.shape == h.shape and g.dh.dtype == h.dtype and g.dx.shape == x.shape
   assert same.dh.shape == x.shape and torch.equal(same.dh.view(12, 40), g.dh)
+
+
+def test_product_into_a_buffer_of_another_type_than_asked(blocks):
+  """out decides the result's type when no type is named; one that is named has to be its."""
+  from advoc_amd._lib import AdvocHipError
+  x = torch.randn(20, 200, generator=gen(0)).cuda()
+  q = blocks.quantize_f8(x)
+  out = torch.empty(20, 20, dtype=torch.bfloat16, device='cuda')
+  assert blocks.matmul_nt_f8(q, q, out=out) is out and torch.equal(out, blocks.matmul_nt_f8(q, q, out_dtype=torch.bfloat16))
+  assert blocks.matmul_nt_f8(q, q, out=out, out_dtype=torch.bfloat16) is out and blocks.matmul_nt_f8(q, q).dtype == torch.float32
+  for other in (torch.float32, torch.float16):
+    with pytest.raises(AdvocHipError):
+      blocks.matmul_nt_f8(q, q, out=out, out_dtype=other)
