@@ -238,6 +238,8 @@ class ResidualNorm(object):
     if h is None:
       if not self.pre:
         raise _lib.AdvocHipError('neither h nor a pre norm: nothing to compute')
+      if r is not None and r is not x:
+        raise _lib.AdvocHipError('without h the residual stream stays x: r is not written')
       r = x
     else:
       ph = self._tensor('h', h, rows, index)
@@ -247,7 +249,8 @@ class ResidualNorm(object):
       else:
         pr = self._tensor('r', r, rows, index, x.dtype)
     if not self.pre:
-      z = None
+      if z is not None:
+        raise _lib.AdvocHipError('without a pre norm there is no z')
     elif z is None:
       z = torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
       pz = z.data_ptr(), self.cols

@@ -151,3 +151,15 @@ def test_product_into_a_buffer_of_another_type_than_asked(blocks):
   for other in (torch.float32, torch.float16):
     with pytest.raises(AdvocHipError):
       blocks.matmul_nt_f8(q, q, out=out, out_dtype=other)
+
+
+def test_buffers_that_a_call_would_not_write_are_refused(blocks):
+  from advoc_amd._lib import AdvocHipError
+  x, buf = torch.randn(4, 40, generator=gen(0)).cuda(), torch.full((4, 40), 7.0, device='cuda')
+  with pytest.raises(AdvocHipError):
+    blocks.ResidualNorm(40).forward(None, x, r=buf)                      # r is x
+  with pytest.raises(AdvocHipError):
+    blocks.ResidualNorm(40, pre='none').forward(x, x, z=buf)             # there is no z
+  assert bool((buf == 7).all())
+  r, z, _ = blocks.ResidualNorm(40).forward(None, x, r=x, z=buf)
+  assert r is x and z is buf
