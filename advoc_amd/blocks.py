@@ -4,7 +4,8 @@ gate and residual scale, and products of 8-bit block-scaled matrices, each with 
 Like ``conv.Layer`` this module only checks arguments and calls into libadvoc_hip.so (``include/advoc_hip.h`` holds the
 formulas); no arithmetic happens in Python/torch, and there is no CPU path.  Tensors live in HBM; fp32, bf16 and fp16 are
 taken, rows may be padded (unit stride inside a row, one distance between rows).  Every call is asynchronous on the current
-stream of the tensors' device and can be captured into a graph.
+stream of the tensors' device and can be captured into a graph.  None takes part in torch's autograd: gradients come from the
+backward calls below, and a tensor that autograd follows is refused while it is on (parameters of a norm are taken as they are).
 
   z, x8   = one block:   z = N_pre(x);  y = W z;  r = x + alpha * scale * gate * dropout(N_post(y));  next z = N_pre(r)
 
@@ -53,6 +54,9 @@ def _rows(t, name, index=None):
     raise _lib.AdvocHipError('{} must be a torch tensor on a HIP device (no CPU path exists)'.format(name))
   if index is not None and t.get_device() != index:
     raise _lib.AdvocHipError('{} is on {}, the other tensors on device {}'.format(name, t.device, index))
+  if t.requires_grad and torch.is_grad_enabled():
+    raise _lib.AdvocHipError('{} needs a gradient, which autograd does not get from here: call under torch.no_grad() or on '
+                             '{}.detach(), and the backward calls by hand'.format(name, name))
   if not t.dim():
     raise _lib.AdvocHipError('{} must have at least one dimension'.format(name))
   cols = t.shape[-1]

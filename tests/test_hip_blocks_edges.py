@@ -163,3 +163,26 @@ def test_buffers_that_a_call_would_not_write_are_refused(blocks):
   assert bool((buf == 7).all())
   r, z, _ = blocks.ResidualNorm(40).forward(None, x, r=x, z=buf)
   assert r is x and z is buf
+
+
+def test_tensors_that_autograd_follows_are_refused(blocks):
+  """No call records a gradient: a tensor that needs one is taken only where autograd is off."""
+  from advoc_amd._lib import AdvocHipError
+  x = torch.randn(4, 40, generator=gen(0)).cuda()
+  leaf = x.clone().requires_grad_()
+  norm = blocks.ResidualNorm(40)
+  r, z, stats = norm.forward(x, x, save=True)
+  calls = [lambda t: blocks.dropout(t, 0.5, 1), lambda t: blocks.quantize_f8(t), lambda t: blocks.quantize_f8_both(t),
+           lambda t: norm.forward(t, x), lambda t: norm.forward(x, t), lambda t: norm.forward(x, x, gate=t),
+           lambda t: norm.backward(t, x, x, r, stats), lambda t: norm.backward(z, x, t, r, stats)]
+  for i, call in enumerate(calls):
+    for t in (leaf, leaf * 2):
+      with pytest.raises(AdvocHipError, match='autograd'):
+        call(t)
+        pytest.fail('case %d was taken' % i)
+    with torch.no_grad():
+      call(leaf)
+    call(leaf.detach())
+  # parameters belong to whoever updates them with the gradients that backward returns
+  p = torch.nn.Parameter(torch.ones(40, device='cuda'))
+  assert blocks.ResidualNorm(40, w_pre=p).forward(x, x)[1].requires_grad is False
