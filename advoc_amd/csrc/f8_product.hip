@@ -6,8 +6,11 @@
 // What that instruction adds up is not quite fp32: it aligns the products of eight consecutive k to the largest of them and drops
 // what is below 2^-13 of it (measured, also of the unscaled 16x16x32 form).  Against the definition the result is 1.5e-5 off in norm
 // -- 1/100 of the rounding of a 16-bit output, so those take it.  An fp32 output is computed EXACTly: the bytes become bf16 with the
-// block's power of two applied (v_cvt_scalef32_pk_bf16_fp8; every 8-bit value is a bf16 value) and go through
-// v_mfma_f32_16x16x32_bf16, whose sums are fp32's: 4e-8 off in norm, at half the rate.
+// block's power of two applied (v_cvt_scalef32_pk_bf16_fp8) and go through v_mfma_f32_16x16x32_bf16, whose sums are fp32's: 4e-8 off
+// in norm, at half the rate.  bf16 holds every 8-bit value with its power of two but at the two ends: below 2^-130 it is rounded to a
+// multiple of 2^-133 (blocks whose largest is below 2^-114), and what quantising rounded up to 2^128 (blocks whose largest is above
+// 3.1e38) becomes infinite, as it would in fp32.  So a caller's choice of the output's type is one of the sums' too; one or two rows
+// (f8_dot_kernel) are summed in fp32 for either, exponents applied to the sums.
 // The operand with n rows is the instruction's first: the four accumulators of a lane are then four consecutive n of one output
 // row, and for 16-bit outputs the n that two fragments stand for are dealt so that one continues the other: a lane stores 16 bytes,
 // four of them 64 consecutive ones, without a turn through LDS.

@@ -186,3 +186,28 @@ def test_tensors_that_autograd_follows_are_refused(blocks):
   # parameters belong to whoever updates them with the gradients that backward returns
   p = torch.nn.Parameter(torch.ones(40, device='cuda'))
   assert blocks.ResidualNorm(40, w_pre=p).forward(x, x)[1].requires_grad is False
+
+
+# ---- the ends of the exponent range ----
+@pytest.mark.parametrize('fmt', ['e4m3', 'e5m2'])
+@pytest.mark.parametrize('m', [1, 3, 16, 70, 300])
+def test_product_at_the_ends_of_the_exponent_range(blocks, fmt, m):
+  """fp32 outputs of three rows and more take what a value stands for as a bfloat16: a multiple of 2^-133 below 2^-130, infinite at
+  2^128.  16-bit outputs and one or two rows take it as it is.  A term to an output, powers of two on the other side: exact."""
+  types = {'e4m3': torch.float8_e4m3fn, 'e5m2': torch.float8_e5m2}
+  lead = torch.tensor([100.0, 110, 114, 116, 118, 120, 124, 126])
+  tiny = torch.zeros(64, 128)
+  tiny[:, 0] = torch.exp2(-lead).repeat(8)                              # the block's largest, times 0
+  tiny[:, 1] = tiny[:, 0] * torch.exp2(-torch.arange(64) / 4.0)
+  huge = torch.zeros(8, 128)
+  huge[:, 1] = torch.tensor([1.5e38, 1.7e38, 3.0e38, 3.1e38, 3.2e38, 3.3e38, 3.39e38, torch.finfo(torch.float32).max])
+  for b, up in ((tiny, 2.0 ** 100), (huge, 2.0 ** -120)):
+    a = torch.zeros(m, 128)
+    a[:, 1] = up
+    qa, qb = blocks.quantize_f8(a.cuda()), blocks.quantize_f8(b.cuda(), fmt)
+    v = qb.data.cpu().view(types[fmt]).float()[:, 1].double() * torch.exp2(qb.scale.cpu()[:, 0].double() - 127)
+    assert bool((v == 2.0 ** 128).any()) == (b is huge)
+    as_taken = v if m < 3 else v.bfloat16().double()
+    assert torch.equal(blocks.matmul_nt_f8(qa, qb).cpu().double(), (as_taken * up).expand(m, -1))
+    got = blocks.matmul_nt_f8(qa, qb, out_dtype=torch.bfloat16).cpu()
+    assert torch.equal(got, (v * up).bfloat16().expand(m, -1))
