@@ -37,7 +37,8 @@ struct DropKey {
   uint64_t seed, offset;        // offset is a multiple of 4
   const uint64_t* seed_dev;     // added to the seed when not NULL: read by the kernel, so a replayed graph draws anew
   uint32_t thresh;
-  float scale;                  // 1 / keep
+  float scale;                  // 1 / keep, rounded once: what is kept is multiplied by it (1.5 units of fp32 off x / keep at most, a
+                                // division would be 0.5 and a dozen instructions; nothing where keep is a power of two)
 };
 
 // (1 - keep) 2^32 in fp32, as dropout_mask_kernel (train_ops.hip) computes it on the device, where the conversion to an

@@ -245,7 +245,8 @@ __device__ __forceinline__ void draw_chunk(uint32_t (&words)[V], uint64_t i, boo
 }
 
 // 1 / (1 + exp(-x)), the exponential as 2^t (1 + the part of -x log2 e that t's rounding dropped, times ln 2): within 6 units in the
-// last place at every x (half the instructions of expf and a division).  0 where exp(-x) would be no finite number.
+// last place wherever the result is a normal number, x >= -87.33 (half the instructions of expf and a division; 16-bit outputs
+// round 2^13 units and more away).  Subnormal results become 0.
 __device__ __forceinline__ float sigmoid(float x) {
   const float kHigh = 1.44269502f, kLow = 1.92596303e-8f;            // log2 e in two parts
   x = x > 88.f ? 88.f : x;                                           // (1 from 17 on; a NaN stays one)

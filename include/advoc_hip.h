@@ -554,9 +554,10 @@ int advoc_dropout_mask_u8(uint8_t* mask, int64_t count, uint64_t seed, uint64_t 
 #define ADVOC_BF16 1
 #define ADVOC_F16 2
 
-/* y[i] = keep_i ? x[i] / keep_prob : 0 with keep_i of advoc_dropout_mask_u8 at (seed, offset + i), i = row * cols + column
- * (the LOGICAL index: a pitch does not change what is dropped).  The mask is never stored: the gradient is the same call on
- * dy.  A dropped element is 0 whatever x holds (NaN and infinities included); keep_prob 1 copies.
+/* y[i] = keep_i ? x[i] * (1 / keep_prob) : 0, the reciprocal rounded to fp32, with keep_i of advoc_dropout_mask_u8 at
+ * (seed, offset + i), i = row * cols + column (the LOGICAL index: a pitch does not change what is dropped).  The mask is never
+ * stored: the gradient is the same call on dy.  A dropped element is 0 whatever x holds (NaN and infinities included);
+ * keep_prob 1 copies.
  *   seed_dev  NULL, or a device word that the kernel adds to `seed`: a captured graph whose program changes that word
  *             between replays draws another mask each time
  * y may be x (same pitch).  offset % 4 == 0.  Up to 2^35 - 2048 elements (a launch's 2^32 - 1 work-items of 8);

@@ -211,3 +211,14 @@ def test_product_at_the_ends_of_the_exponent_range(blocks, fmt, m):
     assert torch.equal(blocks.matmul_nt_f8(qa, qb).cpu().double(), (as_taken * up).expand(m, -1))
     got = blocks.matmul_nt_f8(qa, qb, out_dtype=torch.bfloat16).cpu()
     assert torch.equal(got, (v * up).bfloat16().expand(m, -1))
+
+
+def test_a_sigmoid_gate_that_is_nearly_shut(blocks):
+  """Within 6 units in the last place down to the smallest normal number; a smaller value is 0 or that near."""
+  gate = torch.linspace(-104, -86, 512, device='cuda').reshape(1, 512)
+  norm = blocks.ResidualNorm(512, post='none', pre='none', gate_act='sigmoid')
+  r = norm.forward(torch.ones(1, 512, device='cuda'), torch.zeros(1, 512, device='cuda'), gate=gate)[0].cpu().double()
+  want = torch.sigmoid(gate.cpu().double())
+  near = (r - want).abs() <= 12 * 2.0 ** -24 * want
+  normal = want >= 2.0 ** -126 * (1 + 2.0 ** -20)
+  assert bool(near[normal].all()) and bool((near | (r == 0))[~normal].all()) and 0 < int(normal.sum()) < 100
