@@ -81,8 +81,16 @@ struct Team {
 };
 
 // The instance for a number of columns: L lanes, NV chunks of V.  Rows of up to 512 columns have one chunk of 8 a lane.
-// (V = 1 only below 8 columns, where a chunk of 8 does not fit.  V = 9 for what is a little more than a power of two, as the 2^n + 1
-// bins of a transform are: 16384 x 513 forward 25 us, with two chunks of 8 32; 3999 x 513 fp32 backward 21, 25.)
+// V = 1 only below 8 columns, where a chunk of 8 does not fit.
+// V = 9 up to an eighth more than a power of two (the 2^n + 1 bins of a transform), where the next instance would leave half of its
+// lanes empty or hold two chunks.  Forward | backward in us, 9 columns a lane against 8, bf16 with fp32 residuals and dropout:
+//   16384 x 513 fwd 25 | two chunks 32, 3999 x 513 fp32 bwd 21 | 25;   8192 x 2049 fwd 61 | 73, bwd 95 | 124, x 2304 62 | 61, 96 | 110;
+//   4096 x 4097 60 | 83, 102 | 140, x 4608 62 | 66, 103 | 113;  1677 rows of fp32: x 2049 23 | 25, 43 | 47, x 4097 43 | 51, 71 | 88.
+// Not where a row's share of few rows' time is small or its column sums would come from twice the workgroups, and not by the number
+// of rows either (a row's bits depend on its width alone):
+//   16384 x 257 17 | 20, 30 | 36, but 256 to 1024 rows 4.7 | 4.1, 11.7 | 10.0, 1677 of fp32 6.3 | 5.8, 15.6 | 15.0;
+//   16384 x 1025 (128 lanes) 59 | 72, 90 | 112, but 1024 rows 8.1 | 9.0, 25 | 19, 1677 of fp32 15.5 | 15.3, 31 | 26;
+//   16384 x 129 11.5 | 12.9, 24.5 | 22.9.
 // Wider rows than 1024 are a workgroup's, 8 columns a lane as far as 512 lanes go: 8192 x 2048 forward 53 us when that was
 // chosen, 16 columns a lane 62; 4096 x 4096 51, 78, and backward 88, 97.
 template <typename F>
@@ -94,7 +102,9 @@ static inline bool norm_dispatch(int cols, F&& f) {
   else if (cols <= 576) f.template run<9, 64, 1>();
   else if (cols <= 1024) f.template run<8, 64, 2>();
   else if (cols <= 2048) f.template run<8, 256, 1>();
+  else if (cols <= 2304) f.template run<9, 256, 1>();
   else if (cols <= 4096) f.template run<8, 512, 1>();
+  else if (cols <= 4608) f.template run<9, 512, 1>();
   else if (cols <= 8192) f.template run<8, 512, 2>();
   else return false;
   return true;
@@ -141,7 +151,7 @@ struct Raw {
   // The loads have returned behind this.  (A wave may use what it has loaded behind a rendezvous; without this the wait for it would
   // lie there too, and another wave could store to the place first.)
   __device__ __forceinline__ void arrived() {
-    static_assert(V == 8, "wide rows");
+    static_assert(V >= 8, "wide rows");
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       int w[sizeof(v[j]) / 4];
@@ -149,6 +159,12 @@ struct Raw {
 #pragma unroll
       for (int i = 0; i < (int)(sizeof(w) / 4); ++i) asm volatile("" : "+v"(w[i]));
       __builtin_memcpy(&v[j], w, sizeof(w));
+      if constexpr (V == 9) {
+        int last = 0;
+        __builtin_memcpy(&last, &one[j], sizeof(T));
+        asm volatile("" : "+v"(last));
+        __builtin_memcpy(&one[j], &last, sizeof(T));
+      }
     }
   }
 };

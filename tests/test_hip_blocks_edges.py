@@ -6,6 +6,7 @@ import ctypes
 import pytest
 import torch
 
+import test_hip_blocks as T
 from oracle import blocks_torch as O
 
 pytestmark = pytest.mark.gpu
@@ -222,3 +223,29 @@ def test_a_sigmoid_gate_that_is_nearly_shut(blocks):
   near = (r - want).abs() <= 12 * 2.0 ** -24 * want
   normal = want >= 2.0 ** -126 * (1 + 2.0 ** -20)
   assert bool(near[normal].all()) and bool((near | (r == 0))[~normal].all()) and 0 < int(normal.sum()) < 100
+
+
+# ---- rows of a little more than a power of two ----
+@pytest.mark.parametrize('kind', [0, 1, 2, 3])
+@pytest.mark.parametrize('cols', [2050, 2057, 2303, 2304, 2305, 4097, 4103, 4607, 4608, 4609])
+def test_norm_of_nine_columns_a_lane(blocks, cols, kind):
+  """Every output against float64 at the edges of these widths (tolerances of tests/test_hip_blocks.py)."""
+  T.check_norm(blocks, cols + kind, (3, 5), cols, *T.TYPES[kind], *T.KINDS[kind])
+
+
+@pytest.mark.parametrize('cols', [2050, 2304, 4100])
+def test_norm_of_nine_columns_a_lane_over_its_inputs(blocks, cols):
+  """r over x and z over h, dx over dr and dh over h: a workgroup's waves that hold the same columns, clips cut into segments."""
+  from advoc_amd import _lib
+  norm, d, call, g, (r, z, stats) = T.check_norm(blocks, 2, (200, 3), cols, 'f32', 'f32', 'rms', 'layer', 'clip', 'sigmoid', 0.9)
+  h, x = d['h'].clone(), d['x'].clone()
+  norm.forward(h, x, r=x, z=h, **call)
+  assert torch.equal(x, r) and torch.equal(h, z)
+  h, dr = d['h'].clone(), d['dr'].clone()
+  q = T.descriptor(norm, r, d['gate'], call)
+  for name, t in (('dz', d['dz']), ('dr', dr), ('dx', dr), ('h', h), ('dh', h)):
+    getattr(q, name).p, getattr(q, name).pitch = t.data_ptr(), cols
+  q.stats = stats.data_ptr()
+  assert _lib.load().advoc_residual_norm_workspace_bytes(ctypes.byref(q)) == 0
+  _lib.check(_lib.load().advoc_residual_norm_backward(ctypes.byref(q), _lib.stream()))
+  assert torch.equal(dr, g.dx) and torch.equal(h, g.dh)
