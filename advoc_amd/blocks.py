@@ -7,15 +7,17 @@ taken, rows may be padded (unit stride inside a row, one distance between rows).
 stream of the tensors' device and can be captured into a graph.  None takes part in torch's autograd: gradients come from the
 backward calls below, and a tensor that autograd follows is refused while it is on (parameters of a norm are taken as they are).
 
-  z, x8   = one block:   z = N_pre(x);  y = W z;  r = x + alpha * scale * gate * dropout(N_post(y));  next z = N_pre(r)
+  one block:   z = N_pre(x);   y = W z;   r = x + alpha * scale * gate * dropout(N_post(y));   next block's z1 = N_pre(r)
 
-  norm = blocks.ResidualNorm(cols, post='rms', pre='rms', w_post=..., scale=..., w_pre=..., keep_prob=0.9)
-  y = blocks.matmul_nt_f8(blocks.quantize_f8(z), w8, out_dtype=z.dtype)          # w8 = blocks.quantize_f8(w), once
-  r, z, stats = norm.forward(y, x, gate=gate, seed=step, save=True)
-  g = norm.backward(dz, dr, y, r, stats, gate=gate, seed=step)                   # g.dh is dL/dy, g.dx dL/dx
-  dy, dyt = blocks.quantize_f8_both(g.dh, 'e5m2')
-  dz = blocks.matmul_nt_f8(dy, w8t)                                              # w8t = blocks.quantize_f8_transposed(w)
-  dw = blocks.matmul_nt_f8(dyt, z8t)                                             # z8t = blocks.quantize_f8_transposed(z)
+  norm = blocks.ResidualNorm(cols, post='rms', pre='rms', w_post=w_post, scale=scale, w_pre=w_pre, keep_prob=0.9)
+  w8, w8t = blocks.quantize_f8(w), blocks.quantize_f8_transposed(w)              # once per update of w [cols, cols]
+  z8, z8t = blocks.quantize_f8_both(z)                                           # z8t is for dw
+  y = blocks.matmul_nt_f8(z8, w8, out_dtype=z.dtype)
+  r, z1, stats = norm.forward(y, x, gate=gate, seed=step, save=True)
+  g = norm.backward(dz1, dr, y, r, stats, gate=gate, seed=step)                  # g.dh is dL/dy, g.dx dL/dx
+  dy8, dy8t = blocks.quantize_f8_both(g.dh, 'e5m2')
+  dz = blocks.matmul_nt_f8(dy8, w8t, out_dtype=z.dtype)                          # the dz1 of the block before
+  dw = blocks.matmul_nt_f8(dy8t, z8t)
 """
 import collections
 import functools

@@ -50,16 +50,6 @@ struct vec8 {
   typedef T type __attribute__((ext_vector_type(8)));
 };
 
-template <typename T>
-__device__ __forceinline__ f32x8 load8(const T* p) {
-  typename vec8<T>::type v;
-  __builtin_memcpy(&v, p, sizeof(v));
-  f32x8 f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) f.v[k] = (float)v[k];
-  return f;
-}
-
 // nearest, ties to even (v_cvt_pk_bf16_f32 and v_cvt_f16_f32 in the default mode)
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const f32x8& f) {

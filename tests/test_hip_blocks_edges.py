@@ -249,3 +249,18 @@ def test_norm_of_nine_columns_a_lane_over_its_inputs(blocks, cols):
   assert _lib.load().advoc_residual_norm_workspace_bytes(ctypes.byref(q)) == 0
   _lib.check(_lib.load().advoc_residual_norm_backward(ctypes.byref(q), _lib.stream()))
   assert torch.equal(dr, g.dx) and torch.equal(h, g.dh)
+
+
+def test_the_modules_example(blocks):
+  """The block of the module's text, twice in a row in 16 bits: what one block hands back is what the one before takes."""
+  import textwrap
+  lines = textwrap.dedent(blocks.__doc__[blocks.__doc__.index('  norm = blocks'):])
+  cols, r = 136, lambda *s: torch.randn(*s, generator=gen(sum(s))).cuda()      # noqa: E731
+  f = dict(blocks=blocks, cols=cols, w_post=r(cols), scale=r(cols), w_pre=r(cols), w=r(cols, cols) * cols ** -0.5, step=3, x=r(2, 9, cols),
+           gate=r(2, 1, cols).bfloat16(), z=r(2, 9, cols).bfloat16(), dz1=r(2, 9, cols).bfloat16(), dr=r(2, 9, cols))
+  for _ in range(2):
+    exec(lines, f)
+    assert f['y'].dtype == f['dz'].dtype == f['z1'].dtype == torch.bfloat16 and f['dw'].dtype == torch.float32
+    assert f['dz'].shape == (18, cols) and f['dw'].shape == (cols, cols) and f['g'].dh.shape == f['y'].shape
+    assert all(bool(torch.isfinite(f[k]).all()) for k in ('r', 'z1', 'dz', 'dw'))
+    f.update(dz1=f['dz'].view(2, 9, cols), dr=f['g'].dx)                       # one block back
