@@ -377,9 +377,46 @@ __global__ __launch_bounds__(576) void lws_causal_fast_kernel(const CausalParams
 // + cl, j = the lane's index), so W[q][p][(cl + p) mod 4] is one scalar load per (q, p), and rows are stored as four
 // PLANES by bin mod 4 -- bin m at plane m & 3, index (m + 4) >> 2 -- so that the lanes of a wave read consecutive words
 // (bins 4 apart in an interleaved row would hit 4 of the 32 banks).  Eight accumulators per thread, no per-thread weights.
+//
+// With windows that are symmetric (awin[n] = awin[nfft - 1 - n], as every one of the reference's is) the weights are real numbers but
+// for a turn: the product awin[n] swin[n - q nhop] is symmetric about (nfft - 1) / 2 + q nhop / 2, so that with c = (nfft - 1) / nfft
+//   W[q][p][(f + p) mod 4] = rho_q(p) exp(i pi p c) exp(-i pi q (2 f + p) / 4),     rho real.
+// The first turn splits into exp(i pi (f + p) c) on the data and exp(-i pi f c) on the sum: rows are turned when they are written to
+// LDS, sums when they are complete.  The second is one of eight, S = (2 f + p) mod 8 is the same for a wave, and q S / 8 of a turn is
+// a matter of which of x, y, x + y, y - x is added with which sign.  A tap is two multiply-adds then instead of four (the library is
+// built without packed fp32 instructions, which did four in two: 100 sweeps of 256 clips of speech took 24.1 ms with those, 31.4 with
+// four scalar ones, 23.6 with two; of noise, every tile active, 19.3, 24.6, 18.9).  A workgroup tells from the table whether it may: where an imaginary part of rho is more than the table's rounding
+// (2^-21 of the largest weight), it takes the weights as they are.
 constexpr int kPlane = 132;                     // float2 per plane: bins -4 .. 516 -> indices 0 .. 130
 constexpr int kPRow = 4 * kPlane;               // float2 per planar row
 __device__ __forceinline__ int planar(int m) { return (m & 3) * kPlane + ((m + 4) >> 2); }
+
+// exp(i pi m (nfft - 1) / nfft) for nfft = 1024, m in 0 ... 512
+__device__ __forceinline__ float2 half_turn(int m) {
+  float sn, cs;
+  sincospif((float)m * (1.f / 1024.f), &sn, &cs);
+  return (m & 1) ? make_float2(-cs, sn) : make_float2(cs, -sn);
+}
+
+// What the taps of one p add to the frames' sums with real weights (those of odd q and p, an odd number of eighths, times sqrt 1/2)
+template <int S>
+__device__ __forceinline__ void real_taps(float2 (&z)[kSweepFrames], const float2* __restrict__ column, const float (&w)[2 * kFQ - 1]) {
+#pragma unroll
+  for (int R = 0; R < kSweepFrames + 2 * (kFQ - 1); ++R) {
+    const float2 x = column[R * kPRow];
+    const float2 e = (S & 1) ? make_float2(x.x + x.y, x.y - x.x) : x;      // an eighth of a turn on, times sqrt 2
+#pragma unroll
+    for (int qi = 0; qi < 2 * kFQ - 1; ++qi) {
+      const int tt = R - qi;
+      if (tt < 0 || tt >= kSweepFrames) continue;
+      const int k = ((qi - (kFQ - 1)) * S) & 7;                            // eighths of a turn back
+      const float2 v = (k & 1) ? e : x;
+      const int quarter = k >> 1;
+      z[tt].x = fmaf(w[qi], quarter == 0 ? v.x : quarter == 1 ? v.y : quarter == 2 ? -v.x : -v.y, z[tt].x);
+      z[tt].y = fmaf(w[qi], quarter == 0 ? v.y : quarter == 1 ? -v.x : quarter == 2 ? -v.y : v.x, z[tt].y);
+    }
+  }
+}
 
 __global__ __launch_bounds__(576) void lws_sweep_fast_kernel(const float2* __restrict__ in, float2* __restrict__ out,
                                                              const float* __restrict__ mag,
@@ -395,26 +432,46 @@ __global__ __launch_bounds__(576) void lws_sweep_fast_kernel(const float2* __res
   if (tile_max && !(tile_max[blockIdx.x] > thr_mult * mean_mag[clip])) return;
   const int t0 = (blockIdx.x - clip * tiles_per_clip) * kSweepFrames;
   const float2* src = in + (int64_t)clip * T * kFBins;
-  // ---- the tile's rows, coalesced (thread = bin), into the planar layout with the mirrored bins either side ----
-  {
-    const int b = threadIdx.x;
-    if (b < kFBins) {
-      float2 vr[kRows];                                    // every row's load in flight before the first LDS write
+  // ---- the tile's rows, coalesced (thread = bin): every row's load in flight before the first LDS write ----
+  float2 vr[kRows];
+  const int b = threadIdx.x;
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const int t = t0 - (kFQ - 1) + r;
-        vr[r] = make_float2(0.f, 0.f);
-        if (t >= 0 && t < T) vr[r] = src[(int64_t)t * kFBins + b];
-      }
+  for (int r = 0; r < kRows; ++r) {
+    const int t = t0 - (kFQ - 1) + r;
+    vr[r] = make_float2(0.f, 0.f);
+    if (b < kFBins && t >= 0 && t < T) vr[r] = src[(int64_t)t * kFBins + b];
+  }
+  // ---- the weights as real numbers, [p][q] ----
+  __shared__ float rho[kFKW][8];
+  __shared__ int complex_weight[64];
+  if (threadIdx.x < 64) {
+    int bad = 0;
+    if (threadIdx.x < (2 * kFQ - 1) * kFKW) {
+      const int qi = threadIdx.x / kFKW, pi = threadIdx.x - qi * kFKW, q = qi - (kFQ - 1), p = pi - (kFL - 1);
+      const float2 w = W[(qi * kFKW + pi) * kFP], turn = half_turn(p < 0 ? -p : p);
+      float sn, cs;
+      sincospif(0.25f * (float)(p * q), &sn, &cs);
+      const float2 u = cmul(make_float2(turn.x, p < 0 ? -turn.y : turn.y), make_float2(cs, sn));      // rho = w conj(u)
+      const float re = w.x * u.x + w.y * u.y, im = w.y * u.x - w.x * u.y;
+      bad = !(fabsf(im) <= 4.76837158e-7f * fabsf(W[((kFQ - 1) * kFKW + kFL - 1) * kFP].x));
+      rho[pi][qi] = p == 0 && q == 0 ? 0.f : (p & q & 1) ? re * 0.70710678118654752f : re;            // the bin itself is not a tap
+    }
+    complex_weight[threadIdx.x] = bad;
+  }
+  __syncthreads();
+  const bool real = __ballot(complex_weight[threadIdx.x & 63]) == 0;
+  // ---- into the planar layout with the mirrored bins either side ----
+  if (b < kFBins) {
+    const float2 turn = real ? half_turn(b) : make_float2(1.f, 0.f);
+    const float beyond = real ? -1.f : 1.f;              // exp(i pi 1024 c) = -1
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const float2 v = vr[r];
-        float2* row = rows + r * kPRow;
-        row[planar(b)] = v;
-        const float2 cv = make_float2(v.x, -v.y);          // bin m < 0 is conj(bin -m), bin m >= 513 is conj(bin 1024 - m)
-        if (b >= 1 && b <= kFH) row[planar(-b)] = cv;
-        if (b >= kFBins - 1 - kFH && b <= kFBins - 2) row[planar(2 * (kFBins - 1) - b)] = cv;
-      }
+    for (int r = 0; r < kRows; ++r) {
+      const float2 v = real ? cmul(vr[r], turn) : vr[r];
+      float2* row = rows + r * kPRow;
+      row[planar(b)] = v;
+      const float2 cv = make_float2(v.x, -v.y);          // bin m < 0 is conj(bin -m), bin m >= 513 is conj(bin 1024 - m)
+      if (b >= 1 && b <= kFH) row[planar(-b)] = cv;
+      if (b >= kFBins - 1 - kFH && b <= kFBins - 2) row[planar(2 * (kFBins - 1) - b)] = make_float2(beyond * cv.x, beyond * cv.y);
     }
   }
   // ---- wave -> residue class, lane -> index within it: waves 0-2 class 0 (129 bins), 3-4 / 5-6 / 7-8 classes 1 / 2 / 3 ----
@@ -437,13 +494,30 @@ __global__ __launch_bounds__(576) void lws_sweep_fast_kernel(const float2* __res
   }
   const bool wave_active = __ballot(any && live) != 0;
   __syncthreads();
-  f2v z[kSweepFrames];
+  float2 z[kSweepFrames];
 #pragma unroll
-  for (int tt = 0; tt < kSweepFrames; ++tt) z[tt] = (f2v){0.f, 0.f};
+  for (int tt = 0; tt < kSweepFrames; ++tt) z[tt] = make_float2(0.f, 0.f);
 #pragma unroll 1                                          // (unrolled, the scheduler hoists all 126 reads and spills)
   for (int p = wave_active ? -(kFL - 1) : kFL; p <= kFL - 1; ++p) {
     const int cp = cl + p;                                // uniform
     const int off = (cp & 3) * kPlane + ((cp + 4) >> 2) + j;
+    if (real) {
+      float w[2 * kFQ - 1];
+#pragma unroll
+      for (int qi = 0; qi < 2 * kFQ - 1; ++qi) w[qi] = rho[p + kFL - 1][qi];
+      const float2* column = rows + off;
+      switch ((2 * cl + p) & 7) {
+        case 0: real_taps<0>(z, column, w); break;
+        case 1: real_taps<1>(z, column, w); break;
+        case 2: real_taps<2>(z, column, w); break;
+        case 3: real_taps<3>(z, column, w); break;
+        case 4: real_taps<4>(z, column, w); break;
+        case 5: real_taps<5>(z, column, w); break;
+        case 6: real_taps<6>(z, column, w); break;
+        case 7: real_taps<7>(z, column, w); break;
+      }
+      continue;
+    }
     float2 w[2 * kFQ - 1];
 #pragma unroll
     for (int qi = 0; qi < 2 * kFQ - 1; ++qi) w[qi] = W[(qi * kFKW + p + kFL - 1) * kFP + (cp & 3)];      // scalar loads
@@ -455,17 +529,23 @@ __global__ __launch_bounds__(576) void lws_sweep_fast_kernel(const float2* __res
       for (int qi = 0; qi < 2 * kFQ - 1; ++qi) {
         const int tt = R - qi;                            // row R = frame tt + (Q - 1) + q, q = qi - (Q - 1)
         if (tt < 0 || tt >= kSweepFrames) continue;
-        cmac(z[tt], w[qi], x);
+        f2v zz = {z[tt].x, z[tt].y};
+        cmac(zz, w[qi], x);
+        z[tt] = make_float2(zz.x, zz.y);
       }
     }
   }
+  if (!wave_active && tile_max) return;                   // (sparse: `out` holds these bins already, as above)
+  const float2 back = half_turn(f);
 #pragma unroll
   for (int tt = 0; tt < kSweepFrames; ++tt) {
     if (tt >= nt) break;
     const int64_t i = ((int64_t)clip * T + t0 + tt) * kFBins + f;
-    float2 v = rows[(tt + kFQ - 1) * kPRow + planar(f)];
-    if (a[tt] > thr) v = with_phase_of(a[tt], make_float2(z[tt].x, z[tt].y), v);
-    if (live) out[i] = v;
+    const bool updated = a[tt] > thr;
+    if (!live || (!updated && tile_max)) continue;
+    float2 v = src[(int64_t)(t0 + tt) * kFBins + f];      // (as it is: a bin that is not updated keeps its bits)
+    if (updated) v = with_phase_of(a[tt], real ? cmul(z[tt], make_float2(back.x, -back.y)) : z[tt], v);
+    out[i] = v;
   }
 }
 
