@@ -1,7 +1,7 @@
 // Dropout whose mask is never stored (gfx950): y_i = x_i / keep where word i of the Philox stream (philox.h) is kept, exactly 0
 // elsewhere whatever x_i holds; the gradient is the same call on dy.  Reads and writes each element once: no byte of mask in
-// HBM, and the backward pass draws the same words again.  HBM-bound: 65536 x 1024 bf16 (268 MB) in 43 us, 6.2 TB/s, a copy's rate
-// (45 with the loads behind the drawing); 8192 x 513 fp16 in padded rows 8.4, one round of workgroups; one frame takes the 6.6 us of a
+// HBM, and the backward pass draws the same words again.  HBM-bound: 65536 x 1024 bf16 (268 MB) in 43 us, 6.2 TB/s (adding 1
+// to as much: 46 to 48 us; 45 with the loads behind the drawing); 8192 x 513 fp16 in padded rows 8.4, one round of workgroups; one frame takes the 6.6 us of a
 // call.
 #include "philox.h"
 #include "rows.h"

@@ -108,9 +108,10 @@ __device__ __forceinline__ void store_part(const Args& g, int64_t row, int64_t c
 
 // ---- one or two rows: dot products ----
 // A wave is one row of b and reads it in pieces of 1024 bytes, 16 a lane, all of up to 8192 in flight together; a lane's products are
-// summed in fp32 and take their two exponents once per piece.  Bound by the weights' latency: 1 x 512 x 8192 3.9 us a call and 1 x
-// 4096 x 4096 4.2 (the thin kernel: 8.4 and 6.4; the host's share of a call alone is 3.9); from three rows on its arithmetic costs
-// more (3 x 4096 x 4096: 8.1, thin 6.5).
+// summed in fp32 and take their two exponents once per piece.  Bound by the weights' latency, and with 512 rows of b half of the
+// CUs have no workgroup: 1 x 512 x 8192 3.5 us with the weights in a cache, 5.5 to 5.9 from HBM; 1 x 4096 x 4096 3.7 and 6.4.  (Calls
+// with the same weights again and again: 3.9 and 4.2, the thin kernel 8.4 and 6.4.)  From three rows on its arithmetic costs more (3 x
+// 4096 x 4096: 8.1, thin 6.5).
 template <int F>
 __device__ __forceinline__ void widen(int word, float (&v)[4]) {
   if constexpr (F == ADVOC_E4M3) {
@@ -180,8 +181,8 @@ __global__ __launch_bounds__(256) void f8_dot_kernel(Args g) {
 // ---- three to 16 rows: the weights are read once, by whoever multiplies them ----
 // A workgroup is 16 rows of b; its waves take the blocks of the contraction in turn, straight from memory to registers (lane
 // group g the 16-byte pieces g and g + 4 of 16 rows, so that a load covers half lines whole), and meet in LDS in wave order.
-// Bound by the weights' latency and, with few columns, by the lines a CU asks for: 4 x 4096 x 4096 6.6 us (2.5 TB/s), 4 x 512 x 8192
-// 9.4 (32 workgroups).
+// Bound by the weights' latency and, with few columns, by the lines a CU asks for: 4 x 4096 x 4096 6.0 us, 7.2 with the weights from HBM
+// (2.3 TB/s), 4 x 512 x 8192 9.4 (32 workgroups).
 template <typename O, bool EXACT, int FA, int FB>
 __global__ __launch_bounds__(1024) void f8_thin_kernel(Args g) {
   extern __shared__ f32x4 red[];
@@ -429,7 +430,10 @@ __device__ __forceinline__ void settled(f32x4& c) { asm volatile("" : "+v"(c)); 
 // half of the workgroup read the fragments of a block from LDS (24 reads of 16 bytes a lane: 768 cycles of the CU's 128 bytes a
 // cycle for four waves), the other half multiplies the block before (32 instructions of 32 cycles), with a rendezvous between; the
 // matrix pipe has work in both halves of a block's time.  16384 x 4096 x 4096: 231 us, 2.38 PFLOP/s; 4096 x 4096 x 8192: 100 us, 2.74
-// (a library product of 8-bit matrices of 8192 reaches 2.69).
+// (a library product of 8-bit matrices of 8192 reaches 2.69).  Stamped in a run of 1500 calls: 2.07 GHz, a tile of 32 blocks 4600 cycles
+// to begin, 107000 for its blocks, 4400 to store; the matrix cores' 2048 cycles a block are 0.61 of those.  What the rest is: with
+// reads, fetches and stores left out a call still took 205 of the 243 us it took then, so most of it is the way an instruction with
+// two exponent registers issues and the rendezvous between the halves, a sixth the fragments and fetches that show through.
 template <typename O, int FA, int FB>
 __global__ __launch_bounds__(512) void f8_big_kernel(Args g) {
   using T = Tile<O, 256, 256, 128, 64, 2>;

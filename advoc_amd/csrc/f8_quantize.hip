@@ -105,7 +105,7 @@ struct Args {
   int64_t kp, sp, mp, sp_t;      // row pitches of the outputs
 };
 
-// Blocks of rows: 16 lanes x 8 values are a block.  16384 x 4096 bf16 (201 MB): 43.5 us, 4.6 TB/s; a copy of that size takes 39.
+// Blocks of rows: 16 lanes x 8 values are a block.  16384 x 4096 bf16 (202 MB): 44 us, 4.6 TB/s; adding 1 to as much takes 36.
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(Args a) {
   const int sub = threadIdx.x & 15;
@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(Args a) {
 // magnitude meets over 4 lanes and, in LDS, over the 4 waves; the bytes of a column are turned around through LDS and leave as whole
 // 128-byte lines.  ROWS: the row blocks of the same tile as well, from the same registers.
 // Bound by HBM and by the load, arithmetic and store of one round of workgroups not overlapping: 16384 x 1024 bf16, both forms, in
-// 17 us (67 MB, 3.9 TB/s; a copy of that size takes 13).  What it took from 24: the largest magnitude as an integer maximum that
+// 17 us (67 MB, 3.9 TB/s; adding 1 to as much takes 11, or 14 where no cache holds it).  What it took from 24: the largest magnitude as an integer maximum that
 // looks at infinities only where there are any, lanes met by moves instead of LDS, the division by the scale inside the conversion,
 // the turned bytes without bank conflicts, 65 registers instead of 167 (four workgroups to a CU).
 template <typename T, int FMT, bool ROWS>

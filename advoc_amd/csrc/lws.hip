@@ -385,8 +385,8 @@ __global__ __launch_bounds__(576) void lws_causal_fast_kernel(const CausalParams
 // LDS, sums when they are complete.  The second is one of eight, S = (2 f + p) mod 8 is the same for a wave, and q S / 8 of a turn is
 // a matter of which of x, y, x + y, y - x is added with which sign.  A tap is two multiply-adds then instead of four (the library is
 // built without packed fp32 instructions, which did four in two: 100 sweeps of 256 clips of speech took 24.1 ms with those, 31.4 with
-// four scalar ones, 23.6 with two; of noise, every tile active, 19.3, 24.6, 18.9).  A workgroup tells from the table whether it may: where an imaginary part of rho is more than the table's rounding
-// (2^-21 of the largest weight), it takes the weights as they are.
+// four scalar ones, 23.6 with two; of noise, every tile active, 19.3, 24.6, 18.9).  A workgroup tells from the table whether it may:
+// where an imaginary part of rho is more than the table's rounding (2^-21 of the largest weight), it takes the weights as they are.
 constexpr int kPlane = 132;                     // float2 per plane: bins -4 .. 516 -> indices 0 .. 130
 constexpr int kPRow = 4 * kPlane;               // float2 per planar row
 __device__ __forceinline__ int planar(int m) { return (m & 3) * kPlane + ((m + 4) >> 2); }

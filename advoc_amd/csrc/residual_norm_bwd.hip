@@ -6,17 +6,19 @@
 //   dgate = sum e scale (hhat w_post + b_post) act'(gate)
 //   dw_post = scale E1,  db_post = scale E0,  dscale = w_post E1 + b_post E0;      dw_pre = sum dz rhat, db_pre = sum dz
 //
-// Four column sums give the five parameter gradients: what is constant in a column stays outside its sums.  One pass: the five
+// Four column sums in registers give the five parameter gradients: what is constant in a column stays outside its sums, and is
+// multiplied in when a workgroup's sums leave it (five of them, those that are wanted).  One pass: the five
 // inputs of a row are read once and the three outputs written once; the mask is drawn again.  The sums live in registers while a
 // worker (the lanes of one row) walks over its rows, meet in LDS per workgroup and in HBM once per workgroup; a second small launch
 // adds those up in a fixed order (no atomics: two runs give the same bits).  A gate row shared by the frames of a clip is summed the
 // same way, a worker's rows never crossing a clip: G0 = sum e, G1 = sum e hhat over them give dgate = scale (w_post G1 + b_post G0)
 // act' and their part of E0, E1.
 //
-// Measured (kernel + the second launch): 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (302 MB): 67 + 5 us, 4.5
-// TB/s (69 + 6 when every worker of a clip left its part of the gate's gradient in memory, not every workgroup); each further row comes at 5.0 TB/s, a copy's rate, and 12 us are the way of the first row (arguments and vectors 4, loads 2,
-// arithmetic 4, the workgroup's column sums 3).  4096 x 4096 fp16 (201 MB, and 25 MB of column sums): 51 + 5.  3999 x 513 fp32 (66
-// MB): 21 + 4, two rows a worker: the same start, and the arithmetic.
+// Measured (kernel + the second launch): 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (302 MB): 68 + 5 us, 4.4
+// TB/s; each further row comes at 5.0 TB/s (adding 1 to as much: 5.8), and 12 us are the way of the first row (arguments and vectors 4,
+// loads 2, arithmetic 4, the workgroup's column sums 3).  (A gate's gradient that left every worker instead of every workgroup: 69 + 6.)
+// 4096 x 4096 fp16 (201 MB, and 21 MB of column sums written and read again): 52 + 5.  3999 x 513 fp32 (66 MB): 21 + 4, two rows a
+// worker: the same start and end, and the arithmetic.
 #include "residual_norm.h"
 
 namespace {
@@ -33,7 +35,7 @@ struct Sums {
 
 // Two waves to a SIMD, 256 registers to a lane: rows of 16 columns a lane need them all, a third for the sums, and have 512 lanes to a
 // workgroup (half the partial column sums of 256); rows of 8 columns a lane use the rest to fetch a row ahead, which is worth more
-// than a third wave (16384 x 256: 24 -> 20 us, 8192 x 2048: 80 -> 74, 4096 x 4096 fp16: 60 -> 51).
+// than a third wave (16384 x 256: 24 -> 20 us, 8192 x 2048: 80 -> 74, 4096 x 4096 fp16: 60 -> 52).
 constexpr int kWavesPerSimd = 2;
 template <int L, int NV>
 constexpr int kLanes = L > 64 ? L : NV > 1 ? 512 : 256;
