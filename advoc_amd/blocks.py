@@ -388,7 +388,8 @@ def _product_workspace(m, n, k, code):
 def matmul_nt_f8(a, b, out_dtype=None, out=None, accumulate=False):
   """a b^T of two F8Matrix operands with the same k -> [a.rows, b.rows] (``advoc_matmul_nt_f8``); a float32 result is
   accumulated in fp32 throughout, a 16-bit one in the 8-bit matrix instruction's sums, at twice the rate and 1.5e-5 off in norm
-  (bounds in include/advoc_hip.h).  out_dtype: that of `out`, without one float32.  accumulate: add to `out` (float32), e.g. a gradient arena's slice."""
+  (bounds in include/advoc_hip.h).  out_dtype: that of `out`, without one float32.  accumulate: add to `out` (float32), e.g. a
+  gradient arena's slice."""
   if not isinstance(a, F8Matrix) or not isinstance(b, F8Matrix) or a.k != b.k or a.buffer.device != b.buffer.device:
     raise _lib.AdvocHipError('two F8Matrix operands with the same k on one device are needed')
   device, m, n = a.buffer.device, a.rows, b.rows

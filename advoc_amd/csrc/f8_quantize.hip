@@ -132,9 +132,9 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(Args a) {
 // magnitude meets over 4 lanes and, in LDS, over the 4 waves; the bytes of a column are turned around through LDS and leave as whole
 // 128-byte lines.  ROWS: the row blocks of the same tile as well, from the same registers.
 // Bound by HBM and by the load, arithmetic and store of one round of workgroups not overlapping: 16384 x 1024 bf16, both forms, in
-// 17 us (67 MB, 3.9 TB/s; adding 1 to as much takes 11, or 14 where no cache holds it).  What it took from 24: the largest magnitude as an integer maximum that
-// looks at infinities only where there are any, lanes met by moves instead of LDS, the division by the scale inside the conversion,
-// the turned bytes without bank conflicts, 65 registers instead of 167 (four workgroups to a CU).
+// 17 us (67 MB, 3.9 TB/s; adding 1 to as much takes 11, or 14 where no cache holds it).  What it took from 24: the largest magnitude
+// as an integer maximum that looks at infinities only where there are any, lanes met by moves instead of LDS, the division by the
+// scale inside the conversion, the turned bytes without bank conflicts, 65 registers instead of 167 (four workgroups to a CU).
 template <typename T, int FMT, bool ROWS>
 __global__ __launch_bounds__(256, 4) void quantize_tile_kernel(Args a) {
   __shared__ __align__(16) uint32_t cm[4][kBlock];

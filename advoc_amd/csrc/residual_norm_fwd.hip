@@ -34,7 +34,8 @@ __device__ __forceinline__ void row_stats(const Vals<V> (&a)[NV], const int (&du
 
 // Vectors in LDS: five, and four where a row is a workgroup's: five of 2048 or 4096 columns and the sums' place are more than a CU's
 // 160 KB over the workgroups that its waves allow, and one of those then waits for a round of its own (8192 x 2048 bf16: 50 us, four
-// vectors 45; 4096 x 4096 fp16: 39, 33; with five vectors and the launch cut to what fits 44 and 35).  There a lane holds its part of b_pre in registers; with 16 columns a lane it reads it for each row.
+// vectors 45; 4096 x 4096 fp16: 39, 33; with five vectors and the launch cut to what fits 44 and 35).  There a lane
+// holds its part of b_pre in registers; with 16 columns a lane it reads it for each row.
 template <int L>
 constexpr int kVectors = L > 64 ? 4 : 5;
 
@@ -52,9 +53,9 @@ constexpr int lds_taken(int cols) {
 // (measured with five vectors: 8192 x 2048 50 us, without 55; 4096 x 4096 50, without 62); with 16 they would spill (16384 x 1024: 38
 // us, with them 65).  A wave waits for its loads and stores in the order of their issue, so that the number of stores behind the loads
 // is to be known where the loads are waited for: hence the templates.
-// 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (202 MB): 36.6 us, 5.5 TB/s (adding 1 to as much: 36.4).  Rows of a whole
-// workgroup meet four times on their way: 4096 x 4096 in the same types 50 us, 4.0 TB/s, 8192 x 2048 48.  16384 x 513: 25 us, 4.0 TB/s, bound by arithmetic (rows at
-// odd offsets, three Philox blocks for nine words).  One row: 3 us, latency.
+// 16384 x 1024, bf16 with fp32 residuals, a gate per clip, dropout (202 MB): 36.6 us, 5.5 TB/s (adding 1 to as much: 36.4).  Rows of a
+// whole workgroup meet four times on their way: 4096 x 4096 in the same types 50 us, 4.0 TB/s, 8192 x 2048 48.  16384 x 513: 25 us, 4.0
+// TB/s, bound by arithmetic (rows at odd offsets, three Philox blocks for nine words).  One row: 3 us, latency.
 template <typename T, typename R, int V, int L, int NV, int WG, bool H, bool PRE>
 __global__ __launch_bounds__(WG, kWavesPerSimd) void norm_forward_kernel(NormArgs a) {
   using Row = Team<L, WG>;

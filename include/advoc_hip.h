@@ -649,15 +649,17 @@ int advoc_f8_quantize(const void* x, int64_t x_pitch, int64_t rows, int64_t cols
                       uint8_t* scale, uint8_t* qt, uint8_t* scale_t, advoc_stream_t stream);
 
 /* out[i, j] = sum_k a[i, k] b[j, k] of two quantised matrices (m and n rows, the same k; formats may differ), like
- * advoc_matmul_nt_f32.  The output's type is the choice of the sums' too.  ADVOC_F32: fp32 throughout, the operands' values as bfloat16,
- * which is exact but below 2^-130 (rounded to multiples of 2^-133) and for what quantising rounded up to 2^128 (infinite); who needs
- * such sums in 16 bits takes an ADVOC_F32 output and rounds it.  16-bit outputs take the 8-bit matrix instruction at twice the rate: it
- * adds up in fp32 but for products below 2^-13 of the largest of eight neighbours, which it drops (1.5e-5 of the result in norm; their
- * own rounding is 1.7e-3 or 2e-4).  One or two rows are summed in fp32 whatever the output.  out [m, n] dense; accumulate != 0 (out_dtype ADVOC_F32) adds to it.
+ * advoc_matmul_nt_f32.  out [m, n] dense; accumulate != 0 (out_dtype ADVOC_F32) adds to it.
+ * The output's type is the choice of the sums' too.
+ *   ADVOC_F32  fp32 throughout, the operands' values as bfloat16, which is exact but below 2^-130 (rounded to multiples of
+ *              2^-133) and for what quantising rounded up to 2^128 (infinite); who needs such sums in 16 bits rounds this output
+ *   16 bits    the 8-bit matrix instruction at twice the rate: it adds up in fp32 but for products below 2^-13 of the largest of
+ *              eight neighbours, which it drops (1.5e-5 of the result in norm; their own rounding is 1.7e-3 or 2e-4)
+ * One or two rows are summed in fp32 whatever the output, without those limits.
  * workspace: advoc_matmul_nt_f8_workspace_bytes(m, n, k, out_dtype) bytes, 4-byte aligned (0: may be NULL); with too little the
  * product runs unsplit.  k <= 8 000 000, and the launch may take 2^32 - 1 work-items (up to 16 rows: n < 2^26 always does;
- * otherwise fewer than 2^36 outputs, in whole tiles, do); ADVOC_ERR_UNSUPPORTED beyond.  The order of every sum is fixed by the shapes: two
- * calls give the same bits. */
+ * otherwise fewer than 2^36 outputs, in whole tiles, do); ADVOC_ERR_UNSUPPORTED beyond.
+ * The order of every sum is fixed by the shapes: two calls give the same bits. */
 int64_t advoc_matmul_nt_f8_workspace_bytes(int64_t m, int64_t n, int64_t k, int32_t out_dtype);
 int advoc_matmul_nt_f8(const uint8_t* a, const uint8_t* a_scale, int32_t a_format, const uint8_t* b, const uint8_t* b_scale,
                        int32_t b_format, void* out, int32_t out_dtype, int32_t accumulate, int64_t m, int64_t n, int64_t k,

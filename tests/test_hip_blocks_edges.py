@@ -264,3 +264,23 @@ def test_the_modules_example(blocks):
     assert f['dz'].shape == (18, cols) and f['dw'].shape == (cols, cols) and f['g'].dh.shape == f['y'].shape
     assert all(bool(torch.isfinite(f[k]).all()) for k in ('r', 'z1', 'dz', 'dw'))
     f.update(dz1=f['dz'].view(2, 9, cols), dr=f['g'].dx)                       # one block back
+
+
+@pytest.mark.parametrize('cols', [5, 200, 520, 1000, 2048, 2050, 4096, 4100, 8192])
+@pytest.mark.parametrize('dt,res', [('f32', 'f32'), ('bf16', 'f32'), ('f16', 'f16')])
+def test_norm_before_the_first_block_at_every_width(blocks, cols, dt, res):
+  """z = N_pre(x) alone, with weight and bias, and its gradients."""
+  t, p, kw, _ = T.norm_case(cols, (2, 5), cols, dt, res, 'none', 'layer', 'none', 'none', 1.0)
+  norm = blocks.ResidualNorm(cols, post='none', pre='layer', w_pre=p['w_pre'].cuda(), b_pre=p['b_pre'].cuda())
+  z = torch.empty(2, 5, cols, dtype=T.DT[dt], device='cuda')
+  r, z, stats = norm.forward(None, t['x'].cuda(), z=z, save=True)
+  w = T.f64({**t, **p})
+  want = O.residual_norm(None, w['x'], pre='layer', w_pre=w['w_pre'], b_pre=w['b_pre'])
+  m1, s1 = (want['stats'].reshape(2, 5, 4)[..., i:i + 1] for i in (2, 3))
+  rb = w['x'].abs().amax(-1, keepdim=True)
+  T.off(z, want['z'], ((rb + m1.abs()) * s1 * w['w_pre'].abs() + w['b_pre'].abs()) * (1 + rb * s1), 256, 'z')
+  g = norm.backward(t['dz'].cuda(), t['dr'].cuda(), None, r, stats)
+  ref, size = O.residual_norm_backward(w['dz'], w['dr'], None, w['x'], stats.cpu().double(), pre='layer', w_pre=w['w_pre'], b_pre=w['b_pre'])
+  T.off(g.dx, ref['dx'], size['dx'], 256, 'dx')
+  for name in ('dw_pre', 'db_pre'):
+    T.off(getattr(g, name), ref[name], size[name], 10 + 416, name)
