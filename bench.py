@@ -26,7 +26,7 @@ Extra objects on the JSON line:
                 algorithmic flops / measured time against the roof of the pipe the kernel runs on: dense fp32
                 MFMA (157.3 TFLOP/s), or, for the split-bf16 kernels, dense bf16 MFMA / 6 partial products
                 (416.7 TFLOP/s algorithmic).  `traffic` = L2-miss bytes per launch of that kernel from the
-                committed rocprofv3 counter passes of this same command (the newest profiles/rNN_traffic.json; FETCH_SIZE
+                committed rocprofv3 counter passes of this same command (profiles/traffic.json; FETCH_SIZE
                 doubled per the gfx950 correction + WRITE_SIZE), null when not recorded for this workload.  The operand-image
                 passes (amax_kernel + pair_image_kernel) that precede an image-based GEMM are launched and timed on their
                 own during the instrumented steps (`operand_images(...)` in `kernels`); the small weight-image kernels
@@ -69,14 +69,7 @@ H3_PEAK_TFLOPS = BF16_MFMA_PEAK_TFLOPS / 3.0
 HBM_PEAK_GBS = 8000.0           # ibid., HBM3E peak BW
 CLIP_FRAMES = 256
 CLIP_SAMPLES = (CLIP_FRAMES - 1) * 256 + 1024   # 66304
-def _latest_traffic_json():
-  """profiles/rNN_traffic.json of the highest round (tools/run_gpu_prof_r04.sh writes it next to the other summaries)."""
-  import glob
-  found = sorted(glob.glob(os.path.join(ROOT, 'profiles', 'r[0-9][0-9]_traffic.json')))
-  return found[-1] if found else os.path.join(ROOT, 'profiles', 'r03_traffic.json')
-
-
-TRAFFIC_JSON = _latest_traffic_json()
+TRAFFIC_JSON = os.path.join(ROOT, 'profiles', 'traffic.json')      # tools/run_gpu_traffic.sh, on the kernel sources that it names
 
 
 def synth_waveforms(batch, seed, device):
